@@ -23,29 +23,32 @@ class LLM:
     sequence's count rounded up to a multiple of 64.  ``max_seq`` (the reference's name for
     the per-sequence capacity) is a shorthand: with ``max_batch`` it gives
     ``max_tokens = max_batch * max_seq``.
+
+    ``kv_dtype="fp8"`` holds keys and values in eight bits (e4m3 codes and a power of two per head and token): half the cache of
+    bfloat16, and half the bytes that a step reads of it.  Models whose keys belong to other mixers than ``Attention`` refuse it.
     """
 
     def __init__(self, model_dir: str, compute_dtype="bf16", device: str = "cuda:0",
                  max_tokens: Optional[int] = None, max_seq: Optional[int] = None, max_batch: int = 8,
-                 graph: bool = True, source=None, nvtx: bool = False):
+                 graph: bool = True, source=None, nvtx: bool = False, kv_dtype: Optional[str] = None):
         self._setup(load_model(model_dir, dtype=compute_dtype, device=device, source=source),
-                    max_tokens, max_seq, max_batch, graph, nvtx)
+                    max_tokens, max_seq, max_batch, graph, nvtx, kv_dtype)
 
     @classmethod
     def from_model(cls, model, max_tokens: Optional[int] = None, max_seq: Optional[int] = None,
-                   max_batch: int = 8, graph: bool = True, nvtx: bool = False) -> "LLM":
+                   max_batch: int = 8, graph: bool = True, nvtx: bool = False, kv_dtype: Optional[str] = None) -> "LLM":
         """An ``LLM`` around a model that already has its weights bound (``DecoderModel.load``)."""
         self = cls.__new__(cls)
-        self._setup(model, max_tokens, max_seq, max_batch, graph, nvtx)
+        self._setup(model, max_tokens, max_seq, max_batch, graph, nvtx, kv_dtype)
         return self
 
-    def _setup(self, model, max_tokens, max_seq, max_batch, graph, nvtx=False) -> None:
+    def _setup(self, model, max_tokens, max_seq, max_batch, graph, nvtx=False, kv_dtype=None) -> None:
         self.model = model
         cfg = self.model.config
         if max_tokens is None:
             per_seq = max_seq or getattr(cfg, "max_position_embeddings", None) or 4096
             max_tokens = max_batch * per_seq
-        self.engine = Engine(self.model, max_tokens=max_tokens, use_graphs=graph, nvtx=nvtx)
+        self.engine = Engine(self.model, max_tokens=max_tokens, use_graphs=graph, nvtx=nvtx, kv_dtype=kv_dtype)
         self.last_stats: Optional[GenerationStats] = None
 
     @property
@@ -199,10 +202,10 @@ def load_llm(model_dir: str, **kw) -> LLM:
 
 
 def generate(model_dir: str, prompts: Sequence[Sequence[int]], compute_dtype="bf16", device="cuda:0",
-             max_tokens: Optional[int] = None, **gen_kw) -> List[List[int]]:
+             max_tokens: Optional[int] = None, kv_dtype: Optional[str] = None, **gen_kw) -> List[List[int]]:
     """One-shot: load ``model_dir`` and generate for ``prompts`` (lists of token ids)."""
     if max_tokens is None:
         new = gen_kw.get("max_new_tokens", 64)
         max_tokens = sum(((len(p) + new + 63) // 64) * 64 for p in prompts)
-    return LLM(model_dir, compute_dtype=compute_dtype, device=device, max_tokens=max_tokens).generate(
+    return LLM(model_dir, compute_dtype=compute_dtype, device=device, max_tokens=max_tokens, kv_dtype=kv_dtype).generate(
         prompts, **gen_kw)

@@ -15,6 +15,8 @@ each group storage of its own:
   once every key in it lies before the chunk the sequence has reached.
   ``keys_only`` says that the mixer reads its values out of the key rows (a
   latent from which keys and values are both made): no storage for V.
+  ``eight_bit`` says that the mixer can work on keys and values held in eight bits
+  (``Cache(kv_dtype="fp8")``): uint8 codes and exponents as ``ops.KV8Pages`` describes them.
 * ``StateRequest(shape, dtype)``: state of fixed size per sequence,
   ``[max_seqs + 1, *shape]`` per entry, zeroed when a slot is opened.  The last
   row belongs to no sequence (``Cache.spare_slot``): rows that pad a step up to
@@ -38,7 +40,10 @@ from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 
+from ..ops.kv8 import KV8Pages, kv8_shapes
 from .pages import PAGE_TOKENS, PagePool, SequenceSlots, pages_for
+
+KV_DTYPES = (None, "fp8")
 
 
 @dataclasses.dataclass(frozen=True)
@@ -49,6 +54,7 @@ class KVRequest:
     v_head_dim: Optional[int] = None
     chunk: Optional[int] = None
     keys_only: bool = False
+    eight_bit: bool = dataclasses.field(default=False, compare=False)
 
     @property
     def value_dim(self) -> int:
@@ -73,22 +79,29 @@ CacheRequest = Union[KVRequest, StateRequest, BundleRequest, None]
 
 class KVView:
     """What an attention-like mixer sees of its cache entry."""
-    __slots__ = ("k", "v", "group", "window")
+    __slots__ = ("k", "v", "group", "window", "pages8")
 
-    def __init__(self, k: torch.Tensor, v: torch.Tensor, group: int, window: Optional[int]):
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, group: int, window: Optional[int], exps=None):
         self.k = k          # [n_pages, n_kv_heads, PAGE_TOKENS, head_dim]
         self.v = v          # [n_pages, n_kv_heads, PAGE_TOKENS, value_dim]
         self.group = group  # index of the block table to use (StepContext.block_tables[group])
         self.window = window
+        # a cache in eight bits: the codes k, v with their exponents (None: k and v are numbers of the compute dtype)
+        self.pages8 = None if exps is None else KV8Pages(k, v, *exps)
 
 
 class Cache:
     """All cache storage of one model on one device, with its slot bookkeeping."""
 
     def __init__(self, requests: Sequence[CacheRequest], *, max_tokens: int,
-                 max_seqs: Optional[int], dtype: torch.dtype, device):
+                 max_seqs: Optional[int], dtype: torch.dtype, device, kv_dtype: Optional[str] = None):
+        """``kv_dtype="fp8"``: keys and values in eight bits (e4m3 codes with a power of two per head and token) instead of
+        ``dtype``; every mixer with keys has to take that."""
+        if kv_dtype not in KV_DTYPES:
+            raise ValueError(f"unknown kv_dtype {kv_dtype!r}: use fp8, or None for the compute dtype")
         self.device = torch.device(device)
         self.dtype = dtype
+        self.kv_dtype = kv_dtype
         # page 0 of every group is never handed out: rows that pad a batch up to a captured
         # graph's size write there, and released or unused block-table entries point there
         self.n_pages = max(1, pages_for(max_tokens)) + 1
@@ -127,12 +140,22 @@ class Cache:
 
         for r in requests:
             self._entry.append(place(r))
+        if kv_dtype is not None and not (kv_keys and all(r.eight_bit for r in kv_keys)):
+            raise ValueError("kv_dtype='fp8': the model has " + ("layers whose keys cannot be held in eight bits" if kv_keys else "no keys"))
         self.kv_groups = kv_keys
         self.state_groups = st_keys
 
         self._k: List[torch.Tensor] = []
         self._v: List[torch.Tensor] = []
+        self._exps: List[Optional[Tuple[torch.Tensor, torch.Tensor]]] = []
         for r, n in zip(kv_keys, kv_counts):
+            if kv_dtype is not None:
+                *codes, exp = kv8_shapes(self.n_pages, r.n_kv_heads, r.head_dim)
+                for to, s in zip((self._k, self._v), codes):
+                    to.append(torch.zeros((n,) + s, dtype=torch.uint8, device=self.device))
+                self._exps.append(tuple(torch.zeros((n,) + exp, dtype=torch.uint8, device=self.device) for _ in range(2)))
+                continue
+            self._exps.append(None)
             shape = (n, self.n_pages, r.n_kv_heads, PAGE_TOKENS)
             self._k.append(torch.zeros(shape + (r.head_dim,), dtype=dtype, device=self.device))
             self._v.append(torch.zeros(shape + (r.value_dim,), dtype=dtype, device=self.device))
@@ -154,7 +177,8 @@ class Cache:
     def kv_bytes_per_token(self) -> int:
         """Bytes of keys and values one cached token takes over all layers (the reference's figure of that name,
         crates/synaptix-models/llm/common/src/model.rs:932-954): 147,456 for the Qwen3-4B shape in bfloat16."""
-        return sum(t.shape[0] * t.shape[2] * t.shape[4] * t.element_size() for t in self._k + self._v)
+        exps = [t for both in self._exps if both is not None for t in both]
+        return sum(t.numel() // (self.n_pages * PAGE_TOKENS) * t.element_size() for t in self._k + self._v + exps)
 
     # -- views ------------------------------------------------------------
     @property
@@ -176,11 +200,13 @@ class Cache:
             return tuple(self._view_of(i) for i in e)
         kind, g, i = e
         if kind == "kv":
-            return KVView(self._k[g][i], self._v[g][i], g, self.kv_groups[g].window)
+            exps = self._exps[g]
+            return KVView(self._k[g][i], self._v[g][i], g, self.kv_groups[g].window, None if exps is None else (exps[0][i], exps[1][i]))
         return self._state[g][i]
 
     def bytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in self._k + self._v + self._state)
+        exps = [t for both in self._exps if both is not None for t in both]
+        return sum(t.numel() * t.element_size() for t in self._k + self._v + exps + self._state)
 
     # -- slots --------------------------------------------------------------
     def open(self) -> int:

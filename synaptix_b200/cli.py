@@ -36,6 +36,15 @@ def _dtype_arg(s: str) -> str:
     return table[s.lower()]
 
 
+def _kv_dtype_arg(s: str):
+    """``--kv-dtype``, the reference's option: ``auto`` (the compute dtype) or eight bits."""
+    table = {"auto": None, "fp8": "fp8", "mxfp8": "fp8", "e4m3": "fp8"}
+    if s.lower() not in table:
+        raise SystemExit(f"unknown --kv-dtype {s!r}: use auto (the compute dtype) or fp8")
+    return table[s.lower()]
+
+
+_KV_HELP = "keys and values in the cache: auto (the compute dtype) or fp8 (eight bits, a power of two per head and token)"
 _ATTN = {"auto": None, "flash-decode": None, "flash_decode": None, "decode": None,
          "fa2": False, "flash2": False, "flash-attn-2": False, "fa4": True, "flash4": True, "flash-attn-4": True}
 _ATTN_HELP = ("attention backend, the reference's names (synaptix-core/src/backend/attn.rs:47-56): auto (default); "
@@ -80,6 +89,7 @@ def build_parser() -> argparse.ArgumentParser:
     run.add_argument("--max-seq", type=int, default=None,
                      help="cache capacity per sequence; default prompt + max-tokens")
     run.add_argument("--attn", default=None, help=_ATTN_HELP)
+    run.add_argument("--kv-dtype", default="auto", help=_KV_HELP)
     run.add_argument("--compute-dtype", default="bf16", help="bf16 or f32 (f32: everything in true 32-bit)")
     run.add_argument("--no-graph", action="store_true", help="do not replay decode steps as CUDA graphs")
     run.add_argument("--nvtx", action="store_true", help="name every step for a profiler's timeline (NVTX ranges)")
@@ -95,6 +105,7 @@ def build_parser() -> argparse.ArgumentParser:
     bench.add_argument("--warmup", type=int, default=3)
     bench.add_argument("--device", default="cuda")
     bench.add_argument("--attn", default=None, help=_ATTN_HELP)
+    bench.add_argument("--kv-dtype", default="auto", help=_KV_HELP)
     bench.add_argument("--dtype", default="bf16")
 
     ins = sub.add_parser("inspect", help="list the tensors of a safetensors file, or of a model folder with what its configuration says")
@@ -134,7 +145,7 @@ def cmd_run(a) -> int:
     max_tokens = sum(((min(per_seq, len(p) + a.max_tokens) + 63) // 64) * 64 for p in prompts)
     t0 = time.perf_counter()
     llm = LLM(a.model, compute_dtype=_dtype_arg(a.compute_dtype), device=_device(a.device),
-              max_tokens=max_tokens, graph=not a.no_graph, nvtx=a.nvtx)
+              max_tokens=max_tokens, graph=not a.no_graph, nvtx=a.nvtx, kv_dtype=_kv_dtype_arg(a.kv_dtype))
     load_s = time.perf_counter() - t0
     kw = dict(max_new_tokens=a.max_tokens, temperature=a.temperature, top_k=a.top_k, top_p=a.top_p,
               min_p=a.min_p, repetition_penalty=a.repetition_penalty, repeat_last_n=a.repeat_last_n,
@@ -228,7 +239,7 @@ def cmd_bench(a) -> int:
     n_prompt = a.prompt_tokens or 32
     B = a.batch_size
     llm = LLM(a.model, compute_dtype=_dtype_arg(a.dtype), device=_device(a.device),
-              max_tokens=B * (((n_prompt + a.n_tokens + 63) // 64) * 64))
+              max_tokens=B * (((n_prompt + a.n_tokens + 63) // 64) * 64), kv_dtype=_kv_dtype_arg(a.kv_dtype))
     vocab = llm.model.vocab_size
     # synthetic ids as the reference's perf tools make them (qwen3/examples/format_perf.rs:70,94)
     prompts = [[((i * 7 + 13 + b) % min(200, vocab - 5)) + 5 for i in range(n_prompt)] for b in range(B)]

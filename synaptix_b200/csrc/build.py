@@ -50,6 +50,7 @@ LIBRARIES: Dict[str, tuple] = {
     "mlstm": ("mlstm.cu", []),
     "delta": ("delta.cu", []),
     "latent": ("latent.cu", []),
+    "kv8": ("kv8.cu", []),
     "moe": ("moe.cu", []),
     "moe_tc": ("moe_tc.cu", []),
     "decode": ("decode.cu", []),

@@ -1,0 +1,404 @@
+// A cache of keys and values in eight bits: heads are prepared and quantised as they are written, pages are read back, and
+// single tokens attend over them whatever the head size, type and options (kv8.cuh says what the format is and why).
+#include "kv8.cuh"
+
+#define KV8_MAX_HD 256
+
+// ---------------------------------------------------------------------------------------
+// Head preparation with the write into the cache.  A block a token (and a share of its heads), a warp a head:
+//   q heads: x / rms(x) * gain (optional), rotate-half rotation of the first rotary_dim elements (optional), to q_out;
+//   k heads: the same, then quantised into the sequence's page;   v heads: quantised.
+// The rotation's angle is position * inv_freq in about 48 bits: the product rounded to 32 bits and what that left out, by which
+// sine and cosine are moved on.  (In 32 bits alone an angle at position 100,000 is off by up to 0.004.)
+// ---------------------------------------------------------------------------------------
+#define KV8_WARPS 8
+// cosine and sine of pos * f: the angle is hi + lo with |lo| <= 2^-24 |hi|, up to 2^-8 at position 131,072, so the series in lo needs its
+// second term (lo^2 / 2 = 8e-6 there) and not its third (1e-8)
+__device__ __forceinline__ float2 kv8_turn(int pos, float f) {
+  const float p = (float)pos, hi = p * f, lo = fmaf(p, f, -hi), q = -0.5f * lo * lo;
+  float sn, cs;
+  sincosf(hi, &sn, &cs);
+  return make_float2(fmaf(-lo, sn, fmaf(q, cs, cs)), fmaf(lo, cs, fmaf(q, sn, sn)));
+}
+template <typename T>
+__global__ void __launch_bounds__(KV8_WARPS * 32) kv8_prepare_kernel(
+    const T* __restrict__ qkv, T* __restrict__ q_out, uint8_t* __restrict__ k_pages, uint8_t* __restrict__ v_pages,
+    uint8_t* __restrict__ k_exp, uint8_t* __restrict__ v_exp, const float* __restrict__ wq, const float* __restrict__ wk,
+    const float* __restrict__ inv_freq, int rotary_dim, float eps, const int* __restrict__ positions,
+    const int* __restrict__ seq_of_token, const int* __restrict__ block_table, int maxp, int nh, int nkv, int hd, int n_pages,
+    int row) {
+  __shared__ float s_cs[KV8_MAX_HD / 2], s_sn[KV8_MAX_HD / 2];
+  __shared__ float s_x[KV8_WARPS][KV8_MAX_HD];
+  pdl_wait();
+  pdl_trigger();
+  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int pos = positions[t], half = inv_freq ? rotary_dim / 2 : 0;
+  for (int i = threadIdx.x; i < half; i += KV8_WARPS * 32) {
+    const float2 r = kv8_turn(pos, inv_freq[i]);
+    s_cs[i] = r.x;
+    s_sn[i] = r.y;
+  }
+  const int page = (unsigned)(pos >> 6) < (unsigned)maxp ? block_table[(size_t)seq_of_token[t] * maxp + (pos >> 6)] : -1;
+  const bool page_ok = k_pages && page >= 0 && page < n_pages;        // the host guarantees a page; never write outside
+  __syncthreads();
+  const int cb = kv8_block(hd), heads = k_pages ? nh + 2 * nkv : nh;
+  float* xs = s_x[warp];
+  for (int head = blockIdx.y * KV8_WARPS + warp; head < heads; head += gridDim.y * KV8_WARPS) {
+    const bool is_q = head < nh, is_k = !is_q && head < nh + nkv;
+    const T* src = qkv + (size_t)t * row + (size_t)head * hd;
+    const float* gain = is_q ? wq : is_k ? wk : nullptr;
+    __syncwarp();
+    float ss = 0.f;
+    for (int i = lane; i < hd; i += 32) {
+      const float x = to_f32(src[i]);
+      xs[i] = x;
+      ss += x * x;
+    }
+    const float inv = gain ? rsqrtf(warp_sum(ss) / (float)hd + eps) : 1.f;
+    __syncwarp();
+    float y[KV8_MAX_HD / 32];
+    float a = 0.f;
+    bool finite = true;
+#pragma unroll
+    for (int k = 0; k < KV8_MAX_HD / 32; ++k) {
+      const int i = lane + 32 * k;
+      y[k] = 0.f;
+      if (i < hd) {
+        float x = xs[i] * inv;
+        if (gain) x *= gain[i];
+        if ((is_q || is_k) && i < 2 * half) {
+          const int j = i < half ? i + half : i - half, p = i < half ? i : j;
+          float z = xs[j] * inv;
+          if (gain) z *= gain[j];
+          x = i < half ? x * s_cs[p] - z * s_sn[p] : x * s_cs[p] + z * s_sn[p];
+        }
+        y[k] = x;
+        a = fmaxf(a, fabsf(x));
+        finite = finite && fabsf(x) < INFINITY;                        // (false for NaN)
+      }
+    }
+    if (is_q) {
+      for (int k = 0; k < KV8_MAX_HD / 32; ++k)
+        if (lane + 32 * k < hd) q_out[((size_t)t * nh + head) * hd + lane + 32 * k] = from_f32<T>(y[k]);
+      continue;
+    }
+    const int e = kv8_exponent(warp_max(a), __all_sync(0xffffffffu, finite));
+    if (!page_ok) continue;
+    const float inverse = kv8_inverse(e);
+    const int kvh = is_k ? head - nh : head - nh - nkv, key = pos & (SX_PAGE - 1);
+    const size_t place = (size_t)page * nkv + kvh;
+    uint8_t* dst = (is_k ? k_pages : v_pages) + place * SX_PAGE * hd;
+#pragma unroll
+    for (int k = 0; k < KV8_MAX_HD / 32; ++k) {
+      const int i = lane + 32 * k;
+      if (i < hd) dst[is_k ? kv8_k_at(key, i, cb) : kv8_v_at(key, i)] = (uint8_t)kv8_codes2(kv8_scaled(y[k], inverse), 0.f);
+    }
+    if (lane == 0) (is_k ? k_exp : v_exp)[place * SX_PAGE + key] = (uint8_t)e;
+  }
+}
+
+// qkv: rows of `row` elements, q heads, k heads and v heads first (q heads alone where k_pages is null and nothing is written)
+extern "C" int sx_kv8_prepare(const void* qkv, void* q_out, void* k_pages, void* v_pages, void* k_exp, void* v_exp, const float* wq,
+                              const float* wk, const float* inv_freq, int rotary_dim, float eps, const int* positions,
+                              const int* seq_of_token, const int* block_table, int maxp, int n_tokens, int nh, int nkv, int hd,
+                              int n_pages, int row, int dt, cudaStream_t stream) {
+  if (n_tokens <= 0) return 0;
+  if (hd <= 0 || hd % 16 || hd > KV8_MAX_HD || rotary_dim < 0 || rotary_dim > hd || (rotary_dim & 1) || nh < 0 || nkv <= 0)
+    return SX_ERR_SIZE;
+  const int heads = nh + (k_pages ? 2 * nkv : 0), groups = (heads + KV8_WARPS - 1) / KV8_WARPS;
+  if (heads == 0) return 0;
+  // few tokens: a block for every eight heads; many: a block walks its token's heads and makes the angles once
+  const dim3 grid(n_tokens, n_tokens * groups <= 4 * sx_sm_count() ? groups : 1);
+  if (dt == SX_F32)
+    return sx_launch(kv8_prepare_kernel<float>, grid, dim3(KV8_WARPS * 32), 0, stream, (const float*)qkv, (float*)q_out, (uint8_t*)k_pages,
+                     (uint8_t*)v_pages, (uint8_t*)k_exp, (uint8_t*)v_exp, wq, wk, inv_freq, rotary_dim, eps, positions, seq_of_token,
+                     block_table, maxp, nh, nkv, hd, n_pages, row);
+  if (dt == SX_BF16)
+    return sx_launch(kv8_prepare_kernel<bf16>, grid, dim3(KV8_WARPS * 32), 0, stream, (const bf16*)qkv, (bf16*)q_out, (uint8_t*)k_pages,
+                     (uint8_t*)v_pages, (uint8_t*)k_exp, (uint8_t*)v_exp, wq, wk, inv_freq, rotary_dim, eps, positions, seq_of_token,
+                     block_table, maxp, nh, nkv, hd, n_pages, row);
+  return SX_ERR_DTYPE;
+}
+
+// ---------------------------------------------------------------------------------------
+// Pages read back: page i of the result holds page page_idx[i] of sequence page_seq[i] as [kv heads][64][hd] in T, rows
+// behind the sequence's end as zeros.  A block a (page, kv head) and keys or values; values turn around in shared memory.
+// ---------------------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(256) kv8_read_kernel(
+    const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages, const uint8_t* __restrict__ k_exp,
+    const uint8_t* __restrict__ v_exp, T* __restrict__ k_out, T* __restrict__ v_out, const int* __restrict__ page_seq,
+    const int* __restrict__ page_idx, const int* __restrict__ seq_lens, const int* __restrict__ block_table, int maxp, int nkv, int hd,
+    int n_pages) {
+  __shared__ uint8_t s_c[SX_PAGE][KV8_MAX_HD + 4];
+  __shared__ float s_f[SX_PAGE];
+  pdl_wait();
+  pdl_trigger();
+  const int i = blockIdx.x, kvh = blockIdx.y;
+  const bool is_k = blockIdx.z == 0;
+  const int s = page_seq[i], j = page_idx[i];
+  const int page = block_table[(size_t)s * maxp + j], held = min(SX_PAGE, max(0, seq_lens[s] - j * SX_PAGE));
+  const bool ok = page >= 0 && page < n_pages;
+  const size_t from = (size_t)(ok ? page : 0) * nkv + kvh;
+  const uint8_t* src = (is_k ? k_pages : v_pages) + from * SX_PAGE * hd;
+  T* dst = (is_k ? k_out : v_out) + ((size_t)i * nkv + kvh) * SX_PAGE * hd;
+  const int cb = kv8_block(hd);
+  if (threadIdx.x < SX_PAGE) s_f[threadIdx.x] = kv8_scale((is_k ? k_exp : v_exp)[from * SX_PAGE + threadIdx.x]);
+  for (int o = threadIdx.x * 16; o < SX_PAGE * hd; o += 256 * 16) {
+    const uint4 c = *reinterpret_cast<const uint4*>(src + o);
+    const uint8_t* b = reinterpret_cast<const uint8_t*>(&c);
+    for (int n = 0; n < 16; ++n) {
+      const int at = o + n;
+      if (is_k) s_c[at / cb % SX_PAGE][at / (cb * SX_PAGE) * cb + at % cb] = b[n];
+      else s_c[at % SX_PAGE][at / SX_PAGE] = b[n];
+    }
+  }
+  __syncthreads();
+  for (int o = threadIdx.x; o < SX_PAGE * hd; o += 256) {
+    const int key = o / hd;
+    dst[o] = from_f32<T>(ok && key < held ? kv8_float2(s_c[key][o % hd]).x * s_f[key] : 0.f);
+  }
+}
+
+extern "C" int sx_kv8_read(const void* k_pages, const void* v_pages, const void* k_exp, const void* v_exp, void* k_out, void* v_out,
+                           const int* page_seq, const int* page_idx, int n_out, const int* seq_lens, const int* block_table, int maxp,
+                           int nkv, int hd, int n_pages, int dt, cudaStream_t stream) {
+  if (n_out <= 0) return 0;
+  if (hd <= 0 || hd % 16 || hd > KV8_MAX_HD || nkv <= 0 || nkv > 65535) return SX_ERR_SIZE;
+  if (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) return SX_ERR_ALIGN;
+  const dim3 grid(n_out, nkv, 2);
+  if (dt == SX_F32)
+    return sx_launch(kv8_read_kernel<float>, grid, dim3(256), 0, stream, (const uint8_t*)k_pages, (const uint8_t*)v_pages, (const uint8_t*)k_exp,
+                     (const uint8_t*)v_exp, (float*)k_out, (float*)v_out, page_seq, page_idx, seq_lens, block_table, maxp, nkv, hd, n_pages);
+  if (dt == SX_BF16)
+    return sx_launch(kv8_read_kernel<bf16>, grid, dim3(256), 0, stream, (const uint8_t*)k_pages, (const uint8_t*)v_pages, (const uint8_t*)k_exp,
+                     (const uint8_t*)v_exp, (bf16*)k_out, (bf16*)v_out, page_seq, page_idx, seq_lens, block_table, maxp, nkv, hd, n_pages);
+  return SX_ERR_DTYPE;
+}
+
+// ---------------------------------------------------------------------------------------
+// Attention of single tokens over the pages: every head size, type and option.
+//
+// A block serves up to four query heads of a kv head (a group of more takes several blocks) over a share of the sequence's
+// visible pages; its warps take the share's pages in turn, each with a softmax of its own (running maximum and sum), joined in
+// shared memory at the end.  In a page a lane has two keys in the scores (a key's codes are 16-byte loads, queries come from
+// shared memory and serve all lanes) and hd / 32 dims in p v (a dim's 64 keys are four loads).  All sums in 32 bits by FFMA.
+// ---------------------------------------------------------------------------------------
+#define KV8_HEADS 4
+struct Kv8Rows {
+  const uint8_t *k, *v, *ke, *ve;
+  const int *seq_lens, *block_table;
+  const float* sinks;
+  float *part_o, *part_ml;
+  int maxp, n_pages, nh, nkv, hd, window, chunk, n_splits, out_stride;
+  float scale, softcap, out_scale;
+};
+
+template <typename T, int NI>
+__global__ void __launch_bounds__(KV8_WARPS * 32) kv8_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const Kv8Rows a) {
+  extern __shared__ float4 smem4[];
+  float* q_s = reinterpret_cast<float*>(smem4);                              // [KV8_HEADS][hd]
+  const int hd = a.hd, G = a.nh / a.nkv, per_kv = (G + KV8_HEADS - 1) / KV8_HEADS;
+  float* p_s = q_s + KV8_HEADS * hd;                                         // [KV8_WARPS][KV8_HEADS][64]
+  float* o_s = p_s + KV8_WARPS * KV8_HEADS * SX_PAGE;                        // [KV8_WARPS][KV8_HEADS][hd]
+  __shared__ float s_m[KV8_WARPS][KV8_HEADS], s_l[KV8_WARPS][KV8_HEADS], s_r[KV8_HEADS];
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = blockIdx.x, kvh = blockIdx.y / per_kv, g0 = (blockIdx.y % per_kv) * KV8_HEADS, seq = blockIdx.z;
+  const int gn = min(KV8_HEADS, G - g0), h0 = kvh * G + g0;
+  const int len = a.seq_lens[seq], pos = len - 1;
+  int lo = a.window > 0 ? max(0, len - a.window) : 0;
+  if (a.chunk > 0 && pos >= 0) lo = max(lo, pos / a.chunk * a.chunk);
+  const int p_first = lo >> 6, p_end = min((len + 63) >> 6, a.maxp);
+  const int per = (max(0, p_end - p_first) + a.n_splits - 1) / a.n_splits;
+  const int p0 = p_first + split * per, p1 = min(p_end, p0 + per);
+  // queries, each row scaled by a power of two to a largest magnitude of 1 to 2, so that no sum of products with codes leaves the range
+  for (int g = warp; g < KV8_HEADS; g += KV8_WARPS) {
+    const T* src = q + ((size_t)seq * a.nh + h0 + g) * hd;
+    float top = 0.f;
+    bool finite = true;
+    for (int i = lane; g < gn && i < hd; i += 32) {
+      const float x = to_f32(src[i]);
+      top = fmaxf(top, fabsf(x));
+      finite = finite && fabsf(x) < INFINITY;
+    }
+    finite = __all_sync(0xffffffffu, finite);
+    const int x = min(max(__float_as_int(warp_max(top)) >> 23, 1), 253);
+    const float down = __int_as_float((254 - x) << 23);
+    for (int i = lane; i < hd; i += 32) q_s[g * hd + i] = g < gn ? to_f32(src[i]) * down : 0.f;
+    if (lane == 0) s_r[g] = finite ? __int_as_float(x << 23) * a.scale : __int_as_float(0x7fffffff);
+  }
+  __syncthreads();
+  const int cb = kv8_block(hd);
+  float m[KV8_HEADS], l[KV8_HEADS], o[KV8_HEADS][NI];
+#pragma unroll
+  for (int g = 0; g < KV8_HEADS; ++g) {
+    m[g] = -INFINITY;
+    l[g] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) o[g][i] = 0.f;
+  }
+  float* pw = p_s + warp * KV8_HEADS * SX_PAGE;
+  for (int p = p0 + warp; p < p1; p += KV8_WARPS) {
+    const int page = a.block_table[(size_t)seq * a.maxp + p];
+    if (page < 0 || page >= a.n_pages) continue;
+    const size_t place = (size_t)page * a.nkv + kvh;
+    const uint8_t* kp = a.k + place * SX_PAGE * hd;
+    const uint8_t* vp = a.v + place * SX_PAGE * hd;
+    const int v0 = max(0, lo - p * SX_PAGE), v1 = min(SX_PAGE, len - p * SX_PAGE);     // visible keys of the page
+    float s[2][KV8_HEADS];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int key = lane + 32 * h;
+#pragma unroll
+      for (int g = 0; g < KV8_HEADS; ++g) s[h][g] = 0.f;
+      for (int d = 0; d < hd; d += 16) {
+        float x[16];
+        kv8_float16(*reinterpret_cast<const uint4*>(kp + kv8_k_at(key, d, cb)), x);
+#pragma unroll
+        for (int g = 0; g < KV8_HEADS; ++g)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4 y = *reinterpret_cast<const float4*>(q_s + g * hd + d + 4 * i);
+            s[h][g] = fmaf(y.x, x[4 * i], fmaf(y.y, x[4 * i + 1], fmaf(y.z, x[4 * i + 2], fmaf(y.w, x[4 * i + 3], s[h][g]))));
+          }
+      }
+    }
+    const float kf[2] = {kv8_scale(a.ke[place * SX_PAGE + lane]), kv8_scale(a.ke[place * SX_PAGE + lane + 32])};
+    const float vf[2] = {kv8_scale(a.ve[place * SX_PAGE + lane]), kv8_scale(a.ve[place * SX_PAGE + lane + 32])};
+    __syncwarp();
+#pragma unroll
+    for (int g = 0; g < KV8_HEADS; ++g) {
+      float top = m[g];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int key = lane + 32 * h;
+        float z = s[h][g] * kf[h] * s_r[g];
+        if (a.softcap > 0.f) z = a.softcap * tanhf(z / a.softcap);
+        s[h][g] = key >= v0 && key < v1 ? z : -INFINITY;
+        top = fmaxf(top, s[h][g]);
+      }
+      top = warp_max(top);
+      const float base = top == -INFINITY ? 0.f : top, shrink = expf(m[g] - base);
+      m[g] = top;
+      float sum = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int key = lane + 32 * h;
+        const float w = expf(s[h][g] - base);
+        sum += w;
+        pw[g * SX_PAGE + key] = key >= v0 && key < v1 ? w * vf[h] : 0.f;
+      }
+      l[g] = l[g] * shrink + warp_sum(sum);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) o[g][i] *= shrink;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int d = lane + 32 * i;
+      if (d >= hd) continue;
+#pragma unroll
+      for (int c = 0; c < SX_PAGE; c += 16) {
+        float x[16];
+        kv8_float16(*reinterpret_cast<const uint4*>(vp + kv8_v_at(c, d)), x);
+        if (c < v0 || c + 16 > v1) {                                 // codes of keys that are not seen may be anything
+#pragma unroll
+          for (int n = 0; n < 16; ++n)
+            if (c + n < v0 || c + n >= v1) x[n] = 0.f;
+        }
+#pragma unroll
+        for (int g = 0; g < KV8_HEADS; ++g)
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const float4 w = *reinterpret_cast<const float4*>(pw + g * SX_PAGE + c + 4 * n);
+            o[g][i] = fmaf(w.x, x[4 * n], fmaf(w.y, x[4 * n + 1], fmaf(w.z, x[4 * n + 2], fmaf(w.w, x[4 * n + 3], o[g][i]))));
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < KV8_HEADS; ++g) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      if (lane + 32 * i < hd) o_s[(warp * KV8_HEADS + g) * hd + lane + 32 * i] = o[g][i];
+    if (lane == 0) {
+      s_m[warp][g] = m[g];
+      s_l[warp][g] = l[g];
+    }
+  }
+  __syncthreads();
+  for (int n = threadIdx.x; n < gn * hd; n += KV8_WARPS * 32) {
+    const int g = n / hd, d = n % hd, head = h0 + g;
+    float M = -INFINITY;
+    for (int w = 0; w < KV8_WARPS; ++w) M = fmaxf(M, s_m[w][g]);
+    const bool last = a.n_splits == 1;
+    const bool sink = last && a.sinks;
+    if (sink) M = fmaxf(M, a.sinks[head]);
+    const float base = M == -INFINITY ? 0.f : M;
+    float L = sink ? expf(a.sinks[head] - base) : 0.f, O = 0.f;
+    for (int w = 0; w < KV8_WARPS; ++w) {
+      const float f = expf(s_m[w][g] - base);
+      L += s_l[w][g] * f;
+      O += o_s[(w * KV8_HEADS + g) * hd + d] * f;
+    }
+    const size_t r = (size_t)seq * a.nh + head;
+    if (last) {
+      out[(size_t)seq * a.out_stride + head * hd + d] = from_f32<T>(L == 0.f ? 0.f : O / L * a.out_scale);
+    } else {
+      a.part_o[(r * a.n_splits + split) * hd + d] = O;
+      if (d == 0) reinterpret_cast<float2*>(a.part_ml)[r * a.n_splits + split] = make_float2(M, L);
+    }
+  }
+}
+
+// the shares of a row joined: a block a (sequence, head), a thread a dim
+template <typename T>
+__global__ void kv8_rows_merge_kernel(T* __restrict__ out, const Kv8Rows a) {
+  pdl_wait();
+  pdl_trigger();
+  const int seq = blockIdx.x / a.nh, head = blockIdx.x % a.nh, d = threadIdx.x;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)blockIdx.x * a.n_splits;
+  const float* po = a.part_o + (size_t)blockIdx.x * a.n_splits * a.hd + d;
+  float M = a.sinks ? a.sinks[head] : -INFINITY;
+  for (int i = 0; i < a.n_splits; ++i) M = fmaxf(M, ml[i].x);
+  const float base = M == -INFINITY ? 0.f : M;
+  float L = a.sinks ? expf(a.sinks[head] - base) : 0.f, O = 0.f;
+  for (int i = 0; i < a.n_splits; ++i) {
+    const float f = expf(ml[i].x - base);
+    L += ml[i].y * f;
+    O += po[(size_t)i * a.hd] * f;
+  }
+  out[(size_t)seq * a.out_stride + head * a.hd + d] = from_f32<T>(L == 0.f ? 0.f : O / L * a.out_scale);
+}
+
+template <typename T>
+static int kv8_rows_launch(const void* q, void* out, int S, const Kv8Rows& a, cudaStream_t stream) {
+  const int G = a.nh / a.nkv, per_kv = (G + KV8_HEADS - 1) / KV8_HEADS;
+  const dim3 grid(a.n_splits, a.nkv * per_kv, S), block(KV8_WARPS * 32);
+  const size_t smem = (size_t)(KV8_HEADS * a.hd + KV8_WARPS * KV8_HEADS * (SX_PAGE + a.hd)) * sizeof(float);
+  int rc;
+  if (a.hd <= 32) rc = sx_launch(kv8_rows_kernel<T, 1>, grid, block, smem, stream, (const T*)q, (T*)out, a);
+  else if (a.hd <= 64) rc = sx_launch(kv8_rows_kernel<T, 2>, grid, block, smem, stream, (const T*)q, (T*)out, a);
+  else if (a.hd <= 128) rc = sx_launch(kv8_rows_kernel<T, 4>, grid, block, smem, stream, (const T*)q, (T*)out, a);
+  else rc = sx_launch(kv8_rows_kernel<T, 8>, grid, block, smem, stream, (const T*)q, (T*)out, a);
+  if (rc || a.n_splits == 1) return rc;
+  return sx_launch(kv8_rows_merge_kernel<T>, dim3(S * a.nh), dim3(a.hd), 0, stream, (T*)out, a);
+}
+
+extern "C" int sx_kv8_rows(const void* q, void* out, const void* k, const void* v, const void* k_exp, const void* v_exp, const int* seq_lens,
+                           const int* block_table, int maxp, int S, int nh, int nkv, int hd, int n_pages, float scale, int window,
+                           float softcap, const float* sinks, int chunk, int out_stride, float out_scale, int n_splits, float* part_o,
+                           float* part_ml, int dt, cudaStream_t stream) {
+  if (S <= 0) return 0;
+  if (hd <= 0 || hd % 16 || hd > KV8_MAX_HD || nkv <= 0 || nh <= 0 || nh % nkv || n_splits < 1 || S > 65535 ||
+      (long long)nkv * ((nh / nkv + KV8_HEADS - 1) / KV8_HEADS) > 65535 || (n_splits > 1 && (!part_o || !part_ml)))
+    return SX_ERR_SIZE;
+  if (((uintptr_t)k | (uintptr_t)v) & 15) return SX_ERR_ALIGN;
+  const Kv8Rows a = {(const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)k_exp, (const uint8_t*)v_exp, seq_lens, block_table, sinks, part_o,
+                     part_ml, maxp, n_pages, nh, nkv, hd, window, chunk, n_splits, out_stride, scale, softcap, out_scale};
+  if (dt == SX_F32) return kv8_rows_launch<float>(q, out, S, a, stream);
+  if (dt == SX_BF16) return kv8_rows_launch<bf16>(q, out, S, a, stream);
+  return SX_ERR_DTYPE;
+}

@@ -242,8 +242,9 @@ class Engine:
     """A loaded model with its cache: slots are opened, stepped and closed here."""
 
     def __init__(self, model, *, max_tokens: int, max_seqs: Optional[int] = None, use_graphs: bool = True,
-                 nvtx: bool = False):
-        """``nvtx``: name every step for a profiler's timeline (NVTX ranges ``prompt step`` / ``decode step`` with
+                 nvtx: bool = False, kv_dtype: Optional[str] = None):
+        """``kv_dtype="fp8"``: keys and values in eight bits (see ``Cache``), half the bytes of bfloat16; ``None``: in the compute dtype.
+        ``nvtx``: name every step for a profiler's timeline (NVTX ranges ``prompt step`` / ``decode step`` with
         the number of sequences and tokens), as the reference's telemetry does
         (crates/synaptix-runtime/src/telemetry/nvtx.rs); off by default, it costs two calls a step."""
         if model.runtime is None:
@@ -256,7 +257,7 @@ class Engine:
         self.runtime = rt
         self.device = rt.device
         self.cache = Cache(model.cache_requests(), max_tokens=max_tokens, max_seqs=max_seqs,
-                           dtype=rt.dtype, device=rt.device)
+                           dtype=rt.dtype, device=rt.device, kv_dtype=kv_dtype)
         self._staging = _Staging(rt.device)
         self.use_graphs = bool(use_graphs) and model.all_graph_safe()
         self.nvtx = bool(nvtx)

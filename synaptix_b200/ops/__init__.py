@@ -34,6 +34,7 @@ from .convqk import convqk_prepare, sigmoid_gate
 from .scored import attn_scored as attn_scored_all_heads, heads_prepare
 from .latent import (head_gate, latent_attention, latent_expand, latent_gather, latent_output, latent_prepare, latent_query,
                      latent_rotate_q)
+from .kv8 import KV8Pages, kv8_attention, kv8_prepare, kv8_read, kv8_shapes, kv8_supported
 from .mlstm import mlstm
 from .moe import ExpertPlan, moe_combine, moe_down, moe_gate_up, moe_route, moe_sort, moe_up
 
@@ -44,7 +45,8 @@ __all__ = ["OPTIONS", "KernelOptions", "options", "set_options", "KernelsUnavail
            "add_rmsnorm_conv", "capped_glu", "mingru", "retention", "stream_add", "gate_activation",
            "add_normed", "WeightedRows", "embed_bigram", "convqk_prepare", "sigmoid_gate", "add_scaled", "add_scaled_rmsnorm", "scale_rows", "add_layernorm", "attn_scored", "heads_prepare", "latent_attention", "latent_output", "latent_prepare",
            "latent_query", "latent_gather", "latent_expand", "latent_rotate_q", "head_gate", "mlstm", "ExpertPlan", "moe_combine", "moe_down", "moe_gate_up", "moe_route", "moe_sort", "moe_up",
-           "add_dyn_tanh", "linear_into_dyn_tanh", "late_launch", "recording", "side_gate", "decode_layers", "decode_layers_words", "DECODE_LAYERS_MAX_ROWS", "DeltaWeights", "delta_rule", "delta_step_fits"]
+           "add_dyn_tanh", "linear_into_dyn_tanh", "late_launch", "recording", "side_gate", "decode_layers", "decode_layers_words", "DECODE_LAYERS_MAX_ROWS", "DeltaWeights", "delta_rule", "delta_step_fits",
+           "KV8Pages", "kv8_attention", "kv8_prepare", "kv8_read", "kv8_shapes", "kv8_supported"]
 
 
 _STATUS_READERS = {"gemm_tc": ("the tcgen05 matrix product (gemm_tc)", "gemm_tc_status"),

@@ -22,6 +22,8 @@ score for all heads in place of learned ones (0: ``exp(s_j) / (1 + sum exp(s_k))
 ``bias_suffix``: q, k and v have biases, added in the projection.  ``own_kv=False``:
 the layer has no keys and values of its own; the schedule gives it the cache entry of
 the layer whose (rotated) keys and values it reads, ``LayerRun(..., write_cache=False)``.
+Keys and values of one size may also be held in eight bits (``Cache(kv_dtype="fp8")``):
+``ops.kv8_prepare`` then quantises them as it writes them and ``ops.kv8_attention`` reads them.
 
 A rotation of part of the head (``rotary_dim < head_dim``) runs as a rotation of the
 whole head: scores do not change when the elements of queries and keys are put into
@@ -175,13 +177,28 @@ class Attention(Mixer):
     def cache_request(self):
         if not self.own_kv:
             return None
-        return KVRequest(self.nkv, self.hd, self.window, None if self.vd == self.hd else self.vd, self.chunk)
+        return KVRequest(self.nkv, self.hd, self.window, None if self.vd == self.hd else self.vd, self.chunk,
+                         eight_bit=ops.kv8_supported(self.hd, self.vd))
+
+    def _mix8(self, proj: torch.Tensor, col: int, ctx: StepContext, cache_view: KVView, write_cache: bool, **where) -> torch.Tensor:
+        """``mix`` over a cache in eight bits."""
+        T = proj.shape[0]
+        inv_freq, rotary_dim = self._rotation()
+        bt = ctx.block_tables[cache_view.group]
+        q = torch.empty((T, self.nh * self.hd), dtype=proj.dtype, device=proj.device)
+        ops.kv8_prepare(proj, q, cache_view.pages8 if write_cache else None, self.wq, self.wk, inv_freq, rotary_dim,
+                        self.qk_norm_eps if self.qk_norm_eps is not None else 0.0, ctx.positions, ctx.seq_of_token, bt, self.nh, self.nkv,
+                        self.hd, col=col)
+        return ops.kv8_attention(q, cache_view.pages8, ctx, bt, self.nh, self.nkv, self.hd, self.scale, self.window, softcap=self.softcap,
+                                 sinks=self.sinks, chunk=self.chunk, **where)
 
     def mix(self, proj: torch.Tensor, col: int, ctx: StepContext, cache_view: KVView, write_cache: bool = True,
             out: Optional[torch.Tensor] = None, out_col: int = 0, out_scale: float = 1.0) -> torch.Tensor:
         """Head preparation, cache write and attention from a projection ``proj [T, row]`` whose columns from ``col``
         on are this part's q, k and v heads; what the output projection reads goes, times ``out_scale``, into the
         columns of ``out`` from ``out_col`` on (default: a new ``[T, nh * vd]``)."""
+        if cache_view.pages8 is not None:
+            return self._mix8(proj, col, ctx, cache_view, write_cache, out=out, out_col=out_col, out_scale=out_scale)
         T = proj.shape[0]
         inv_freq, rotary_dim = self._rotation()
         bt = ctx.block_tables[cache_view.group]
@@ -199,7 +216,7 @@ class Attention(Mixer):
         if write_cache and not self.own_kv:
             raise ValueError("an attention layer without keys of its own writes no cache")
         out = self.o.deferred if defer_output else self.o.forward
-        if not self.is_plain:
+        if not self.is_plain or cache_view.pages8 is not None:
             return out(self.mix(self.qkv.forward(x), 0, ctx, cache_view, write_cache))
         T = x.shape[0]
         inv_freq, rotary_dim = self._rotation()
