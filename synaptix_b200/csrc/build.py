@@ -51,6 +51,7 @@ LIBRARIES: Dict[str, tuple] = {
     "delta": ("delta.cu", []),
     "latent": ("latent.cu", []),
     "kv8": ("kv8.cu", []),
+    "kv8_decode": ("kv8_decode.cu", []),
     "moe": ("moe.cu", []),
     "moe_tc": ("moe_tc.cu", []),
     "decode": ("decode.cu", []),

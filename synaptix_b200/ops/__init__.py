@@ -54,6 +54,7 @@ _STATUS_READERS = {"gemm_tc": ("the tcgen05 matrix product (gemm_tc)", "gemm_tc_
                    "attn_decode": ("the TMA-fed decode attention (attn_decode)", "attn_decode_status"),
                    "gemm_ws": ("the weight-streaming tcgen05 product (gemm_ws)", "gemm_ws_status"),
                    "moe_tc": ("the experts' grouped tcgen05 product (moe_tc)", "moe_tc_status"),
+                   "kv8_decode": ("the attention of single tokens over a cache in eight bits (kv8_decode)", "kv8_decode_status"),
                    "layers": ("the layers of a single-token step in one kernel (layers)", "decode_layers_status")}
 
 
@@ -69,10 +70,11 @@ def check_status(readers=None) -> None:
         from .attention import attn_decode_status, attn_tc_status
         from .gemm_tc import gemm_tc_status
         from .gemm_ws import gemm_ws_status
+        from .kv8 import kv8_decode_status
         from .layers import decode_layers_status
         from .moe import moe_tc_status
         fns = {"moe_tc_status": moe_tc_status, "gemm_tc_status": gemm_tc_status, "attn_tc_status": attn_tc_status, "attn_decode_status": attn_decode_status,
-               "gemm_ws_status": gemm_ws_status, "decode_layers_status": decode_layers_status}
+               "gemm_ws_status": gemm_ws_status, "decode_layers_status": decode_layers_status, "kv8_decode_status": kv8_decode_status}
         readers = {}
         for lib, (what, fname) in _STATUS_READERS.items():
             if loaded(lib):

@@ -6,6 +6,7 @@ A token's key (or value) of a head is one exponent byte ``e`` and ``hd`` e4m3 co
 ``448 * 2^119`` saturate.  Head sizes are multiples of 16 up to 256, keys and values of one size."""
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple, Optional, Tuple
 
 import numpy as np
@@ -203,6 +204,37 @@ def kv8_rows(q: torch.Tensor, pages: KV8Pages, seq_lens: torch.Tensor, block_tab
     return out
 
 
+DECODE_HEAD_DIMS = (64, 128)
+DECODE_MAX_GROUP = 16
+DECODE_MAX_SEQS = 2047
+DECODE_MIN_PAGES = 1
+
+
+def kv8_decode_supported(dtype, nh: int, nkv: int, hd: int, S: int) -> bool:
+    """Whether single tokens of these sizes attend on the tensor cores (``csrc/kv8_decode.cu``)."""
+    return dtype == torch.bfloat16 and hd in DECODE_HEAD_DIMS and nh // nkv <= DECODE_MAX_GROUP and S <= DECODE_MAX_SEQS
+
+
+def kv8_decode(q: torch.Tensor, pages: KV8Pages, seq_lens: torch.Tensor, block_table: torch.Tensor, nh: int, scale: float,
+               window: Optional[int], max_len: int, sinks: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One query token a sequence (row ``s`` of ``q``) on the tensor cores; sizes as ``kv8_decode_supported`` says."""
+    n_pages, nkv, hd = pages.v.shape[:3]
+    out = torch.empty_like(q)
+    part = torch.empty(sm_count(q.device) * 16 * (nh // nkv) * (hd + 2), dtype=torch.float32, device=q.device)
+    check(fn("kv8_decode", "sx_kv8_decode")(
+        ptr(q), ptr(out), ptr(pages.k), ptr(pages.v), ptr(pages.k_exp), ptr(pages.v_exp), ptr(seq_lens), ptr(block_table), c_int(block_table.shape[1]),
+        c_int(q.shape[0]), c_int(nh), c_int(nkv), c_int(hd), c_int(n_pages), c_float(scale), c_int(window or 0), ptr(sinks), ptr(part),
+        c_int(-(-min(max_len, (window or max_len) + PAGE) // PAGE)), c_int(DECODE_MIN_PAGES), stream()), "kv8_attention", launches=2)
+    return out
+
+
+def kv8_decode_status(reset: bool = False) -> int:
+    """0, or 1: a bounded wait of ``kv8_decode`` ran out in a launch the host has already waited for.  ``reset`` puts it back to 0."""
+    v = ctypes.c_int(0)
+    check(fn("kv8_decode", "sx_kv8_decode_status")(ctypes.byref(v), c_int(1 if reset else 0)), "kv8_decode_status", launches=0)
+    return int(v.value)
+
+
 def kv8_attention(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tensor, nh: int, nkv: int, hd: int, scale: float,
                   window: Optional[int] = None, *, softcap: Optional[float] = None, sinks: Optional[torch.Tensor] = None,
                   chunk: Optional[int] = None, out: Optional[torch.Tensor] = None, out_col: int = 0,
@@ -229,6 +261,8 @@ def kv8_attention(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tens
         if block_table.dim() != 2 or block_table.shape[0] < ctx.n_seqs or ctx.seq_lens.numel() < ctx.n_seqs:
             raise KernelError("kv8_attention: a row of the table and a length per sequence")
         _check_device("kv8_attention", q, *pages, ctx.seq_lens, block_table, sinks, out)
+        if out is None and softcap is None and chunk is None and out_scale == 1.0 and kv8_decode_supported(q.dtype, nh, nkv, hd, q.shape[0]):
+            return kv8_decode(q, pages, ctx.seq_lens, block_table, nh, scale, window, ctx.max_len, sinks)
         return kv8_rows(q, pages, ctx.seq_lens, block_table, nh, scale, window, ctx.max_len, softcap=softcap, sinks=sinks, chunk=chunk,
                         out=out, out_col=out_col, out_scale=out_scale)
     from . import attention
