@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(KV8_WARPS * 32) kv8_prepare_kernel(
 #pragma unroll
     for (int k = 0; k < KV8_MAX_HD / 32; ++k) {
       const int i = lane + 32 * k;
-      if (i < hd) dst[is_k ? kv8_k_at(key, i, cb) : kv8_v_at(key, i)] = (uint8_t)kv8_codes2(kv8_scaled(y[k], inverse), 0.f);
+      if (i < hd) dst[is_k ? kv8_k_at(key, i, cb) : kv8_v_at(key, i)] = (uint8_t)kv8_codes2(y[k] * inverse, 0.f);
     }
     if (lane == 0) (is_k ? k_exp : v_exp)[place * SX_PAGE + key] = (uint8_t)e;
   }

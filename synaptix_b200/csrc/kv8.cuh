@@ -3,7 +3,7 @@
 // A head's row of a token, x[0 .. hd), is one exponent byte e and hd e4m3 codes c_i and stands for c_i 2^(e - 127).  With a
 // the row's largest magnitude, a = m 2^x and 1 <= m < 2, e - 127 is x - 8 where m <= 1.75 and x - 7 above (448 = 1.75 2^8 is
 // the largest e4m3 number), kept in -117 .. 119; codes are rounded to nearest even and saturate.  e = 255: the row was not
-// finite and reads as NaN (its codes are 0).  A scale that is a power of two takes nothing from a floating format: all
+// finite and reads as NaN; its codes are e4m3's NaN (0x7f) too, so a kernel may look at either.  A scale that is a power of two takes nothing from a floating format: all
 // magnitudes within 2^15 of the row's largest keep their three bits of mantissa, as with any other scale, and in return x / scale and
 // code * scale are exact in bfloat16, float16 (within its range) and float32.  So writing rounds once, whatever
 // else a kernel does in which order, and reading back rounds never.
@@ -33,21 +33,22 @@ __device__ __forceinline__ int kv8_exponent(float a, bool finite) {
   const int e = (bits >> 23) - ((bits & 0x7fffff) <= 0x600000 ? 8 : 7);
   return a == 0.f ? KV8_MIN : min(max(e, KV8_MIN), KV8_MAX);
 }
-// 2^(127 - e), what a row's elements are multiplied by ahead of their rounding (0 for a row that is not finite)
-__device__ __forceinline__ float kv8_inverse(int e) { return e == KV8_NAN ? 0.f : __int_as_float((254 - e) << 23); }
+// 2^(127 - e), what a row's elements are multiplied by ahead of their rounding (NaN for a row that is not finite)
+__device__ __forceinline__ float kv8_inverse(int e) { return __int_as_float(e == KV8_NAN ? 0x7fffffff : (254 - e) << 23); }
 // 2^(e - 127); NaN for 255
 __device__ __forceinline__ float kv8_scale(int e) { return e == KV8_NAN ? __int_as_float(0x7fffffff) : __int_as_float(e << 23); }
 // two codes at once: `lo` in the low byte
 __device__ __forceinline__ uint32_t kv8_codes2(float lo, float hi) {
   return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
-// a row that is not finite has codes 0: its elements (infinities, NaN) times 0 would be NaN
-__device__ __forceinline__ float kv8_scaled(float x, float inverse) { return inverse == 0.f ? 0.f : x * inverse; }
-// two codes (the low 16 bits) as half precision, exactly
+// four codes as half precision, exactly: the two of the low 16 bits, the two of the high ones
+__device__ __forceinline__ void kv8_half4(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}\n" : "=r"(lo), "=r"(hi) : "r"(codes));
+}
 __device__ __forceinline__ uint32_t kv8_half2(uint32_t codes) {
-  uint32_t h;
-  asm("{\n .reg .b16 lo;\n cvt.u16.u32 lo, %1;\n cvt.rn.f16x2.e4m3x2 %0, lo;\n}\n" : "=r"(h) : "r"(codes));
-  return h;
+  uint32_t lo, hi;
+  kv8_half4(codes, lo, hi);
+  return lo;
 }
 __device__ __forceinline__ float2 kv8_float2(uint32_t codes) {
   const uint32_t h = kv8_half2(codes);

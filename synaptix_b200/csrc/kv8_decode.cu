@@ -3,17 +3,21 @@
 //
 // A single token reads every code once, so the kernel has to keep HBM busy: 16.1 KB a page and kv head at head size 128 against
 // 0.5 M operations.  Everything is done by warps on their own:
-//   * The visible pages of all (sequence, kv head) pairs are one line of items, and each warp takes an equal stretch of it, whatever
-//     the sequences' lengths are; a pair that several warps share is joined by a second, small kernel.
+//   * The visible pages of all (sequence, kv head) pairs are one line of items; each block takes an equal stretch of it, and each of its
+//     warps an equal stretch of that, whatever the sequences' lengths are.  A pair that several warps share is joined by those warps at the
+//     block's end, one that several blocks share by a second, small kernel.  Where every pair has a block and no more than two pages a warp,
+//     blocks take pairs instead and there is no second kernel.
 //   * A warp has its own ring of shared memory, filled by untiled bulk copies (K and V tile of a page are one stretch of memory each;
-//     no tensor map), and no barrier with other warps.  K and V take turns in the slots, so a slot is free again after half a page.
-//   * q k^T: the G heads are the M rows of m16n8k16 in half precision.  e4m3 codes become half precision exactly (one conversion for two),
-//     queries are bfloat16 scaled by a power of two of the row's so that its largest lies in 2^14 .. 2^15: every element down to 2^-28 of
-//     that is exact too.  The order of the inner axis is free as long as both operands agree, so a thread takes 16 neighbouring codes
-//     of a key in one 16-byte load (four k-steps' worth) and the query's elements to match.
-//   * The same freedom in p v (values lie dim by dim): with keys dealt to columns as 16 t + 2 j + i, the scores a thread holds are exactly
-//     the weights its fragments need, and the exponents of its 16 keys are one 16-byte load.  Nothing moves between lanes but the
-//     row's maxima.
+//     no tensor map; the exponents come by plain loads an item ahead, since a copy of 64 bytes costs as much to ask for as one of 8 KB), and no barrier with other warps on the way.  K and V take turns in the slots, so a slot is free again after half a page.
+//   * q k^T: m16n8k32 on the codes as they are.  A bfloat16 query (8 bits of mantissa) is the sum of TWO e4m3 numbers of 4 bits each: the
+//     G <= 8 heads' larger parts are the fragment's rows 0-7, the rests rows 8-15 that would be idle, and the two results are added.  Queries
+//     are scaled by a power of two so that the row's largest lies in 2^7 .. 2^8: elements down to 2^-9 of that are exact, smaller ones off by at
+//     most 2^-18 of it.  (m16n8k32 of e4m3 issues at 0.97 an SM and clock, m16n8k16 of f16 at 0.5, a pair of conversions to f16 at 0.67.)
+//     The order of the inner axis is free as long as both operands agree, so a thread takes 16 neighbouring codes of a key in one 16-byte
+//     load and the query's elements to match.
+//   * p v: m16n8k16 in half precision (e4m3 becomes that exactly), 16 dims of V as M and 8 heads as N, so that no row is idle.  Values lie dim by
+//     dim, and with keys dealt to the scores' columns as 16 t + 2 j + i the scores a thread holds are exactly the weights its fragments need,
+//     and the exponents of its 16 keys are one 16-byte load.  Nothing moves between lanes but the rows' maxima.
 //   * A value's power of two joins the weight before it is rounded: with x the score (base 2) and E the exponent, weights are 2^(x - m) in
 //     the denominator, and 2^(x + E - M + 15) in half precision beside the codes, with M the running maximum of x + E.  So a large value
 //     of next to no weight takes nothing from the precision of the others; weights from 1 down to 2^-29 of the row's largest x + E keep all 11 bits.
@@ -21,19 +25,24 @@
 // Every wait on an mbarrier is bounded; one that runs out sets the library's status word (sx_kv8_decode_status).
 #include "kv8.cuh"
 
-#define KD_WARPS 8
 #define KD_MAX_SEQS 2048
 #define KD_SPIN_LIMIT (1u << 26)
 #define KD_DOWN 3.0517578125e-5f      // 2^-15
 #define KD_DESC 64               // items a warp knows ahead: two batches of 32
+#define KD_LOG2E 1.44269504f
 
-template <int HD> struct KdLayout {
+// Three warps a scheduler hide one another's latencies (a page takes a warp alone 3,400 clocks, HBM delivers one to an SM every 710); with more
+// than 8 heads a kv head a thread has two rows' registers, and there two warps.
+template <int HD, bool MORE> struct KdLayout {
+  static constexpr int WARPS = MORE ? 8 : 12;
   static constexpr int TILE = SX_PAGE * HD;
-  static constexpr int SLOT = TILE + 128;                       // a K or V tile and its 64 exponents
-  static constexpr int SLOTS = HD == 128 ? 3 : 6;
-  static constexpr int RING = KD_WARPS * SLOTS * SLOT;
-  static constexpr int smem() { return RING + KD_WARPS * KD_DESC * (int)sizeof(int4) + KD_MAX_SEQS * (int)sizeof(int) + 128; }
+  static constexpr int SLOTS = (MORE ? 3 : 2) * (128 / HD);
+  static constexpr int AHEAD = (SLOTS + 1) / 2;                 // items whose tiles are under way ahead of the one at work
+  static constexpr int PART = HD + 2;                           // a row's maximum, sum and result
+  static constexpr int RING = WARPS * SLOTS * TILE;
+  static constexpr int smem() { return RING + WARPS * KD_DESC * (int)sizeof(int4) + KD_MAX_SEQS * (int)sizeof(int); }
 };
+#define KD_MAX_WARPS 12
 
 struct KdArgs {
   const bf16* q;
@@ -41,9 +50,9 @@ struct KdArgs {
   const uint8_t *k, *v, *ke, *ve;
   const int *seq_lens, *block_table;
   const float* sinks;
-  float* part;                 // [warps][2][rows of a kv head][HD + 2]
+  float* part;                 // results of pairs' parts [warps, then 2 a block][rows of a kv head][HD + 2]: maximum, sum, the row
   int* status;
-  int maxp, n_pages, S, nh, nkv, window, warps, min_pages;
+  int maxp, n_pages, S, nh, nkv, window, blocks, warps, by_pair;
   float scale;
 };
 
@@ -63,6 +72,10 @@ __device__ __forceinline__ void kd_copy(uint32_t dst, const void* src, uint32_t 
 }
 __device__ __forceinline__ void kd_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void kd_mma8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ float kd_ex2(float x) {
@@ -113,9 +126,9 @@ __device__ __forceinline__ void kd_starts(const KdArgs& a, int* start, int* warp
   if (threadIdx.x == 0) start[a.S] = before;
   __syncthreads();
 }
-// the warps that work and the first item of warp w (of all items `n`)
-__device__ __forceinline__ int kd_workers(const KdArgs& a, int n) { return max(1, min(a.warps, (n + a.min_pages - 1) / a.min_pages)); }
-__device__ __forceinline__ int kd_first(int w, int n, int workers) { return (int)((long long)w * n / workers); }
+// the blocks that work (a block of fewer items than warps would leave some idle), and the first item of block b
+__device__ __forceinline__ int kd_workers(const KdArgs& a, int n) { return max(1, min(a.blocks, (n + a.warps - 1) / a.warps)); }
+__device__ __forceinline__ int kd_first(int b, int n, int workers) { return (int)((long long)b * n / workers); }
 __device__ __forceinline__ int kd_worker_of(int item, int n, int workers) { return (int)((((long long)item + 1) * workers - 1) / n); }
 // the sequence of item x: the last s with start[s] * nkv <= x among those that have pages
 __device__ __forceinline__ int kd_seq_of(const int* start, int S, int nkv, int x) {
@@ -127,16 +140,16 @@ __device__ __forceinline__ int kd_seq_of(const int* start, int S, int nkv, int x
   return lo;
 }
 
-// MORE: more than 8 query heads a kv head, so that the fragments' second eight rows are used
+// MORE: more than 8 query heads a kv head (two rows of scores a thread, two tiles of heads in p v)
 template <int HD, bool MORE>
-__global__ void __launch_bounds__(KD_WARPS * 32, 1) kv8_decode_kernel(const KdArgs a) {
-  using L = KdLayout<HD>;
-  constexpr int RP = MORE ? 2 : 1;                              // rows a thread has
+__global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_kernel(const KdArgs a) {
+  using L = KdLayout<HD, MORE>;
+  constexpr int RP = MORE ? 2 : 1, WARPS = L::WARPS;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ __align__(8) uint64_t bars[KD_WARPS * L::SLOTS];
-  __shared__ int warp_sums[KD_WARPS];
+  __shared__ __align__(8) uint64_t bars[WARPS * L::SLOTS];
+  __shared__ int warp_sums[WARPS], first_unit[WARPS], last_unit[WARPS];
   int4* desc_all = reinterpret_cast<int4*>(smem + L::RING);
-  int* start = reinterpret_cast<int*>(smem + L::RING + KD_WARPS * KD_DESC * sizeof(int4));
+  int* start = reinterpret_cast<int*>(smem + L::RING + WARPS * KD_DESC * sizeof(int4));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   if (lane == 0) {
 #pragma unroll
@@ -146,58 +159,53 @@ __global__ void __launch_bounds__(KD_WARPS * 32, 1) kv8_decode_kernel(const KdAr
   }
   pdl_wait();
   pdl_trigger();
-  kd_starts<KD_WARPS * 32>(a, start, warp_sums);
+  kd_starts<WARPS * 32>(a, start, warp_sums);
   const int G = a.nh / a.nkv, n_all = start[a.S] * a.nkv;
-  const int workers = kd_workers(a, n_all), me = warp * gridDim.x + blockIdx.x;      // neighbours on different SMs
   if (n_all == 0) {                                             // nobody sees anything
-    for (size_t i = blockIdx.x * KD_WARPS * 32 + threadIdx.x; i < (size_t)a.S * a.nh * HD; i += gridDim.x * KD_WARPS * 32) a.out[i] = __float2bfloat16_rn(0.f);
+    for (size_t i = blockIdx.x * WARPS * 32 + threadIdx.x; i < (size_t)a.S * a.nh * HD; i += gridDim.x * WARPS * 32) a.out[i] = __float2bfloat16_rn(0.f);
     return;
   }
   // sequences without a visible key are nobody's items
-  for (int s = me; s < a.S; s += gridDim.x * KD_WARPS)
+  for (int s = blockIdx.x * WARPS + warp; s < a.S; s += gridDim.x * WARPS)
     if (start[s + 1] == start[s])
       for (int i = lane; i < a.nh * HD; i += 32) a.out[(size_t)s * a.nh * HD + i] = __float2bfloat16_rn(0.f);
-  if (me >= workers) return;
-  const int x0 = kd_first(me, n_all, workers), n_items = kd_first(me + 1, n_all, workers) - x0;
+  int b0, b1;                                                   // the block's items
+  if (a.by_pair) {
+    const int s = blockIdx.x / a.nkv, n = start[s + 1] - start[s];
+    b0 = start[s] * a.nkv + (blockIdx.x % a.nkv) * n;
+    b1 = b0 + n;
+  } else {
+    const int workers = kd_workers(a, n_all);
+    if (blockIdx.x >= workers) return;
+    b0 = kd_first(blockIdx.x, n_all, workers);
+    b1 = kd_first(blockIdx.x + 1, n_all, workers);
+  }
+  auto first_of = [&](int w) { return b0 + (b1 - b0) * w / WARPS; };
+  const int x0 = first_of(warp), n_items = first_of(warp + 1) - x0;
   int4* desc = desc_all + warp * KD_DESC;                       // (sequence, kv head, page of the sequence, page of the pool)
-  auto describe = [&](int batch) {
-    const int i = batch * 32 + lane;
-    if (i < n_items) {
-      const int s = kd_seq_of(start, a.S, a.nkv, x0 + i), n = start[s + 1] - start[s], at = x0 + i - start[s] * a.nkv;
-      const int kvh = at / n, j = kd_range(a, s).x + at % n, page = a.block_table[(size_t)s * a.maxp + j];
-      desc[i & (KD_DESC - 1)] = make_int4(s, kvh, j, (unsigned)page < (unsigned)a.n_pages ? page : 0);
-    }
-    __syncwarp();
-  };
-  unsigned char* ring = smem + warp * L::SLOTS * L::SLOT;
+  unsigned char* ring = smem + warp * L::SLOTS * L::TILE;
   const uint32_t ring_a = kd_smem(ring), bar_a = kd_smem(&bars[warp * L::SLOTS]);
   // load number n of the warp: the K (even) or V (odd) tile of item n / 2, into slot n % SLOTS
   auto issue = [&](int n) {
     const int i = n >> 1;
-    if (i >= n_items) return;
-    if (!(n & 1) && (i & 31) == 0) describe(i >> 5);
-    if (lane == 0) {
+    if (lane == 0 && i < n_items) {
       const int4 d = desc[i & (KD_DESC - 1)];
-      const size_t place = (size_t)d.w * a.nkv + d.y;
       const int slot = n % L::SLOTS;
-      const uint32_t dst = ring_a + slot * L::SLOT, bar = bar_a + slot * 8;
-      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(L::TILE + SX_PAGE) : "memory");
-      kd_copy(dst, ((n & 1) ? a.v : a.k) + place * L::TILE, L::TILE, bar);
-      kd_copy(dst + L::TILE, ((n & 1) ? a.ve : a.ke) + place * SX_PAGE, SX_PAGE, bar);
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar_a + slot * 8), "r"(L::TILE) : "memory");
+      kd_copy(ring_a + slot * L::TILE, ((n & 1) ? a.v : a.k) + ((size_t)d.w * a.nkv + d.y) * L::TILE, L::TILE, bar_a + slot * 8);
     }
   };
-#pragma unroll
-  for (int n = 0; n < L::SLOTS; ++n) issue(n);
 
-  uint32_t qf[HD / 16][2 * RP];
-  float c[RP], m[RP], l[RP], M[RP], o[HD / 8][4];
-  int seq = -1, kvh = -1, unit_first = 0;                       // the pair at work and the item of the warp it began with
+  uint32_t qf[HD / 16][2][RP];                                  // [4 dims each][larger part, rest][row]
+  float c[RP], m[RP], l[RP], M[RP], o[HD / 16][RP][4];          // o: dims 16 d + g (+ 8), heads 8 r + 2 t + {0, 1}
+  int seq = -1, kvh = -1, unit_first = 0, unit0 = -1, len = 0;  // the pair at work, the item of the warp it began with; the warp's first pair
   auto begin = [&](int s, int h, int i) {
     seq = s; kvh = h; unit_first = i;
+    len = a.seq_lens[s];
 #pragma unroll
     for (int r = 0; r < RP; ++r) {
       const int row = g + 8 * r;
-      uint4 w[HD / 32];                                         // dims 64 c + 16 t .. + 15 of the row
+      uint4 w[HD / 32];                                         // dims 64 b + 16 t .. + 15 of the row
 #pragma unroll
       for (int b = 0; b < HD / 64; ++b) {
         const uint4* src = reinterpret_cast<const uint4*>(a.q + ((size_t)s * a.nh + (size_t)h * G + row) * HD + 64 * b + 16 * t);
@@ -211,90 +219,132 @@ __global__ void __launch_bounds__(KD_WARPS * 32, 1) kv8_decode_kernel(const KdAr
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int e = max((int)(top >> 7), 28);                   // biased exponent of the largest; tiny rows stay tiny
-      const float down = __int_as_float((268 - e) << 23);       // 2^(14 - (e - 127)); e from 28 to 254
-      c[r] = top >= 0x7f80u ? __int_as_float(0x7fffffff) : __int_as_float(max(e - 14, 1) << 23) * a.scale * 1.44269504f;
+      const float down = __int_as_float((261 - e) << 23);       // 2^(7 - (e - 127)); e from 28 to 254
+      c[r] = top >= 0x7f80u ? __int_as_float(0x7fffffff) : __int_as_float((e - 7) << 23) * a.scale * KD_LOG2E;
 #pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks)
-#pragma unroll
-        for (int h2 = 0; h2 < 2; ++h2) {
-          const uint32_t pair = u[(ks >> 2) * 8 + (ks & 3) * 2 + h2];
-          qf[ks][h2 * RP + r] = kd_half2(__uint_as_float(pair << 16) * down, __uint_as_float(pair & 0xffff0000u) * down);
-        }
+      for (int k = 0; k < HD / 16; ++k) {
+        const float x[4] = {__uint_as_float(u[2 * k] << 16) * down, __uint_as_float(u[2 * k] & 0xffff0000u) * down,
+                            __uint_as_float(u[2 * k + 1] << 16) * down, __uint_as_float(u[2 * k + 1] & 0xffff0000u) * down};
+        const uint32_t p0 = kv8_codes2(x[0], x[1]), p1 = kv8_codes2(x[2], x[3]);
+        const float2 y0 = kv8_float2(p0), y1 = kv8_float2(p1);
+        qf[k][0][r] = p0 | p1 << 16;
+        qf[k][1][r] = kv8_codes2(x[0] - y0.x, x[1] - y0.y) | kv8_codes2(x[2] - y1.x, x[3] - y1.y) << 16;
+      }
       m[r] = M[r] = -INFINITY;
       l[r] = 0.f;
-    }
 #pragma unroll
-    for (int n = 0; n < HD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+      for (int d = 0; d < HD / 16; ++d) o[d][r][0] = o[d][r][1] = o[d][r][2] = o[d][r][3] = 0.f;
+    }
+  };
+  // what a row's lanes (those of g) hold, for the two heads 2 t and 2 t + 1 of the thread's results
+  auto of_heads = [&](float x) { return make_float2(__shfl_sync(0xffffffffu, x, 8 * t), __shfl_sync(0xffffffffu, x, 8 * t + 4)); };
+  // parts of pairs: the one a warp ends with in its ring, which nothing uses any more, one that another warp began before it in global memory
+  auto part_of = [&](int w, bool at_end) {
+    return at_end ? reinterpret_cast<float*>(smem + w * L::SLOTS * L::TILE) : a.part + (size_t)(blockIdx.x * WARPS + w) * G * L::PART;
   };
   auto finish = [&](int i_end) {
     const int n = start[seq + 1] - start[seq], at = x0 + unit_first - start[seq] * a.nkv - kvh * n, count = i_end - unit_first;
     const bool whole = at == 0 && count == n;
+    float* part = part_of(warp, i_end == n_items);
 #pragma unroll
     for (int r = 0; r < RP; ++r) {
       const int row = g + 8 * r;
-      float L_ = l[r];
-      L_ += __shfl_xor_sync(0xffffffffu, L_, 1);
-      L_ += __shfl_xor_sync(0xffffffffu, L_, 2);
+      float sum = l[r];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       // 2^-15 o is 2^-M times sum 2^(x + E) code; times this it is the sum of 2^(x - m) 2^E code
       float f = m[r] == -INFINITY || M[r] == -INFINITY ? 0.f : kd_ex2(M[r] - m[r]);
-      if (row >= G) continue;
-      const int head = kvh * G + row;
       if (whole) {
-        if (a.sinks) {
-          const float sink = a.sinks[head] * 1.44269504f, top = fmaxf(m[r], sink);
-          const float shrink = kd_ex2(m[r] - top);
-          L_ = L_ * shrink + kd_ex2(sink - top);
-          f *= shrink;
+        const float sink = a.sinks && row < G ? a.sinks[kvh * G + row] * KD_LOG2E : -INFINITY, top = fmaxf(m[r], sink);
+        const float base = top == -INFINITY ? 0.f : top, shrink = kd_ex2(m[r] - base);
+        sum = sum * shrink + kd_ex2(sink - base);
+        f = sum == 0.f ? 0.f : f * shrink / sum;
+      } else if (row < G && t == 0) {
+        *reinterpret_cast<float2*>(part + row * L::PART) = make_float2(m[r], sum);
+      }
+      const float2 fh = of_heads(f);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int head = 8 * r + 2 * t + h;
+        if (head >= G) continue;
+        const float fx = h ? fh.y : fh.x;
+        bf16* dst = a.out + ((size_t)seq * a.nh + kvh * G + head) * HD + g;
+        float* dstp = part + head * L::PART + 2 + g;
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) {
+          const float x = o[d][r][h] * KD_DOWN * fx, y = o[d][r][2 + h] * KD_DOWN * fx;
+          if (whole) {
+            dst[16 * d] = __float2bfloat16_rn(x);
+            dst[16 * d + 8] = __float2bfloat16_rn(y);
+          } else {
+            dstp[16 * d] = x;
+            dstp[16 * d + 8] = y;
+          }
         }
-        f = L_ == 0.f ? 0.f : f / L_;
-        bf16* dst = a.out + ((size_t)seq * a.nh + head) * HD + 2 * t;
-#pragma unroll
-        for (int d = 0; d < HD / 8; ++d)
-          *reinterpret_cast<__nv_bfloat162*>(dst + 8 * d) = __floats2bfloat162_rn(o[d][2 * r] * KD_DOWN * f, o[d][2 * r + 1] * KD_DOWN * f);
-      } else {
-        // a pair's first stretch goes to the warp's second place, one that another warp began to its first
-        float* dst = a.part + ((size_t)(me * 2 + (at == 0 ? 1 : 0)) * G + row) * (HD + 2);
-        if (t == 0) *reinterpret_cast<float2*>(dst) = make_float2(m[r], L_);
-#pragma unroll
-        for (int d = 0; d < HD / 8; ++d) *reinterpret_cast<float2*>(dst + 2 + 8 * d + 2 * t) = make_float2(o[d][2 * r] * KD_DOWN * f, o[d][2 * r + 1] * KD_DOWN * f);
       }
     }
   };
 
   bool ok = true;
   int done = 0;
-  for (int i = 0; i < n_items; ++i) {
+  uint4 ke4 = make_uint4(0, 0, 0, 0), ve4 = ke4, ke4_next = ke4, ve4_next = ke4;       // exponents of the thread's keys 16 t ..
+  for (int i = -L::AHEAD; i < n_items; ++i) {
+    if (((i + L::AHEAD) & 31) == 0) {                           // the next 32 items
+      const int x = i + L::AHEAD + lane;
+      if (x < n_items) {
+        const int s = kd_seq_of(start, a.S, a.nkv, x0 + x), n = start[s + 1] - start[s], at = x0 + x - start[s] * a.nkv;
+        const int h = at / n, j = kd_range(a, s).x + at - h * n, page = a.block_table[(size_t)s * a.maxp + j];
+        desc[x & (KD_DESC - 1)] = make_int4(s, h, j, (unsigned)page < (unsigned)a.n_pages ? page : 0);
+      }
+      __syncwarp();
+      if (i == -L::AHEAD)
+        for (int n = 0; n < L::SLOTS; ++n) issue(n);
+    }
+    ke4 = ke4_next;
+    ve4 = ve4_next;
+    if (i >= -1 && i + 1 < n_items) {
+      const int4 d = desc[(i + 1) & (KD_DESC - 1)];
+      const size_t at = ((size_t)d.w * a.nkv + d.y) * SX_PAGE + 16 * t;
+      ke4_next = *reinterpret_cast<const uint4*>(a.ke + at);
+      ve4_next = *reinterpret_cast<const uint4*>(a.ve + at);
+    }
+    if (i < 0) continue;
     done = i;
     const int4 d = desc[i & (KD_DESC - 1)];
     if (d.x != seq || d.y != kvh) {
-      if (seq >= 0) finish(i);
       begin(d.x, d.y, i);
+      if (i == 0) unit0 = d.x * a.nkv + d.y;
     }
-    const int len = a.seq_lens[seq];
     const int v0 = a.window > 0 ? max(0, len - a.window - d.z * SX_PAGE) : 0, v1 = len - d.z * SX_PAGE;   // visible keys of the page: v0 <= key < v1
     const bool edge = v0 > 0 || v1 < SX_PAGE;
     // ---- scores
     int n = 2 * i, slot = n % L::SLOTS;
     ok = ok && kd_wait(bar_a + slot * 8, (n / L::SLOTS) & 1);
     if (!__all_sync(0xffffffffu, ok)) break;
-    const unsigned char* tile = ring + slot * L::SLOT;
-    float s[8][4];
+    unsigned char* tile = ring + slot * L::TILE;
+    float s[8][2 * RP];                                         // keys 16 t + 2 j + {0, 1}, rows g (+ 8)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-      const int key = 16 * (g >> 1) + 2 * j + (g & 1);
+      const unsigned char* row = tile + (16 * (g >> 1) + 2 * j + (g & 1)) * 64 + 16 * t;
+      float acc[4] = {0.f, 0.f, 0.f, 0.f}, rest[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int b = 0; b < HD / 64; ++b) {
-        const uint4 w = *reinterpret_cast<const uint4*>(tile + b * 4096 + key * 64 + 16 * t);
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+        const uint4 w = *reinterpret_cast<const uint4*>(row + b * 4096);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t(&qa)[2 * RP] = qf[4 * b + k];
-          kd_mma(s[j], qa[0], MORE ? qa[RP - 1] : 0u, qa[RP], MORE ? qa[2 * RP - 1] : 0u, kv8_half2(ww[k]), kv8_half2(ww[k] >> 16));
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t b0_ = h ? w.z : w.x, b1_ = h ? w.w : w.y;
+          const int k = 4 * b + 2 * h;
+          if (MORE) {
+            kd_mma8(acc, qf[k][0][0], qf[k][0][RP - 1], qf[k + 1][0][0], qf[k + 1][0][RP - 1], b0_, b1_);
+            kd_mma8(rest, qf[k][1][0], qf[k][1][RP - 1], qf[k + 1][1][0], qf[k + 1][1][RP - 1], b0_, b1_);
+          } else {
+            kd_mma8(acc, qf[k][0][0], qf[k][1][0], qf[k + 1][0][0], qf[k + 1][1][0], b0_, b1_);
+          }
         }
       }
+#pragma unroll
+      for (int e = 0; e < 2 * RP; ++e) s[j][e] = acc[e] + (MORE ? rest[e] : acc[2 + e]);
     }
-    const uint4 ke4 = *reinterpret_cast<const uint4*>(tile + L::TILE + 16 * t);    // exponents of the thread's keys 16 t ..
     __syncwarp();
     issue(n + L::SLOTS);
     const uint32_t ke[4] = {ke4.x, ke4.y, ke4.z, ke4.w};
@@ -305,16 +355,27 @@ __global__ void __launch_bounds__(KD_WARPS * 32, 1) kv8_decode_kernel(const KdAr
     for (int j = 0; j < 8; ++j)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float kf = kv8_scale((ke[j >> 1] >> (16 * (j & 1) + 8 * e)) & 0xff);
-        const int key = 16 * t + 2 * j + e;
+        // 2^(e - 127) from the byte's bits (255: an infinity, which times the NaN of such a row's codes is NaN)
+        const int at = 2 * (j & 1) + e;
+        const float kf = __uint_as_float((at < 3 ? ke[j >> 1] << (23 - 8 * at) : ke[j >> 1] >> 1) & 0x7f800000u);
 #pragma unroll
-        for (int r = 0; r < RP; ++r) {
-          float x = s[j][2 * r + e] * kf * c[r];
-          if (edge && (key < v0 || key >= v1)) x = -INFINITY;
-          s[j][2 * r + e] = x;
-          top[r] = fmaxf(top[r], x);
-        }
+        for (int r = 0; r < RP; ++r) s[j][2 * r + e] *= kf * c[r];
       }
+    if (edge) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int key = 16 * t + 2 * j + e;
+#pragma unroll
+          for (int r = 0; r < RP; ++r)
+            if (key < v0 || key >= v1) s[j][2 * r + e] = -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int r = 0; r < RP; ++r) top[r] = fmaxf(top[r], fmaxf(s[j][2 * r], s[j][2 * r + 1]));
 #pragma unroll
     for (int r = 0; r < RP; ++r) {
       top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
@@ -331,8 +392,23 @@ __global__ void __launch_bounds__(KD_WARPS * 32, 1) kv8_decode_kernel(const KdAr
     slot = n % L::SLOTS;
     ok = ok && kd_wait(bar_a + slot * 8, (n / L::SLOTS) & 1);
     if (!__all_sync(0xffffffffu, ok)) break;
-    tile = ring + slot * L::SLOT;
-    const uint4 ve4 = *reinterpret_cast<const uint4*>(tile + L::TILE + 16 * t);
+    tile = ring + slot * L::TILE;
+    if (edge) {                                                 // codes of keys that are not seen may be anything: zeros instead
+      uint32_t keep[4];                                         // bytes of the lane's 16 keys, the same in every row it has
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int key = ((lane & 3) << 4) + 4 * k, lo = min(max(v0 - key, 0), 4), hi = min(max(v1 - key, 0), 4);
+        keep[k] = (hi == 4 ? ~0u : (1u << (8 * hi)) - 1u) & (lo == 4 ? 0u : ~((1u << (8 * lo)) - 1u));
+      }
+#pragma unroll 4
+      for (int at = lane * 16; at < L::TILE; at += 512) {
+        uint4 w = *reinterpret_cast<uint4*>(tile + at);
+        w.x &= keep[0]; w.y &= keep[1]; w.z &= keep[2]; w.w &= keep[3];
+        *reinterpret_cast<uint4*>(tile + at) = w;
+      }
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");      // (the next copy into this slot comes behind these writes)
+      __syncwarp();
+    }
     const uint32_t ve[4] = {ve4.x, ve4.y, ve4.z, ve4.w};
     float Top[RP];
 #pragma unroll
@@ -341,9 +417,8 @@ __global__ void __launch_bounds__(KD_WARPS * 32, 1) kv8_decode_kernel(const KdAr
     for (int j = 0; j < 8; ++j)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int b = (ve[j >> 1] >> (16 * (j & 1) + 8 * e)) & 0xff, key = 16 * t + 2 * j + e;
-        float E = b == KV8_NAN ? __int_as_float(0x7fffffff) : (float)(b - 127);
-        if (edge && (key < v0 || key >= v1)) E = 0.f;
+        // the byte as the last one of 2^23 + byte.  (A row that is not finite is NaN by its codes, whatever its weight.)
+        const float E = __uint_as_float(__byte_perm(ve[j >> 1], 0x4b000000u, 0x7440 + 2 * (j & 1) + e)) - 8388735.f;
 #pragma unroll
         for (int r = 0; r < RP; ++r) {
           s[j][2 * r + e] += E;
@@ -360,12 +435,12 @@ __global__ void __launch_bounds__(KD_WARPS * 32, 1) kv8_decode_kernel(const KdAr
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
       for (int r = 0; r < RP; ++r) {
-        const float shrink = Top[r] == -INFINITY ? 1.f : kd_ex2(M[r] - Top[r]);
+        const float2 shrink = of_heads(Top[r] == -INFINITY ? 1.f : kd_ex2(M[r] - Top[r]));
         M[r] = Top[r];
 #pragma unroll
-        for (int d2 = 0; d2 < HD / 8; ++d2) {
-          o[d2][2 * r] *= shrink;
-          o[d2][2 * r + 1] *= shrink;
+        for (int d2 = 0; d2 < HD / 16; ++d2) {
+          o[d2][r][0] *= shrink.x; o[d2][r][1] *= shrink.y;
+          o[d2][r][2] *= shrink.x; o[d2][r][3] *= shrink.y;
         }
       }
     }
@@ -376,24 +451,24 @@ __global__ void __launch_bounds__(KD_WARPS * 32, 1) kv8_decode_kernel(const KdAr
 #pragma unroll
       for (int j = 0; j < 8; ++j) p[j][r] = kd_half2(kd_ex2(s[j][2 * r] - base), kd_ex2(s[j][2 * r + 1] - base));
     }
-    uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};                    // codes of keys that are not seen may be anything: zeros instead
-    if (edge) {
 #pragma unroll
-      for (int k = 0; k < 16; ++k)
-        if (16 * t + k < v0 || 16 * t + k >= v1) keep[k >> 2] &= ~(0xffu << (8 * (k & 3)));
-    }
+    for (int d2 = 0; d2 < HD / 16; ++d2) {
+      const uint4 w0 = *reinterpret_cast<const uint4*>(tile + (16 * d2 + g) * 64 + 16 * t);
+      const uint4 w1 = *reinterpret_cast<const uint4*>(tile + (16 * d2 + 8 + g) * 64 + 16 * t);
+      const uint32_t u0[4] = {w0.x, w0.y, w0.z, w0.w}, u1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-    for (int d2 = 0; d2 < HD / 8; ++d2) {
-      const uint4 w = *reinterpret_cast<const uint4*>(tile + (8 * d2 + g) * 64 + 16 * t);
-      const uint32_t ww[4] = {w.x & keep[0], w.y & keep[1], w.z & keep[2], w.w & keep[3]};
+      for (int k = 0; k < 4; ++k) {
+        uint32_t a0, a1, a2, a3;
+        kv8_half4(u0[k], a0, a2);
+        kv8_half4(u1[k], a1, a3);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        kd_mma(o[d2], p[2 * k][0], MORE ? p[2 * k][RP - 1] : 0u, p[2 * k + 1][0], MORE ? p[2 * k + 1][RP - 1] : 0u, kv8_half2(ww[k]),
-               kv8_half2(ww[k] >> 16));
+        for (int r = 0; r < RP; ++r) kd_mma(o[d2][r], a0, a1, a2, a3, p[2 * k][r], p[2 * k + 1][r]);
+      }
     }
     __syncwarp();
     issue(n + L::SLOTS);
-    if (i + 1 == n_items) finish(n_items);
+    const int4 next = desc[(i + 1) & (KD_DESC - 1)];            // (of the last item: anything)
+    if (i + 1 == n_items || next.x != seq || next.y != kvh) finish(i + 1);
   }
   if (!__all_sync(0xffffffffu, ok)) {
     if (lane == 0) sx_set_status(a.status, 1);
@@ -402,34 +477,125 @@ __global__ void __launch_bounds__(KD_WARPS * 32, 1) kv8_decode_kernel(const KdAr
       if ((n >> 1) < n_items) kd_wait(bar_a + n % L::SLOTS * 8, (n / L::SLOTS) & 1);
     }
   }
+  // ---- pairs that several warps worked at, or that go on in another block, are joined: their rows are dealt out to all warps
+  const int unit1 = n_items ? seq * a.nkv + kvh : -1;
+  if (lane == 0) {
+    first_unit[warp] = unit0;
+    last_unit[warp] = unit1;
+  }
+  __syncthreads();
+  // lanes 0-15 look at warp k's first pair (unless a warp before has a part of it, too), lanes 16-31 at its last one where that is another
+  const int k_ = lane & 15, fu = k_ < WARPS ? first_unit[k_] : -1, lu = k_ < WARPS ? last_unit[k_] : -1;
+  int before = lu;
+#pragma unroll
+  for (int o_ = 1; o_ < 16; o_ <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, before, o_, 16);
+    if (k_ >= o_) before = max(before, y);
+  }
+  before = __shfl_up_sync(0xffffffffu, before, 1, 16);
+  const int mine = lane < 16 ? fu : lu, mine_s = max(mine, 0) / a.nkv, mine_h = max(mine, 0) - mine_s * a.nkv;
+  const int mine_n = start[mine_s + 1] - start[mine_s], mine_from = start[mine_s] * a.nkv + mine_h * mine_n;
+  const bool met = mine < 0 || (lane < 16 ? k_ > 0 && before == fu : lu == fu);
+  const bool alone = mine_from >= first_of(k_) && mine_from + mine_n <= first_of(k_ + 1);      // written by its warp
+  const uint32_t joins = __ballot_sync(0xffffffffu, !met && !alone);
+#pragma unroll 1
+  for (int r = warp; r < __popc(joins) * G; r += WARPS) {
+    const int row = r % G;
+    uint32_t left = joins;
+    for (int j = r / G; j > 0; --j) left &= left - 1;
+    const int from_lane = __ffs(left) - 1;
+    const int u = __shfl_sync(0xffffffffu, mine, from_lane), us = __shfl_sync(0xffffffffu, mine_s, from_lane);
+    const int from = __shfl_sync(0xffffffffu, mine_from, from_lane), n = __shfl_sync(0xffffffffu, mine_n, from_lane);
+    const int head = __shfl_sync(0xffffffffu, mine_h, from_lane) * G + row;
+    const bool final = from >= b0 && from + n <= b1, has = lane < WARPS && fu >= 0 && fu <= u && u <= lu;
+    const uint32_t have = __ballot_sync(0xffffffffu, has);      // warps with a part of u
+    float2 v[WARPS][HD / 64];
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) {
+      const float* src = part_of(k, u == last_unit[k]) + row * L::PART + 2 + 2 * lane;
+#pragma unroll
+      for (int h = 0; h < HD / 64; ++h) v[k][h] = have >> k & 1 ? *reinterpret_cast<const float2*>(src + 64 * h) : make_float2(0.f, 0.f);
+    }
+    const float2 ml = has ? *reinterpret_cast<const float2*>(part_of(lane, u == lu) + row * L::PART) : make_float2(-INFINITY, 0.f);
+    const float sink = final && a.sinks ? a.sinks[head] * KD_LOG2E : -INFINITY;
+    const float top = fmaxf(warp_max(ml.x), sink), base = top == -INFINITY ? 0.f : top;
+    float w = kd_ex2(ml.x - base);
+    const float sum = warp_sum(ml.y * w) + kd_ex2(sink - base);
+    if (final) w = sum == 0.f ? 0.f : w / sum;
+    float2 x[HD / 64];
+#pragma unroll
+    for (int h = 0; h < HD / 64; ++h) x[h] = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) {
+      const float f = __shfl_sync(0xffffffffu, w, k);
+#pragma unroll
+      for (int h = 0; h < HD / 64; ++h) {
+        x[h].x += f * v[k][h].x;
+        x[h].y += f * v[k][h].y;
+      }
+    }
+    // a pair's first stretch goes to the block's second place, one that another block began to its first
+    float* dst = a.part + ((size_t)(gridDim.x * WARPS + blockIdx.x * 2 + (from >= b0 ? 1 : 0)) * G + row) * L::PART;
+    if (!final && lane == 0) *reinterpret_cast<float2*>(dst) = make_float2(top, sum);
+#pragma unroll
+    for (int h = 0; h < HD / 64; ++h) {
+      const int d = 2 * lane + 64 * h;
+      if (final) *reinterpret_cast<__nv_bfloat162*>(a.out + ((size_t)us * a.nh + head) * HD + d) = __floats2bfloat162_rn(x[h].x, x[h].y);
+      else *reinterpret_cast<float2*>(dst + 2 + d) = x[h];
+    }
+  }
 }
 
-// Pairs that several warps shared: a block a (pair, row), 4 threads a group of dims take turns over the shares.
+// Pairs that several blocks shared: block (b, row) looks at the border between the stretches b and b + 1, and where a pair's first border is
+// that one, joins the pair's row.  Lengths are read while the first kernel still runs: it lets this one in behind its own wait, so what was
+// there before it is there.
 template <int HD>
 __global__ void __launch_bounds__(256) kv8_decode_merge_kernel(const KdArgs a) {
+  constexpr int TEAMS = 256 / (HD / 2);
   __shared__ int start[KD_MAX_SEQS + 1], warp_sums[8];
-  __shared__ float acc[256 / (HD / 2)][HD], s_m[256 / (HD / 2)], s_l[256 / (HD / 2)];
+  __shared__ float acc[TEAMS][HD], s_m[TEAMS], s_l[TEAMS];
+  kd_starts<256>(a, start, warp_sums);
+  const int G = a.nh / a.nkv, row = blockIdx.y, n_all = start[a.S] * a.nkv, workers = n_all ? kd_workers(a, n_all) : 0;
+  const int w0 = blockIdx.x;
+  int w1 = w0, seq = 0, kvh = 0;
+  if (w0 + 1 < workers) {
+    const int border = kd_first(w0 + 1, n_all, workers);
+    seq = kd_seq_of(start, a.S, a.nkv, border);
+    const int n = start[seq + 1] - start[seq], at = border - start[seq] * a.nkv;
+    kvh = at / n;
+    const int from = start[seq] * a.nkv + kvh * n;
+    if (from < border && kd_worker_of(from, n_all, workers) == w0) w1 = kd_worker_of(from + n - 1, n_all, workers);
+  }
   pdl_wait();
   pdl_trigger();
-  kd_starts<256>(a, start, warp_sums);
-  constexpr int TEAMS = 256 / (HD / 2);
-  const int G = a.nh / a.nkv, seq = blockIdx.x / a.nh, head = blockIdx.x % a.nh, kvh = head / G, row = head % G;
-  const int n = start[seq + 1] - start[seq], n_all = start[a.S] * a.nkv;
-  if (n == 0) return;
-  const int workers = kd_workers(a, n_all), first = start[seq] * a.nkv + kvh * n;
-  const int w0 = kd_worker_of(first, n_all, workers), w1 = kd_worker_of(first + n - 1, n_all, workers);
-  if (w0 == w1) return;
-  const int team = threadIdx.x / (HD / 2), d = threadIdx.x % (HD / 2) * 2;
+  if (w1 == w0) return;
+  const int head = kvh * G + row, team = threadIdx.x / (HD / 2), d = threadIdx.x % (HD / 2) * 2;
+  const float* parts = a.part + ((size_t)a.blocks * a.warps * G + row) * (HD + 2);
   float top = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
-  // (workers are never more than items, so every warp from w0 to w1 has a share)
-#pragma unroll 4
-  for (int w = w0 + team; w <= w1; w += TEAMS) {
-    const float* src = a.part + ((size_t)(w * 2 + (w == w0 ? 1 : 0)) * G + row) * (HD + 2);
-    const float2 ml = *reinterpret_cast<const float2*>(src), v = *reinterpret_cast<const float2*>(src + 2 + d);
-    const float next = fmaxf(top, ml.x), base = next == -INFINITY ? 0.f : next, f = kd_ex2(top - base), h = kd_ex2(ml.x - base);
-    L = L * f + ml.y * h;
-    x = x * f + v.x * h;
-    y = y * f + v.y * h;
+  // (blocks at work are never more than items, so every one from w0 to w1 has a part)
+  for (int w = w0 + team; w <= w1; w += 4 * TEAMS) {
+    float2 ml[4], v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = w + k * TEAMS;
+      ml[k] = make_float2(-INFINITY, 0.f);
+      v[k] = make_float2(0.f, 0.f);
+      if (i <= w1) {
+        const float* src = parts + (size_t)(i * 2 + (i == w0 ? 1 : 0)) * G * (HD + 2);
+        ml[k] = *reinterpret_cast<const float2*>(src);
+        v[k] = *reinterpret_cast<const float2*>(src + 2 + d);
+      }
+    }
+    const float next = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), top), base = next == -INFINITY ? 0.f : next;
+    const float f = kd_ex2(top - base);
+    L *= f; x *= f; y *= f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float h = kd_ex2(ml[k].x - base);
+      L += ml[k].y * h;
+      x += v[k].x * h;
+      y += v[k].y * h;
+    }
     top = next;
   }
   acc[team][d] = x;
@@ -440,12 +606,12 @@ __global__ void __launch_bounds__(256) kv8_decode_merge_kernel(const KdArgs a) {
   }
   __syncthreads();
   if (threadIdx.x >= HD) return;
-  const float sink = a.sinks ? a.sinks[head] * 1.44269504f : -INFINITY;
+  const float sink = a.sinks ? a.sinks[head] * KD_LOG2E : -INFINITY;
   top = sink;
 #pragma unroll
   for (int i = 0; i < TEAMS; ++i) top = fmaxf(top, s_m[i]);
   const float base = top == -INFINITY ? 0.f : top;
-  L = a.sinks ? kd_ex2(sink - base) : 0.f;
+  L = kd_ex2(sink - base);
   float O = 0.f;
 #pragma unroll
   for (int i = 0; i < TEAMS; ++i) {
@@ -468,41 +634,51 @@ extern "C" int sx_kv8_decode_status(int* value, int reset) {
   return 0;
 }
 
-// floats of `part` for a launch on the current device
-extern "C" long long sx_kv8_decode_scratch(int nh, int nkv, int hd) {
-  return (long long)sx_sm_count() * KD_WARPS * 2 * (nh / nkv) * (hd + 2);
-}
-
 template <int HD, bool MORE>
-static int kd_launch(const KdArgs& a, int blocks, cudaStream_t stream) {
+static int kd_launch(KdArgs a, cudaStream_t stream) {
+  using L = KdLayout<HD, MORE>;
   static bool opted[64] = {false};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
   if (dev < 0 || dev >= 64 || !opted[dev]) {
-    e = cudaFuncSetAttribute(kv8_decode_kernel<HD, MORE>, cudaFuncAttributeMaxDynamicSharedMemorySize, KdLayout<HD>::smem());
+    e = cudaFuncSetAttribute(kv8_decode_kernel<HD, MORE>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem());
     if (e != cudaSuccess) return (int)e;
     if (dev >= 0 && dev < 64) opted[dev] = true;
   }
-  const int rc = sx_launch(kv8_decode_kernel<HD, MORE>, dim3(blocks), dim3(KD_WARPS * 32), KdLayout<HD>::smem(), stream, a);
-  if (rc) return rc;
-  return sx_launch(kv8_decode_merge_kernel<HD>, dim3(a.S * a.nh), dim3(256), 0, stream, a);
+  a.warps = L::WARPS;
+  const int rc = sx_launch(kv8_decode_kernel<HD, MORE>, dim3(a.blocks), dim3(L::WARPS * 32), L::smem(), stream, a);
+  if (rc || a.by_pair || a.blocks == 1) return rc;
+  return sx_launch(kv8_decode_merge_kernel<HD>, dim3(a.blocks - 1, a.nh / a.nkv), dim3(256), 0, stream, a);
 }
 
+// a block a pair: pairs no more than SMs, of no more than two pages a warp
+static bool kd_by_pair(int S, int nkv, int max_pages) { return (long long)S * nkv <= sx_sm_count() && max_pages <= 2 * KD_MAX_WARPS; }
+static int kd_blocks(int S, int nkv, int max_pages) {
+  const long long items = (long long)S * nkv * max_pages, few = (items + 7) / 8;         // (the fewest warps of a block are 8)
+  return kd_by_pair(S, nkv, max_pages) ? S * nkv : (int)max(1ll, min((long long)sx_sm_count(), few));
+}
+// kernels that a launch makes, and floats of `part` it needs
+extern "C" int sx_kv8_decode_plan(int S, int nh, int nkv, int hd, int max_pages, long long* floats) {
+  if (nkv <= 0) return 0;
+  const int blocks = kd_blocks(S, nkv, max_pages);
+  *floats = (long long)blocks * (KD_MAX_WARPS + 2) * (nh / nkv) * (hd + 2);
+  return kd_by_pair(S, nkv, max_pages) || blocks == 1 ? 1 : 2;
+}
+
+// max_pages: no sequence has more visible pages
 extern "C" int sx_kv8_decode(const void* q, void* out, const void* k, const void* v, const void* k_exp, const void* v_exp, const int* seq_lens,
                              const int* block_table, int maxp, int S, int nh, int nkv, int hd, int n_pages, float scale, int window,
-                             const float* sinks, float* part, int max_pages, int min_pages, cudaStream_t stream) {
+                             const float* sinks, float* part, int max_pages, cudaStream_t stream) {
   if (S <= 0) return 0;
-  if ((hd != 64 && hd != 128) || nkv <= 0 || nh <= 0 || nh % nkv || nh / nkv > 16 || S >= KD_MAX_SEQS || n_pages <= 0 || maxp <= 0 || min_pages <= 0 ||
+  if ((hd != 64 && hd != 128) || nkv <= 0 || nh <= 0 || nh % nkv || nh / nkv > 16 || S >= KD_MAX_SEQS || n_pages <= 0 || maxp <= 0 || max_pages <= 0 ||
       (long long)S * nkv * maxp >= (1ll << 31) || (long long)S * nh >= (1ll << 31) || !part)
     return SX_ERR_SIZE;
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k | (uintptr_t)v | (uintptr_t)k_exp | (uintptr_t)v_exp | (uintptr_t)part) & 15) return SX_ERR_ALIGN;
   int* status = kd_status();
   if (!status) return SX_ERR_SIZE;
-  const long long items = (long long)S * nkv * max_pages;
-  const int blocks = (int)max(1ll, min((long long)sx_sm_count(), items));
   const KdArgs a = {(const bf16*)q, (bf16*)out, (const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)k_exp, (const uint8_t*)v_exp, seq_lens, block_table,
-                    sinks, part, status, maxp, n_pages, S, nh, nkv, window, blocks * KD_WARPS, min_pages, scale};
-  if (hd == 64) return nh / nkv > 8 ? kd_launch<64, true>(a, blocks, stream) : kd_launch<64, false>(a, blocks, stream);
-  return nh / nkv > 8 ? kd_launch<128, true>(a, blocks, stream) : kd_launch<128, false>(a, blocks, stream);
+                    sinks, part, status, maxp, n_pages, S, nh, nkv, window, kd_blocks(S, nkv, max_pages), 0, kd_by_pair(S, nkv, max_pages), scale};
+  if (hd == 64) return nh / nkv > 8 ? kd_launch<64, true>(a, stream) : kd_launch<64, false>(a, stream);
+  return nh / nkv > 8 ? kd_launch<128, true>(a, stream) : kd_launch<128, false>(a, stream);
 }

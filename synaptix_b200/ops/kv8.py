@@ -207,7 +207,6 @@ def kv8_rows(q: torch.Tensor, pages: KV8Pages, seq_lens: torch.Tensor, block_tab
 DECODE_HEAD_DIMS = (64, 128)
 DECODE_MAX_GROUP = 16
 DECODE_MAX_SEQS = 2047
-DECODE_MIN_PAGES = 1
 
 
 def kv8_decode_supported(dtype, nh: int, nkv: int, hd: int, S: int) -> bool:
@@ -219,12 +218,16 @@ def kv8_decode(q: torch.Tensor, pages: KV8Pages, seq_lens: torch.Tensor, block_t
                window: Optional[int], max_len: int, sinks: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One query token a sequence (row ``s`` of ``q``) on the tensor cores; sizes as ``kv8_decode_supported`` says."""
     n_pages, nkv, hd = pages.v.shape[:3]
+    S = q.shape[0]
+    max_pages = min(-(-max_len // PAGE), block_table.shape[1]) if window is None else min(-(-max_len // PAGE), block_table.shape[1], (window + 126) // PAGE)
+    floats = ctypes.c_longlong(0)
+    launches = fn("kv8_decode", "sx_kv8_decode_plan")(c_int(S), c_int(nh), c_int(nkv), c_int(hd), c_int(max_pages), ctypes.byref(floats))
     out = torch.empty_like(q)
-    part = torch.empty(sm_count(q.device) * 16 * (nh // nkv) * (hd + 2), dtype=torch.float32, device=q.device)
+    part = torch.empty(floats.value, dtype=torch.float32, device=q.device)
     check(fn("kv8_decode", "sx_kv8_decode")(
         ptr(q), ptr(out), ptr(pages.k), ptr(pages.v), ptr(pages.k_exp), ptr(pages.v_exp), ptr(seq_lens), ptr(block_table), c_int(block_table.shape[1]),
-        c_int(q.shape[0]), c_int(nh), c_int(nkv), c_int(hd), c_int(n_pages), c_float(scale), c_int(window or 0), ptr(sinks), ptr(part),
-        c_int(-(-min(max_len, (window or max_len) + PAGE) // PAGE)), c_int(DECODE_MIN_PAGES), stream()), "kv8_attention", launches=2)
+        c_int(S), c_int(nh), c_int(nkv), c_int(hd), c_int(n_pages), c_float(scale), c_int(window or 0), ptr(sinks), ptr(part), c_int(max_pages), stream()),
+        "kv8_attention", launches=launches)
     return out
 
 

@@ -36,7 +36,7 @@ def quantise(x):
     scale = torch.ldexp(torch.ones_like(a), e)
     v = round_e4m3(torch.where(finite[..., None], x / scale[..., None], 0.0))
     value = torch.where(finite[..., None], v * scale[..., None], math.nan)
-    return code_of(v), torch.where(finite, e + 127, 255).to(torch.uint8), value
+    return torch.where(finite[..., None], code_of(v), 127).to(torch.uint8), torch.where(finite, e + 127, 255).to(torch.uint8), value
 
 
 class Held:
