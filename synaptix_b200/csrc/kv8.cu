@@ -97,6 +97,210 @@ __global__ void __launch_bounds__(KV8_WARPS * 32) kv8_prepare_kernel(
   }
 }
 
+// The same for many tokens at head size 64 or 128, the whole head rotated or nothing.  Blocks of one kind take a token's q and k heads each, 16
+// elements a lane (8 of either half of the head, so that rotation stays within the lane and a key's codes leave as 8-byte stores).  Blocks of the
+// other kind take values: a value page lies dim by dim, and a token alone would write a byte here and there (measured: 338 us for 8,191 tokens of
+// 48 heads of 128, where bytes take 28.6).  A thread has two dims of up to 16 tokens that share 16 neighbouring places of a page, finds the rows'
+// largest magnitudes with its warp by 31 exchanges for all 16 tokens, and stores 16 bytes a dim.
+template <typename T> struct Kv8Vec;
+template <> struct Kv8Vec<bf16> {
+  static __device__ __forceinline__ void load8(const bf16* p, float (&x)[8]) {
+    const uint4 w = *reinterpret_cast<const uint4*>(p);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(u[i] << 16);
+      x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ void store8(bf16* p, const float (&x)[8]) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      u[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+  static __device__ __forceinline__ float2 load2(const bf16* p) {
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  }
+};
+template <> struct Kv8Vec<float> {
+  static __device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float4 v = reinterpret_cast<const float4*>(p)[i];
+      x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
+    }
+  }
+  static __device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) reinterpret_cast<float4*>(p)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+  }
+  static __device__ __forceinline__ float2 load2(const float* p) { return *reinterpret_cast<const float2*>(p); }
+};
+__device__ __forceinline__ uint32_t kv8_magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }   // ordered as the magnitudes are, NaN above infinity
+__device__ __forceinline__ int kv8_exponent_of(uint32_t top) { return kv8_exponent(__uint_as_float(top), top < 0x7f800000u); }
+
+#define KV8_TOKENS 16
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) kv8_prepare_wide_kernel(
+    const T* __restrict__ qkv, T* __restrict__ q_out, uint8_t* __restrict__ k_pages, uint8_t* __restrict__ v_pages,
+    uint8_t* __restrict__ k_exp, uint8_t* __restrict__ v_exp, const float* __restrict__ wq, const float* __restrict__ wk,
+    const float* __restrict__ inv_freq, float eps, const int* __restrict__ positions, const int* __restrict__ seq_of_token,
+    const int* __restrict__ block_table, int maxp, int nh, int nkv, int n_pages, int row, int n_tokens) {
+  constexpr int HALF = HD / 2, LPH = HD / 16;                    // lanes a head
+  __shared__ float s_cs[HALF], s_sn[HALF];
+  __shared__ uint32_t s_top[8][KV8_TOKENS];
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto page_of = [&](int t, int pos) {
+    const int page = (unsigned)(pos >> 6) < (unsigned)maxp ? block_table[(size_t)seq_of_token[t] * maxp + (pos >> 6)] : -1;
+    return (unsigned)page < (unsigned)n_pages ? page : -1;
+  };
+  if (blockIdx.x < n_tokens) {
+    const int t = blockIdx.x, pos = positions[t], page = k_pages ? page_of(t, pos) : -1;
+    for (int i = threadIdx.x; i < HALF; i += 256) {
+      const float2 r = inv_freq ? kv8_turn(pos, inv_freq[i]) : make_float2(1.f, 0.f);
+      s_cs[i] = r.x;
+      s_sn[i] = r.y;
+    }
+    __syncthreads();
+    const int heads = nh + (k_pages ? nkv : 0), e0 = (lane % LPH) * 8;
+    for (int head = threadIdx.x / LPH; head < (heads + 32 / LPH - 1) / (32 / LPH) * (32 / LPH); head += 256 / LPH) {
+      const bool live = head < heads, is_q = head < nh;
+      float a[8], b[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
+      if (live) {
+        const T* src = qkv + (size_t)t * row + (size_t)head * HD + e0;
+        Kv8Vec<T>::load8(src, a);
+        Kv8Vec<T>::load8(src + HALF, b);
+      }
+      const float* gain = is_q ? wq : wk;
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
+#pragma unroll
+      for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (gain) {
+        const float inv = rsqrtf(ss / (float)HD + eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          a[i] *= inv * gain[e0 + i];
+          b[i] *= inv * gain[e0 + i + HALF];
+        }
+      }
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = a[i] * s_cs[e0 + i] - b[i] * s_sn[e0 + i], y = a[i] * s_sn[e0 + i] + b[i] * s_cs[e0 + i];
+        a[i] = inv_freq ? x : a[i];
+        b[i] = inv_freq ? y : b[i];
+        top = max(top, max(kv8_magnitude(a[i]), kv8_magnitude(b[i])));
+      }
+#pragma unroll
+      for (int o = LPH / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (!live) continue;
+      if (is_q) {
+        T* dst = q_out + ((size_t)t * nh + head) * HD + e0;
+        Kv8Vec<T>::store8(dst, a);
+        Kv8Vec<T>::store8(dst + HALF, b);
+      } else if (page >= 0) {
+        const int e = kv8_exponent_of(top), key = pos & (SX_PAGE - 1);
+        const float inverse = kv8_inverse(e);
+        const size_t place = (size_t)page * nkv + (head - nh);
+        uint32_t ca[2], cb[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          ca[i] = kv8_codes2(a[4 * i] * inverse, a[4 * i + 1] * inverse) | kv8_codes2(a[4 * i + 2] * inverse, a[4 * i + 3] * inverse) << 16;
+          cb[i] = kv8_codes2(b[4 * i] * inverse, b[4 * i + 1] * inverse) | kv8_codes2(b[4 * i + 2] * inverse, b[4 * i + 3] * inverse) << 16;
+        }
+        uint8_t* dst = k_pages + place * SX_PAGE * HD;
+        *reinterpret_cast<uint2*>(dst + kv8_k_at(key, e0, 64)) = make_uint2(ca[0], ca[1]);
+        *reinterpret_cast<uint2*>(dst + kv8_k_at(key, e0 + HALF, 64)) = make_uint2(cb[0], cb[1]);
+        if (e0 == 0) k_exp[place * SX_PAGE + key] = (uint8_t)e;
+      }
+    }
+    return;
+  }
+  // ---- values: the groups of tokens that share 16 places of a page and begin in this block's 16 tokens
+  constexpr int WPH = HALF / 32;                                 // warps a head, two dims a lane
+  const int t0 = (blockIdx.x - n_tokens) * KV8_TOKENS, t_end = min(t0 + KV8_TOKENS, n_tokens);
+  auto begins = [&](int t) {                                     // (a group is a run of one sequence's neighbouring positions)
+    return t == 0 || (positions[t] & (KV8_TOKENS - 1)) == 0 || seq_of_token[t] != seq_of_token[t - 1] || positions[t] != positions[t - 1] + 1;
+  };
+  for (int t = t0; t < t_end; ++t) {
+    if (!begins(t)) continue;
+    int n = 1;
+    while (n < KV8_TOKENS && t + n < n_tokens && !begins(t + n)) ++n;
+    const int pos = positions[t], page = page_of(t, pos), key = pos & (SX_PAGE - 1);
+    if (page < 0) continue;
+    for (int h0 = 0; h0 < nkv; h0 += 8 / WPH) {
+      const int h = h0 + warp / WPH, d = (warp % WPH) * 64 + 2 * lane;
+      float2 x[KV8_TOKENS];
+      uint32_t top[KV8_TOKENS];
+      const T* src = qkv + (size_t)t * row + (size_t)(nh + nkv + h) * HD + d;
+#pragma unroll
+      for (int i = 0; i < KV8_TOKENS; ++i) x[i] = h < nkv && i < n ? Kv8Vec<T>::load2(src + (size_t)i * row) : make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < KV8_TOKENS; ++i) top[i] = max(kv8_magnitude(x[i].x), kv8_magnitude(x[i].y));
+      // the warp's largest of each token: after the exchanges lane's belongs to token lane >> 1
+      int off = 16;
+#pragma unroll
+      for (int m = KV8_TOKENS; m > 1; m >>= 1, off >>= 1) {
+        const bool up = lane & off;
+#pragma unroll
+        for (int i = 0; i < m / 2; ++i) {
+          const uint32_t keep = up ? top[i + m / 2] : top[i], send = up ? top[i] : top[i + m / 2];
+          top[i] = max(keep, __shfl_xor_sync(0xffffffffu, send, off));
+        }
+      }
+      top[0] = max(top[0], __shfl_xor_sync(0xffffffffu, top[0], 1));
+      if (WPH > 1) {
+        __syncthreads();
+        if (!(lane & 1)) s_top[warp][lane >> 1] = top[0];
+        __syncthreads();
+        top[0] = max(s_top[warp & ~(WPH - 1)][lane >> 1], s_top[warp | (WPH - 1)][lane >> 1]);
+      }
+      const int mine = kv8_exponent_of(top[0]);
+      const size_t place = (size_t)page * nkv + min(h, nkv - 1);
+      uint32_t lo[4], hi[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        lo[w] = hi[w] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const int k = 4 * w + i;
+          const float f0 = kv8_inverse(__shfl_sync(0xffffffffu, mine, 2 * k)), f1 = kv8_inverse(__shfl_sync(0xffffffffu, mine, 2 * k + 2));
+          lo[w] |= kv8_codes2(x[k].x * f0, x[k + 1].x * f1) << (8 * i);
+          hi[w] |= kv8_codes2(x[k].y * f0, x[k + 1].y * f1) << (8 * i);
+        }
+      }
+      if (h >= nkv) continue;
+      uint8_t* dst = v_pages + place * SX_PAGE * HD + kv8_v_at(key, d);
+      if (n == KV8_TOKENS) {                                     // (begins at a multiple of 16)
+        *reinterpret_cast<uint4*>(dst) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        *reinterpret_cast<uint4*>(dst + SX_PAGE) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < KV8_TOKENS; ++i)
+          if (i < n) {
+            dst[i] = (uint8_t)(lo[i >> 2] >> (8 * (i & 3)));
+            dst[SX_PAGE + i] = (uint8_t)(hi[i >> 2] >> (8 * (i & 3)));
+          }
+      }
+      if (warp % WPH == 0 && !(lane & 1) && (lane >> 1) < n) v_exp[place * SX_PAGE + key + (lane >> 1)] = (uint8_t)mine;
+    }
+  }
+}
+
+// fewer tokens than this: a warp a head (a block of 16 tokens' values waits for 16 rows one after the other)
+#define KV8_WIDE_MIN_TOKENS 64
+
 // qkv: rows of `row` elements, q heads, k heads and v heads first (q heads alone where k_pages is null and nothing is written)
 extern "C" int sx_kv8_prepare(const void* qkv, void* q_out, void* k_pages, void* v_pages, void* k_exp, void* v_exp, const float* wq,
                               const float* wk, const float* inv_freq, int rotary_dim, float eps, const int* positions,
@@ -107,6 +311,16 @@ extern "C" int sx_kv8_prepare(const void* qkv, void* q_out, void* k_pages, void*
     return SX_ERR_SIZE;
   const int heads = nh + (k_pages ? 2 * nkv : 0), groups = (heads + KV8_WARPS - 1) / KV8_WARPS;
   if (heads == 0) return 0;
+  const size_t es = dt == SX_F32 ? 4 : 2;
+  if (n_tokens >= KV8_WIDE_MIN_TOKENS && (hd == 64 || hd == 128) && (!inv_freq || rotary_dim == hd) && (dt == SX_F32 || dt == SX_BF16) &&
+      !(((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_pages | (uintptr_t)v_pages | row * es) & 15)) {
+    const dim3 blocks(n_tokens + (k_pages ? (n_tokens + KV8_TOKENS - 1) / KV8_TOKENS : 0));
+#define KV8_WIDE(T, HD)                                                                                                                              \
+  sx_launch(kv8_prepare_wide_kernel<T, HD>, blocks, dim3(256), 0, stream, (const T*)qkv, (T*)q_out, (uint8_t*)k_pages, (uint8_t*)v_pages,             \
+            (uint8_t*)k_exp, (uint8_t*)v_exp, wq, wk, inv_freq, eps, positions, seq_of_token, block_table, maxp, nh, nkv, n_pages, row, n_tokens)
+    if (dt == SX_F32) return hd == 64 ? KV8_WIDE(float, 64) : KV8_WIDE(float, 128);
+    return hd == 64 ? KV8_WIDE(bf16, 64) : KV8_WIDE(bf16, 128);
+  }
   // few tokens: a block for every eight heads; many: a block walks its token's heads and makes the angles once
   const dim3 grid(n_tokens, n_tokens * groups <= 4 * sx_sm_count() ? groups : 1);
   if (dt == SX_F32)
@@ -122,41 +336,65 @@ extern "C" int sx_kv8_prepare(const void* qkv, void* q_out, void* k_pages, void*
 
 // ---------------------------------------------------------------------------------------
 // Pages read back: page i of the result holds page page_idx[i] of sequence page_seq[i] as [kv heads][64][hd] in T, rows
-// behind the sequence's end as zeros.  A block a (page, kv head) and keys or values; values turn around in shared memory.
+// behind the sequence's end as zeros.  A block a (page, kv head) and keys or values, bound by its bytes.  A lane of keys takes 8 codes of a
+// row at a time (16 bytes of bfloat16); a lane of values takes 8 dims of 4 keys, one word a dim, turns the bytes around in registers and
+// stores 16 bytes a key: 8 lanes beside one another read 32 bytes of a dim, 4 write 64 of a key.
 // ---------------------------------------------------------------------------------------
+template <typename T> __device__ __forceinline__ void kv8_store8(T* dst, const uint32_t (&pairs)[4], float f, bool held) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = kv8_float2(pairs[i]);
+    x[2 * i] = held ? v.x * f : 0.f;
+    x[2 * i + 1] = held ? v.y * f : 0.f;
+  }
+  Kv8Vec<T>::store8(dst, x);
+}
 template <typename T>
 __global__ void __launch_bounds__(256) kv8_read_kernel(
     const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages, const uint8_t* __restrict__ k_exp,
     const uint8_t* __restrict__ v_exp, T* __restrict__ k_out, T* __restrict__ v_out, const int* __restrict__ page_seq,
     const int* __restrict__ page_idx, const int* __restrict__ seq_lens, const int* __restrict__ block_table, int maxp, int nkv, int hd,
     int n_pages) {
-  __shared__ uint8_t s_c[SX_PAGE][KV8_MAX_HD + 4];
   __shared__ float s_f[SX_PAGE];
   pdl_wait();
   pdl_trigger();
   const int i = blockIdx.x, kvh = blockIdx.y;
   const bool is_k = blockIdx.z == 0;
   const int s = page_seq[i], j = page_idx[i];
-  const int page = block_table[(size_t)s * maxp + j], held = min(SX_PAGE, max(0, seq_lens[s] - j * SX_PAGE));
+  const int page = block_table[(size_t)s * maxp + j];
   const bool ok = page >= 0 && page < n_pages;
+  const int held = ok ? min(SX_PAGE, max(0, seq_lens[s] - j * SX_PAGE)) : 0;
   const size_t from = (size_t)(ok ? page : 0) * nkv + kvh;
   const uint8_t* src = (is_k ? k_pages : v_pages) + from * SX_PAGE * hd;
   T* dst = (is_k ? k_out : v_out) + ((size_t)i * nkv + kvh) * SX_PAGE * hd;
-  const int cb = kv8_block(hd);
   if (threadIdx.x < SX_PAGE) s_f[threadIdx.x] = kv8_scale((is_k ? k_exp : v_exp)[from * SX_PAGE + threadIdx.x]);
-  for (int o = threadIdx.x * 16; o < SX_PAGE * hd; o += 256 * 16) {
-    const uint4 c = *reinterpret_cast<const uint4*>(src + o);
-    const uint8_t* b = reinterpret_cast<const uint8_t*>(&c);
-    for (int n = 0; n < 16; ++n) {
-      const int at = o + n;
-      if (is_k) s_c[at / cb % SX_PAGE][at / (cb * SX_PAGE) * cb + at % cb] = b[n];
-      else s_c[at % SX_PAGE][at / SX_PAGE] = b[n];
-    }
-  }
   __syncthreads();
-  for (int o = threadIdx.x; o < SX_PAGE * hd; o += 256) {
-    const int key = o / hd;
-    dst[o] = from_f32<T>(ok && key < held ? kv8_float2(s_c[key][o % hd]).x * s_f[key] : 0.f);
+  const int groups = hd / 8;                                     // of 8 dims
+  if (is_k) {
+    const int cb = kv8_block(hd);
+#pragma unroll 4
+    for (int o = threadIdx.x; o < SX_PAGE * groups; o += 256) {
+      const int key = o / groups, d = o % groups * 8;
+      const uint2 w = *reinterpret_cast<const uint2*>(src + kv8_k_at(key, d, cb));
+      const uint32_t pairs[4] = {w.x, w.x >> 16, w.y, w.y >> 16};
+      kv8_store8<T>(dst + key * hd + d, pairs, s_f[key], key < held);
+    }
+    return;
+  }
+  for (int o = threadIdx.x; o < (groups + 3) / 4 * 64; o += 256) {
+    const int key = ((o & 7) | (o >> 2 & 8)) * 4, group = (o >> 3 & 3) | (o >> 6) * 4;      // bits: 3 of the key's word, 2 of the group, 1 of the word, the group's rest
+    if (group >= groups) continue;
+    uint32_t w[8];
+#pragma unroll
+    for (int d = 0; d < 8; ++d) w[d] = *reinterpret_cast<const uint32_t*>(src + kv8_v_at(key, group * 8 + d));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t pairs[4];
+#pragma unroll
+      for (int d = 0; d < 4; ++d) pairs[d] = __byte_perm(w[2 * d], w[2 * d + 1], k | (4 + k) << 4);
+      kv8_store8<T>(dst + (key + k) * hd + group * 8, pairs, s_f[key + k], key + k < held);
+    }
   }
 }
 
