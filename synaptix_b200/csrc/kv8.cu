@@ -97,11 +97,12 @@ __global__ void __launch_bounds__(KV8_WARPS * 32) kv8_prepare_kernel(
   }
 }
 
-// The same for many tokens at head size 64 or 128, the whole head rotated or nothing.  Blocks of one kind take a token's q and k heads each, 16
-// elements a lane (8 of either half of the head, so that rotation stays within the lane and a key's codes leave as 8-byte stores).  Blocks of the
-// other kind take values: a value page lies dim by dim, and a token alone would write a byte here and there (measured: 338 us for 8,191 tokens of
-// 48 heads of 128, where bytes take 28.6).  A thread has two dims of up to 16 tokens that share 16 neighbouring places of a page, finds the rows'
-// largest magnitudes with its warp by 31 exchanges for all 16 tokens, and stores 16 bytes a dim.
+// The same for many tokens at head size 64 or 128, the whole head rotated or nothing, as two kernels.  One takes the q and k heads of four
+// tokens a block, 16 elements a lane (8 of either half of the head, so that rotation stays within the lane and a key's codes leave as 8-byte
+// stores); the block makes the four tokens' angles first, one or two a thread.  The other takes values: a value page lies dim by dim, and a token
+// alone would write a byte here and there (measured in all: 338 us for 8,191 tokens of 48 heads of 128, where bytes take 28.6).  There a thread has
+// two dims of up to 16 tokens that share 16 neighbouring places of a page, finds the rows' largest magnitudes with its warp by 31 exchanges for
+// all 16 tokens, and stores 16 bytes a dim.  (As one kernel its 124 registers left two blocks an SM and the q and k heads waited for themselves: 134 us.)
 template <typename T> struct Kv8Vec;
 template <> struct Kv8Vec<bf16> {
   static __device__ __forceinline__ void load8(const bf16* p, float (&x)[8]) {
@@ -144,92 +145,115 @@ template <> struct Kv8Vec<float> {
 __device__ __forceinline__ uint32_t kv8_magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }   // ordered as the magnitudes are, NaN above infinity
 __device__ __forceinline__ int kv8_exponent_of(uint32_t top) { return kv8_exponent(__uint_as_float(top), top < 0x7f800000u); }
 
+__device__ __forceinline__ int kv8_page_of(const int* positions, const int* seq_of_token, const int* block_table, int maxp, int n_pages, int t) {
+  const int pos = positions[t], page = (unsigned)(pos >> 6) < (unsigned)maxp ? block_table[(size_t)seq_of_token[t] * maxp + (pos >> 6)] : -1;
+  return (unsigned)page < (unsigned)n_pages ? page : -1;
+}
+
+#define KV8_QK_TOKENS 4
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) kv8_prepare_qk_kernel(
+    const T* __restrict__ qkv, T* __restrict__ q_out, uint8_t* __restrict__ k_pages, uint8_t* __restrict__ k_exp, const float* __restrict__ wq,
+    const float* __restrict__ wk, const float* __restrict__ inv_freq, float eps, const int* __restrict__ positions,
+    const int* __restrict__ seq_of_token, const int* __restrict__ block_table, int maxp, int nh, int nkv, int n_pages, int row, int n_tokens) {
+  constexpr int HALF = HD / 2, LPH = HD / 16, TOK = KV8_QK_TOKENS;       // lanes a head
+  __shared__ __align__(16) float s_cs[TOK][HALF], s_sn[TOK][HALF];
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, t0 = blockIdx.x * TOK, tokens = min(TOK, n_tokens - t0);
+  if (inv_freq)
+    for (int i = threadIdx.x; i < tokens * HALF; i += 256) {
+      const float2 r = kv8_turn(positions[t0 + i / HALF], inv_freq[i % HALF]);
+      s_cs[i / HALF][i % HALF] = r.x;
+      s_sn[i / HALF][i % HALF] = r.y;
+    }
+  __syncthreads();
+  const int heads = nh + (k_pages ? nkv : 0), all = tokens * heads, e0 = (lane % LPH) * 8;
+  for (int at = threadIdx.x / LPH; at < (all + 32 / LPH - 1) / (32 / LPH) * (32 / LPH); at += 256 / LPH) {
+    const bool live = at < all;
+    const int tok = live ? at / heads : 0, head = at - tok * heads, t = t0 + tok;
+    const bool is_q = head < nh;
+    float a[8], b[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
+    if (live) {
+      const T* src = qkv + (size_t)t * row + (size_t)head * HD + e0;
+      Kv8Vec<T>::load8(src, a);
+      Kv8Vec<T>::load8(src + HALF, b);
+    }
+    const float* gain = is_q ? wq : wk;
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
+#pragma unroll
+    for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (gain) {
+      const float inv = rsqrtf(ss / (float)HD + eps);
+      float ga[8], gb[8];
+      Kv8Vec<float>::load8(gain + e0, ga);
+      Kv8Vec<float>::load8(gain + e0 + HALF, gb);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        a[i] *= inv * ga[i];
+        b[i] *= inv * gb[i];
+      }
+    }
+    if (inv_freq) {
+      float cs[8], sn[8];
+      Kv8Vec<float>::load8(&s_cs[tok][e0], cs);
+      Kv8Vec<float>::load8(&s_sn[tok][e0], sn);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = a[i] * cs[i] - b[i] * sn[i], y = a[i] * sn[i] + b[i] * cs[i];
+        a[i] = x;
+        b[i] = y;
+      }
+    }
+    if (is_q) {
+      if (live) {
+        T* dst = q_out + ((size_t)t * nh + head) * HD + e0;
+        Kv8Vec<T>::store8(dst, a);
+        Kv8Vec<T>::store8(dst + HALF, b);
+      }
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, max(kv8_magnitude(a[i]), kv8_magnitude(b[i])));
+#pragma unroll
+    for (int o = LPH / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (live && !is_q) {
+      const int page = kv8_page_of(positions, seq_of_token, block_table, maxp, n_pages, t);
+      if (page < 0) continue;
+      const int e = kv8_exponent_of(top), key = positions[t] & (SX_PAGE - 1);
+      const float inverse = kv8_inverse(e);
+      const size_t place = (size_t)page * nkv + (head - nh);
+      uint32_t ca[2], cb[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        ca[i] = kv8_codes2(a[4 * i] * inverse, a[4 * i + 1] * inverse) | kv8_codes2(a[4 * i + 2] * inverse, a[4 * i + 3] * inverse) << 16;
+        cb[i] = kv8_codes2(b[4 * i] * inverse, b[4 * i + 1] * inverse) | kv8_codes2(b[4 * i + 2] * inverse, b[4 * i + 3] * inverse) << 16;
+      }
+      uint8_t* dst = k_pages + place * SX_PAGE * HD;
+      *reinterpret_cast<uint2*>(dst + kv8_k_at(key, e0, 64)) = make_uint2(ca[0], ca[1]);
+      *reinterpret_cast<uint2*>(dst + kv8_k_at(key, e0 + HALF, 64)) = make_uint2(cb[0], cb[1]);
+      if (e0 == 0) k_exp[place * SX_PAGE + key] = (uint8_t)e;
+    }
+  }
+}
+
 #define KV8_TOKENS 16
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) kv8_prepare_wide_kernel(
-    const T* __restrict__ qkv, T* __restrict__ q_out, uint8_t* __restrict__ k_pages, uint8_t* __restrict__ v_pages,
-    uint8_t* __restrict__ k_exp, uint8_t* __restrict__ v_exp, const float* __restrict__ wq, const float* __restrict__ wk,
-    const float* __restrict__ inv_freq, float eps, const int* __restrict__ positions, const int* __restrict__ seq_of_token,
-    const int* __restrict__ block_table, int maxp, int nh, int nkv, int n_pages, int row, int n_tokens) {
-  constexpr int HALF = HD / 2, LPH = HD / 16;                    // lanes a head
-  __shared__ float s_cs[HALF], s_sn[HALF];
+__global__ void __launch_bounds__(256) kv8_prepare_v_kernel(
+    const T* __restrict__ qkv, uint8_t* __restrict__ v_pages, uint8_t* __restrict__ v_exp, const int* __restrict__ positions,
+    const int* __restrict__ seq_of_token, const int* __restrict__ block_table, int maxp, int nh, int nkv, int n_pages, int row, int n_tokens) {
+  constexpr int HALF = HD / 2;
   __shared__ uint32_t s_top[8][KV8_TOKENS];
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto page_of = [&](int t, int pos) {
-    const int page = (unsigned)(pos >> 6) < (unsigned)maxp ? block_table[(size_t)seq_of_token[t] * maxp + (pos >> 6)] : -1;
-    return (unsigned)page < (unsigned)n_pages ? page : -1;
-  };
-  if (blockIdx.x < n_tokens) {
-    const int t = blockIdx.x, pos = positions[t], page = k_pages ? page_of(t, pos) : -1;
-    for (int i = threadIdx.x; i < HALF; i += 256) {
-      const float2 r = inv_freq ? kv8_turn(pos, inv_freq[i]) : make_float2(1.f, 0.f);
-      s_cs[i] = r.x;
-      s_sn[i] = r.y;
-    }
-    __syncthreads();
-    const int heads = nh + (k_pages ? nkv : 0), e0 = (lane % LPH) * 8;
-    for (int head = threadIdx.x / LPH; head < (heads + 32 / LPH - 1) / (32 / LPH) * (32 / LPH); head += 256 / LPH) {
-      const bool live = head < heads, is_q = head < nh;
-      float a[8], b[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
-      if (live) {
-        const T* src = qkv + (size_t)t * row + (size_t)head * HD + e0;
-        Kv8Vec<T>::load8(src, a);
-        Kv8Vec<T>::load8(src + HALF, b);
-      }
-      const float* gain = is_q ? wq : wk;
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
-#pragma unroll
-      for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (gain) {
-        const float inv = rsqrtf(ss / (float)HD + eps);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          a[i] *= inv * gain[e0 + i];
-          b[i] *= inv * gain[e0 + i + HALF];
-        }
-      }
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x = a[i] * s_cs[e0 + i] - b[i] * s_sn[e0 + i], y = a[i] * s_sn[e0 + i] + b[i] * s_cs[e0 + i];
-        a[i] = inv_freq ? x : a[i];
-        b[i] = inv_freq ? y : b[i];
-        top = max(top, max(kv8_magnitude(a[i]), kv8_magnitude(b[i])));
-      }
-#pragma unroll
-      for (int o = LPH / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (!live) continue;
-      if (is_q) {
-        T* dst = q_out + ((size_t)t * nh + head) * HD + e0;
-        Kv8Vec<T>::store8(dst, a);
-        Kv8Vec<T>::store8(dst + HALF, b);
-      } else if (page >= 0) {
-        const int e = kv8_exponent_of(top), key = pos & (SX_PAGE - 1);
-        const float inverse = kv8_inverse(e);
-        const size_t place = (size_t)page * nkv + (head - nh);
-        uint32_t ca[2], cb[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          ca[i] = kv8_codes2(a[4 * i] * inverse, a[4 * i + 1] * inverse) | kv8_codes2(a[4 * i + 2] * inverse, a[4 * i + 3] * inverse) << 16;
-          cb[i] = kv8_codes2(b[4 * i] * inverse, b[4 * i + 1] * inverse) | kv8_codes2(b[4 * i + 2] * inverse, b[4 * i + 3] * inverse) << 16;
-        }
-        uint8_t* dst = k_pages + place * SX_PAGE * HD;
-        *reinterpret_cast<uint2*>(dst + kv8_k_at(key, e0, 64)) = make_uint2(ca[0], ca[1]);
-        *reinterpret_cast<uint2*>(dst + kv8_k_at(key, e0 + HALF, 64)) = make_uint2(cb[0], cb[1]);
-        if (e0 == 0) k_exp[place * SX_PAGE + key] = (uint8_t)e;
-      }
-    }
-    return;
-  }
   // ---- values: the groups of tokens that share 16 places of a page and begin in this block's 16 tokens
   constexpr int WPH = HALF / 32;                                 // warps a head, two dims a lane
-  const int t0 = (blockIdx.x - n_tokens) * KV8_TOKENS, t_end = min(t0 + KV8_TOKENS, n_tokens);
+  const int t0 = blockIdx.x * KV8_TOKENS, t_end = min(t0 + KV8_TOKENS, n_tokens);
   auto begins = [&](int t) {                                     // (a group is a run of one sequence's neighbouring positions)
     return t == 0 || (positions[t] & (KV8_TOKENS - 1)) == 0 || seq_of_token[t] != seq_of_token[t - 1] || positions[t] != positions[t - 1] + 1;
   };
@@ -237,9 +261,9 @@ __global__ void __launch_bounds__(256) kv8_prepare_wide_kernel(
     if (!begins(t)) continue;
     int n = 1;
     while (n < KV8_TOKENS && t + n < n_tokens && !begins(t + n)) ++n;
-    const int pos = positions[t], page = page_of(t, pos), key = pos & (SX_PAGE - 1);
+    const int page = kv8_page_of(positions, seq_of_token, block_table, maxp, n_pages, t), key = positions[t] & (SX_PAGE - 1);
     if (page < 0) continue;
-    for (int h0 = 0; h0 < nkv; h0 += 8 / WPH) {
+    for (int h0 = blockIdx.y * (8 / WPH); h0 < nkv; h0 += gridDim.y * (8 / WPH)) {
       const int h = h0 + warp / WPH, d = (warp % WPH) * 64 + 2 * lane;
       float2 x[KV8_TOKENS];
       uint32_t top[KV8_TOKENS];
@@ -298,28 +322,36 @@ __global__ void __launch_bounds__(256) kv8_prepare_wide_kernel(
   }
 }
 
-// fewer tokens than this: a warp a head (a block of 16 tokens' values waits for 16 rows one after the other)
-#define KV8_WIDE_MIN_TOKENS 64
-
-// qkv: rows of `row` elements, q heads, k heads and v heads first (q heads alone where k_pages is null and nothing is written)
+// qkv: rows of `row` elements, q heads, k heads and v heads first (q heads alone where k_pages is null and nothing is written).
+// wide: by the kernels for many tokens
 extern "C" int sx_kv8_prepare(const void* qkv, void* q_out, void* k_pages, void* v_pages, void* k_exp, void* v_exp, const float* wq,
                               const float* wk, const float* inv_freq, int rotary_dim, float eps, const int* positions,
                               const int* seq_of_token, const int* block_table, int maxp, int n_tokens, int nh, int nkv, int hd,
-                              int n_pages, int row, int dt, cudaStream_t stream) {
+                              int n_pages, int row, int wide, int dt, cudaStream_t stream) {
   if (n_tokens <= 0) return 0;
   if (hd <= 0 || hd % 16 || hd > KV8_MAX_HD || rotary_dim < 0 || rotary_dim > hd || (rotary_dim & 1) || nh < 0 || nkv <= 0)
     return SX_ERR_SIZE;
   const int heads = nh + (k_pages ? 2 * nkv : 0), groups = (heads + KV8_WARPS - 1) / KV8_WARPS;
   if (heads == 0) return 0;
   const size_t es = dt == SX_F32 ? 4 : 2;
-  if (n_tokens >= KV8_WIDE_MIN_TOKENS && (hd == 64 || hd == 128) && (!inv_freq || rotary_dim == hd) && (dt == SX_F32 || dt == SX_BF16) &&
-      !(((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_pages | (uintptr_t)v_pages | row * es) & 15)) {
-    const dim3 blocks(n_tokens + (k_pages ? (n_tokens + KV8_TOKENS - 1) / KV8_TOKENS : 0));
-#define KV8_WIDE(T, HD)                                                                                                                              \
-  sx_launch(kv8_prepare_wide_kernel<T, HD>, blocks, dim3(256), 0, stream, (const T*)qkv, (T*)q_out, (uint8_t*)k_pages, (uint8_t*)v_pages,             \
-            (uint8_t*)k_exp, (uint8_t*)v_exp, wq, wk, inv_freq, eps, positions, seq_of_token, block_table, maxp, nh, nkv, n_pages, row, n_tokens)
-    if (dt == SX_F32) return hd == 64 ? KV8_WIDE(float, 64) : KV8_WIDE(float, 128);
-    return hd == 64 ? KV8_WIDE(bf16, 64) : KV8_WIDE(bf16, 128);
+  if (wide) {
+    if ((hd != 64 && hd != 128) || (inv_freq && rotary_dim != hd)) return SX_ERR_SIZE;
+    if (dt != SX_F32 && dt != SX_BF16) return SX_ERR_DTYPE;
+    if (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)wq | (uintptr_t)wk | row * es) & 15) return SX_ERR_ALIGN;
+    int rc = 0;
+    const dim3 qk((n_tokens + KV8_QK_TOKENS - 1) / KV8_QK_TOKENS), v((n_tokens + KV8_TOKENS - 1) / KV8_TOKENS, (nkv * (hd / 64) + 7) / 8);
+#define KV8_WIDE(T, HD)                                                                                                                                \
+  rc = sx_launch(kv8_prepare_qk_kernel<T, HD>, qk, dim3(256), 0, stream, (const T*)qkv, (T*)q_out, (uint8_t*)k_pages, (uint8_t*)k_exp, wq, wk, inv_freq,  \
+                 eps, positions, seq_of_token, block_table, maxp, nh, nkv, n_pages, row, n_tokens);                                                     \
+  if (!rc && v_pages)                                                                                                                                  \
+    rc = sx_launch(kv8_prepare_v_kernel<T, HD>, v, dim3(256), 0, stream, (const T*)qkv, (uint8_t*)v_pages, (uint8_t*)v_exp, positions, seq_of_token,     \
+                   block_table, maxp, nh, nkv, n_pages, row, n_tokens);
+    if (dt == SX_F32) {
+      if (hd == 64) { KV8_WIDE(float, 64) } else { KV8_WIDE(float, 128) }
+    } else {
+      if (hd == 64) { KV8_WIDE(bf16, 64) } else { KV8_WIDE(bf16, 128) }
+    }
+    return rc;
   }
   // few tokens: a block for every eight heads; many: a block walks its token's heads and makes the angles once
   const dim3 grid(n_tokens, n_tokens * groups <= 4 * sx_sm_count() ? groups : 1);

@@ -12,8 +12,10 @@ from typing import NamedTuple, Optional, Tuple
 import numpy as np
 import torch
 
-from ._lib import KernelError, c_float, c_int, check, dt_code, fn, ptr, require_cuda, stream
+from ._lib import KernelError, c_int, check, dt_code, fn, good, launcher, raw_stream, require_cuda
 from .decode import sm_count
+
+current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 PAGE = 64
 MAX_HEAD_DIM = 256
@@ -48,36 +50,47 @@ def kv8_shapes(n_pages: int, nkv: int, hd: int) -> Tuple[tuple, tuple, tuple]:
 
 
 def _check_pages(pages: KV8Pages, what: str, nkv: Optional[int] = None, hd: Optional[int] = None) -> Tuple[int, int, int]:
-    if any(t.dtype != torch.uint8 for t in pages):
+    k, v, ke, ve = pages
+    u8 = torch.uint8
+    if not (k.dtype == v.dtype == ke.dtype == ve.dtype == u8):
         raise KernelError(f"{what}: codes and exponents are uint8")
-    if pages.v.dim() != 4:
+    if v.dim() != 4:
         raise KernelError(f"{what}: values are [n_pages, kv heads, head size, 64]")
-    n, kv, d = pages.v.shape[:3]
+    n, kv, d, page = v.shape
     if (nkv is not None and nkv != kv) or (hd is not None and hd != d):
         raise KernelError(f"{what}: the pages hold {kv} heads of {d}, not {nkv} of {hd}")
     if not kv8_supported(d):
         raise KernelError(f"{what}: head sizes are multiples of 16 up to {MAX_HEAD_DIM}")
-    ks, vs, es = kv8_shapes(n, kv, d)
-    if tuple(pages.k.shape) != ks or tuple(pages.v.shape) != vs or tuple(pages.k_exp.shape) != es or tuple(pages.v_exp.shape) != es:
-        raise KernelError(f"{what}: codes or exponents have the wrong shape (want {ks}, {vs}, {es})")
+    b = 64 if d % 64 == 0 else 32 if d % 32 == 0 else 16
+    if page != PAGE or k.shape != (n, kv, d // b, PAGE, b) or ke.shape != (n, kv, PAGE) or ve.shape != (n, kv, PAGE):
+        raise KernelError(f"{what}: codes or exponents have the wrong shape (want %s, %s, %s)" % kv8_shapes(n, kv, d))
     if n < 1 or kv < 1:
         raise KernelError(f"{what}: no pages, or no heads")
     return n, kv, d
 
 
-def _check_index(what: str, *tensors: torch.Tensor) -> None:
-    if any(t.dtype != torch.int32 for t in tensors):
-        raise KernelError(f"{what}: index tensors are int32")
-
-
 def _check_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
     """Behind all other checks: contiguous tensors of the current CUDA device."""
-    device = next(t.device for t in tensors if t is not None)
-    if any(t is not None and t.device != device for t in tensors):
-        raise KernelError(f"{what}: tensors lie on several devices")
-    require_cuda(*tensors)
-    if device.index is not None and device.index != torch.cuda.current_device():
-        raise KernelError(f"{what}: the tensors lie on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not good(t):
+            require_cuda(t)
+        if device is None:
+            device = t.get_device()
+        elif t.get_device() != device:
+            raise KernelError(f"{what}: tensors lie on several devices")
+    if device != current_device():
+        raise KernelError(f"{what}: the tensors lie on cuda:{device}, the current device is cuda:{current_device()}")
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+# at least this many tokens: the kernels that take four tokens' queries and keys, and 16 tokens' values, a block
+WIDE_MIN_TOKENS = 64
 
 
 def kv8_prepare(qkv: torch.Tensor, q_out: Optional[torch.Tensor], pages: Optional[KV8Pages], wq: Optional[torch.Tensor],
@@ -91,33 +104,40 @@ def kv8_prepare(qkv: torch.Tensor, q_out: Optional[torch.Tensor], pages: Optiona
     go to ``q_out [T, nh * hd]`` in ``qkv``'s dtype (``nh = 0``: none); keys and values into the pages of each token's sequence at its position.
     Two tokens of a call never share a sequence and a position.  Without ``pages`` nothing is written (a layer that reads another layer's
     cache; ``qkv`` may then hold the q heads alone)."""
+    k = v = ke = ve = None
     n_pages = 0
     if pages is not None:
         n_pages, _, _ = _check_pages(pages, "kv8_prepare", nkv, hd)
+        k, v, ke, ve = pages
     elif not kv8_supported(hd):
         raise KernelError(f"kv8_prepare: head sizes are multiples of 16 up to {MAX_HEAD_DIM}")
-    _check_index("kv8_prepare", positions, seq_of_token, block_table)
-    if qkv.dim() != 2 or block_table.dim() != 2 or positions.numel() < qkv.shape[0] or seq_of_token.numel() < qkv.shape[0]:
+    if not (positions.dtype == seq_of_token.dtype == block_table.dtype == torch.int32):
+        raise KernelError("kv8_prepare: index tensors are int32")
+    if qkv.dim() != 2 or block_table.dim() != 2:
         raise KernelError("kv8_prepare: qkv is [T, row], with a position and a sequence per token and a table [sequences, pages]")
     T, row = qkv.shape
+    if positions.numel() < T or seq_of_token.numel() < T:
+        raise KernelError("kv8_prepare: qkv is [T, row], with a position and a sequence per token and a table [sequences, pages]")
     if nh < 0 or nkv < 1 or col < 0 or col + (nh + (2 * nkv if pages is not None else 0)) * hd > row:
         raise KernelError("kv8_prepare: the heads do not fit the rows of qkv")
-    if nh and (q_out is None or q_out.dtype != qkv.dtype or tuple(q_out.shape) != (T, nh * hd)):
+    if nh and (q_out is None or q_out.dtype != qkv.dtype or q_out.shape != (T, nh * hd)):
         raise KernelError("kv8_prepare: q_out is [T, nh * hd] in qkv's dtype")
-    if any(w is not None and (w.dtype != torch.float32 or w.numel() != hd) for w in (wq, wk)):
-        raise KernelError("kv8_prepare: gains are float32, one per element of a head")
+    for w in (wq, wk):
+        if w is not None and (w.dtype != torch.float32 or w.numel() != hd):
+            raise KernelError("kv8_prepare: gains are float32, one per element of a head")
     if inv_freq is None:
         rotary_dim = 0
     elif inv_freq.dtype != torch.float32 or rotary_dim % 2 or not 0 < rotary_dim <= hd or inv_freq.numel() != rotary_dim // 2:
         raise KernelError("kv8_prepare: inv_freq is float32 with a frequency per rotated pair of the head")
-    dt_code(qkv.dtype)
-    k, v, ke, ve = pages if pages is not None else (None,) * 4
+    dt = dt_code(qkv.dtype)
     _check_device("kv8_prepare", qkv, q_out, k, v, ke, ve, wq, wk, inv_freq, positions, seq_of_token, block_table)
-    check(fn("kv8", "sx_kv8_prepare")(
-        ptr(qkv if col == 0 else qkv.view(-1)[col:]), ptr(q_out), ptr(k), ptr(v), ptr(ke), ptr(ve), ptr(wq), ptr(wk), ptr(inv_freq),
-        c_int(rotary_dim), c_float(eps), ptr(positions), ptr(seq_of_token), ptr(block_table), c_int(block_table.shape[1]), c_int(T), c_int(nh),
-        c_int(nkv), c_int(hd), c_int(n_pages), c_int(row), c_int(dt_code(qkv.dtype)), stream()), "kv8_prepare",
-        launches=1 if T and (nh or pages is not None) else 0)
+    es = qkv.element_size()
+    args = [qkv.data_ptr() + col * es, _ptr(q_out), _ptr(k), _ptr(v), _ptr(ke), _ptr(ve), _ptr(wq), _ptr(wk), _ptr(inv_freq)]
+    wide = (T >= WIDE_MIN_TOKENS and hd in (64, 128) and (inv_freq is None or rotary_dim == hd) and row * es % 16 == 0
+            and not any(p is not None and p % 16 for p in args))
+    check(launcher("kv8", "sx_kv8_prepare")(
+        *args, rotary_dim, eps, positions.data_ptr(), seq_of_token.data_ptr(), block_table.data_ptr(), block_table.shape[1], T, nh, nkv, hd, n_pages,
+        row, wide, dt, raw_stream()), "kv8_prepare", launches=0 if not T or (nh == 0 and k is None) else 2 if wide and k is not None else 1)
 
 
 def _read_plan(ctx, width: int, window: Optional[int], chunk: Optional[int], device):
@@ -144,13 +164,14 @@ def _read_plan(ctx, width: int, window: Optional[int], chunk: Optional[int], dev
 
 
 def _check_host(what: str, ctx, block_table: torch.Tensor) -> None:
-    _check_index(what, ctx.seq_lens, block_table)
+    if not (ctx.seq_lens.dtype == block_table.dtype == torch.int32):
+        raise KernelError(f"{what}: index tensors are int32")
     if ctx.host is None:
         raise KernelError(f"{what}: the step's lengths are not known on the host (a captured step)")
     lens = ctx.host["seq_lens"]
     if block_table.dim() != 2 or block_table.shape[0] < len(lens) or ctx.seq_lens.numel() < len(lens):
         raise KernelError(f"{what}: a row of the table and a length per sequence")
-    if any(-(-n // PAGE) > block_table.shape[1] for n in lens):
+    if lens and -(-max(lens) // PAGE) > block_table.shape[1]:
         raise KernelError(f"{what}: the table is too narrow for the sequences")
 
 
@@ -169,10 +190,9 @@ def kv8_read(pages: KV8Pages, ctx, block_table: torch.Tensor, dtype: torch.dtype
     table, seqs, idx, n = _read_plan(ctx, block_table.shape[1], window, chunk, pages.k.device)
     k = torch.empty((n, nkv, PAGE, hd), dtype=dtype, device=pages.k.device)
     v = torch.empty_like(k)
-    check(fn("kv8", "sx_kv8_read")(
-        ptr(pages.k), ptr(pages.v), ptr(pages.k_exp), ptr(pages.v_exp), ptr(k), ptr(v), ptr(seqs), ptr(idx), c_int(n), ptr(ctx.seq_lens),
-        ptr(block_table), c_int(block_table.shape[1]), c_int(nkv), c_int(hd), c_int(n_pages), c_int(dt), stream()), "kv8_read",
-        launches=1 if n else 0)
+    check(launcher("kv8", "sx_kv8_read")(
+        *(t.data_ptr() for t in pages), k.data_ptr(), v.data_ptr(), seqs.data_ptr(), idx.data_ptr(), n, ctx.seq_lens.data_ptr(),
+        block_table.data_ptr(), block_table.shape[1], nkv, hd, n_pages, dt, raw_stream()), "kv8_read", launches=1 if n else 0)
     return k, v, table
 
 
@@ -195,12 +215,10 @@ def kv8_rows(q: torch.Tensor, pages: KV8Pages, seq_lens: torch.Tensor, block_tab
     if splits > 1:
         part_o = torch.empty(S * nh * splits * hd, dtype=torch.float32, device=q.device)
         part_ml = torch.empty(S * nh * splits * 2, dtype=torch.float32, device=q.device)
-    o = out if out_col == 0 else out.view(-1)[out_col:]
-    check(fn("kv8", "sx_kv8_rows")(
-        ptr(q), ptr(o), ptr(pages.k), ptr(pages.v), ptr(pages.k_exp), ptr(pages.v_exp), ptr(seq_lens), ptr(block_table), c_int(block_table.shape[1]),
-        c_int(S), c_int(nh), c_int(nkv), c_int(hd), c_int(n_pages), c_float(scale), c_int(window or 0), c_float(softcap or 0.0), ptr(sinks),
-        c_int(chunk or 0), c_int(out.shape[1]), c_float(out_scale), c_int(splits), ptr(part_o), ptr(part_ml), c_int(dt_code(q.dtype)), stream()),
-        "kv8_attention", launches=2 if splits > 1 else 1)
+    check(launcher("kv8", "sx_kv8_rows")(
+        q.data_ptr(), out.data_ptr() + out_col * out.element_size(), *(t.data_ptr() for t in pages), seq_lens.data_ptr(), block_table.data_ptr(),
+        block_table.shape[1], S, nh, nkv, hd, n_pages, scale, window or 0, softcap or 0.0, _ptr(sinks), chunk or 0, out.shape[1], out_scale, splits,
+        _ptr(part_o), _ptr(part_ml), dt_code(q.dtype), raw_stream()), "kv8_attention", launches=2 if splits > 1 else 1)
     return out
 
 
@@ -214,20 +232,26 @@ def kv8_decode_supported(dtype, nh: int, nkv: int, hd: int, S: int) -> bool:
     return dtype == torch.bfloat16 and hd in DECODE_HEAD_DIMS and nh // nkv <= DECODE_MAX_GROUP and S <= DECODE_MAX_SEQS
 
 
+_DECODE_PLANS = {}              # of a shape: kernels, floats of scratch
+
+
 def kv8_decode(q: torch.Tensor, pages: KV8Pages, seq_lens: torch.Tensor, block_table: torch.Tensor, nh: int, scale: float,
                window: Optional[int], max_len: int, sinks: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One query token a sequence (row ``s`` of ``q``) on the tensor cores; sizes as ``kv8_decode_supported`` says."""
     n_pages, nkv, hd = pages.v.shape[:3]
     S = q.shape[0]
     max_pages = min(-(-max_len // PAGE), block_table.shape[1]) if window is None else min(-(-max_len // PAGE), block_table.shape[1], (window + 126) // PAGE)
-    floats = ctypes.c_longlong(0)
-    launches = fn("kv8_decode", "sx_kv8_decode_plan")(c_int(S), c_int(nh), c_int(nkv), c_int(hd), c_int(max_pages), ctypes.byref(floats))
+    shape = (S, nh, nkv, hd, max_pages, q.get_device())
+    plan = _DECODE_PLANS.get(shape)
+    if plan is None:
+        floats = ctypes.c_longlong(0)
+        launches = fn("kv8_decode", "sx_kv8_decode_plan")(*map(c_int, shape[:5]), ctypes.byref(floats))
+        plan = _DECODE_PLANS[shape] = (launches, floats.value)
     out = torch.empty_like(q)
-    part = torch.empty(floats.value, dtype=torch.float32, device=q.device)
-    check(fn("kv8_decode", "sx_kv8_decode")(
-        ptr(q), ptr(out), ptr(pages.k), ptr(pages.v), ptr(pages.k_exp), ptr(pages.v_exp), ptr(seq_lens), ptr(block_table), c_int(block_table.shape[1]),
-        c_int(S), c_int(nh), c_int(nkv), c_int(hd), c_int(n_pages), c_float(scale), c_int(window or 0), ptr(sinks), ptr(part), c_int(max_pages), stream()),
-        "kv8_attention", launches=launches)
+    part = torch.empty(plan[1], dtype=torch.float32, device=q.device)
+    check(launcher("kv8_decode", "sx_kv8_decode")(
+        q.data_ptr(), out.data_ptr(), *(t.data_ptr() for t in pages), seq_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1], S, nh, nkv, hd,
+        n_pages, scale, window or 0, _ptr(sinks), part.data_ptr(), max_pages, raw_stream()), "kv8_attention", launches=plan[0])
     return out
 
 
@@ -249,7 +273,8 @@ def kv8_attention(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tens
     with the kernels of the 16- and 32-bit cache: a page serves many rows there, and turning its codes again in every block that
     reads it would cost more than writing it out once."""
     n_pages, _, _ = _check_pages(pages, "kv8_attention", nkv, hd)
-    _check_index("kv8_attention", ctx.seq_lens, block_table)
+    if not (ctx.seq_lens.dtype == block_table.dtype == torch.int32):
+        raise KernelError("kv8_attention: index tensors are int32")
     dt_code(q.dtype)
     if nh < 1 or nh % nkv or q.dim() != 2 or q.shape[1] != nh * hd:
         raise KernelError("kv8_attention: q is [T, nh * hd], and every kv head serves as many query heads")
