@@ -168,65 +168,75 @@ __global__ void __launch_bounds__(256) kv8_prepare_qk_kernel(
       s_sn[i / HALF][i % HALF] = r.y;
     }
   __syncthreads();
-  const int heads = nh + (k_pages ? nkv : 0), all = tokens * heads, e0 = (lane % LPH) * 8;
-  for (int at = threadIdx.x / LPH; at < (all + 32 / LPH - 1) / (32 / LPH) * (32 / LPH); at += 256 / LPH) {
-    const bool live = at < all;
-    const int tok = live ? at / heads : 0, head = at - tok * heads, t = t0 + tok;
-    const bool is_q = head < nh;
-    float a[8], b[8];
+  // 64 threads a token: its angles stay in registers over all heads, the gains over all q and over all k heads
+  constexpr int HPT = 64 / LPH;                                  // heads at a time
+  const int tok = threadIdx.x / 64, t = t0 + tok, e0 = (lane % LPH) * 8, h0 = threadIdx.x % 64 / LPH;
+  const bool here = tok < tokens;
+  float cs[8], sn[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
-    if (live) {
-      const T* src = qkv + (size_t)t * row + (size_t)head * HD + e0;
-      Kv8Vec<T>::load8(src, a);
-      Kv8Vec<T>::load8(src + HALF, b);
+  for (int i = 0; i < 8; ++i) {
+    cs[i] = inv_freq && here ? s_cs[tok][e0 + i] : 1.f;
+    sn[i] = inv_freq && here ? s_sn[tok][e0 + i] : 0.f;
+  }
+  const int pos = here ? positions[t] : 0, page = here && k_pages ? kv8_page_of(positions, seq_of_token, block_table, maxp, n_pages, t) : -1;
+#pragma unroll 1
+  for (int kind = 0; kind < (k_pages ? 2 : 1); ++kind) {
+    const float* gain = kind ? wk : wq;
+    const int n = kind ? nkv : nh;
+    float ga[8], gb[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      ga[i] = gain ? gain[e0 + i] : 1.f;
+      gb[i] = gain ? gain[e0 + HALF + i] : 1.f;
     }
-    const float* gain = is_q ? wq : wk;
-    float ss = 0.f;
+#pragma unroll 1
+    for (int head = h0; head < (n + HPT - 1) / HPT * HPT; head += HPT) {
+      const bool live = here && head < n;
+      float a[8], b[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
-#pragma unroll
-    for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (gain) {
-      const float inv = rsqrtf(ss / (float)HD + eps);
-      float ga[8], gb[8];
-      Kv8Vec<float>::load8(gain + e0, ga);
-      Kv8Vec<float>::load8(gain + e0 + HALF, gb);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        a[i] *= inv * ga[i];
-        b[i] *= inv * gb[i];
-      }
-    }
-    if (inv_freq) {
-      float cs[8], sn[8];
-      Kv8Vec<float>::load8(&s_cs[tok][e0], cs);
-      Kv8Vec<float>::load8(&s_sn[tok][e0], sn);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x = a[i] * cs[i] - b[i] * sn[i], y = a[i] * sn[i] + b[i] * cs[i];
-        a[i] = x;
-        b[i] = y;
-      }
-    }
-    if (is_q) {
+      for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
       if (live) {
+        const T* src = qkv + (size_t)t * row + (size_t)(kind * nh + head) * HD + e0;
+        Kv8Vec<T>::load8(src, a);
+        Kv8Vec<T>::load8(src + HALF, b);
+      }
+      if (gain) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
+#pragma unroll
+        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float inv = rsqrtf(ss / (float)HD + eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          a[i] *= inv * ga[i];
+          b[i] *= inv * gb[i];
+        }
+      }
+      if (inv_freq) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float x = a[i] * cs[i] - b[i] * sn[i], y = a[i] * sn[i] + b[i] * cs[i];
+          a[i] = x;
+          b[i] = y;
+        }
+      }
+      if (kind == 0) {
+        if (!live) continue;
         T* dst = q_out + ((size_t)t * nh + head) * HD + e0;
         Kv8Vec<T>::store8(dst, a);
         Kv8Vec<T>::store8(dst + HALF, b);
+        continue;
       }
-    }
-    uint32_t top = 0;
+      uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, max(kv8_magnitude(a[i]), kv8_magnitude(b[i])));
+      for (int i = 0; i < 8; ++i) top = max(top, max(kv8_magnitude(a[i]), kv8_magnitude(b[i])));
 #pragma unroll
-    for (int o = LPH / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (live && !is_q) {
-      const int page = kv8_page_of(positions, seq_of_token, block_table, maxp, n_pages, t);
-      if (page < 0) continue;
-      const int e = kv8_exponent_of(top), key = positions[t] & (SX_PAGE - 1);
+      for (int o = LPH / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (!live || page < 0) continue;
+      const int e = kv8_exponent_of(top), key = pos & (SX_PAGE - 1);
       const float inverse = kv8_inverse(e);
-      const size_t place = (size_t)page * nkv + (head - nh);
+      const size_t place = (size_t)page * nkv + head;
       uint32_t ca[2], cb[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -253,16 +263,22 @@ __global__ void __launch_bounds__(256) kv8_prepare_v_kernel(
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // ---- values: the groups of tokens that share 16 places of a page and begin in this block's 16 tokens
   constexpr int WPH = HALF / 32;                                 // warps a head, two dims a lane
-  const int t0 = blockIdx.x * KV8_TOKENS, t_end = min(t0 + KV8_TOKENS, n_tokens);
-  auto begins = [&](int t) {                                     // (a group is a run of one sequence's neighbouring positions)
-    return t == 0 || (positions[t] & (KV8_TOKENS - 1)) == 0 || seq_of_token[t] != seq_of_token[t - 1] || positions[t] != positions[t - 1] + 1;
-  };
-  for (int t = t0; t < t_end; ++t) {
-    if (!begins(t)) continue;
-    int n = 1;
-    while (n < KV8_TOKENS && t + n < n_tokens && !begins(t + n)) ++n;
-    const int page = kv8_page_of(positions, seq_of_token, block_table, maxp, n_pages, t), key = positions[t] & (SX_PAGE - 1);
-    if (page < 0) continue;
+  // a group is a run of one sequence's neighbouring positions within 16 places; lane i looks at token t0 + i
+  const int t0 = blockIdx.x * KV8_TOKENS, t_ = min(t0 + lane, n_tokens - 1), before = max(t0 - 1, 0);
+  const int pos_ = positions[t_], seq_ = seq_of_token[t_];
+  int pos_before = __shfl_up_sync(0xffffffffu, pos_, 1), seq_before = __shfl_up_sync(0xffffffffu, seq_, 1);
+  if (lane == 0) {
+    pos_before = positions[before];
+    seq_before = seq_of_token[before];
+  }
+  const bool starts = t0 + lane == 0 || t0 + lane >= n_tokens || (pos_ & (KV8_TOKENS - 1)) == 0 || seq_ != seq_before || pos_ != pos_before + 1;
+  const uint32_t groups = __ballot_sync(0xffffffffu, starts);    // (a bit set where the tokens end, too)
+  for (uint32_t left = groups & 0xffffu; left; left &= left - 1) {
+    const int i0 = __ffs(left) - 1, t = t0 + i0;
+    if (t >= n_tokens) break;
+    const uint32_t behind = groups >> i0 >> 1;
+    const int n = min(KV8_TOKENS, behind ? __ffs(behind) : KV8_TOKENS), pos = __shfl_sync(0xffffffffu, pos_, i0), key = pos & (SX_PAGE - 1);
+    const int page = kv8_page_of(positions, seq_of_token, block_table, maxp, n_pages, t);
     for (int h0 = blockIdx.y * (8 / WPH); h0 < nkv; h0 += gridDim.y * (8 / WPH)) {
       const int h = h0 + warp / WPH, d = (warp % WPH) * 64 + 2 * lane;
       float2 x[KV8_TOKENS];
@@ -291,7 +307,7 @@ __global__ void __launch_bounds__(256) kv8_prepare_v_kernel(
         top[0] = max(s_top[warp & ~(WPH - 1)][lane >> 1], s_top[warp | (WPH - 1)][lane >> 1]);
       }
       const int mine = kv8_exponent_of(top[0]);
-      const size_t place = (size_t)page * nkv + min(h, nkv - 1);
+      const size_t place = (size_t)max(page, 0) * nkv + min(h, nkv - 1);
       uint32_t lo[4], hi[4];
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
@@ -304,7 +320,7 @@ __global__ void __launch_bounds__(256) kv8_prepare_v_kernel(
           hi[w] |= kv8_codes2(x[k].y * f0, x[k + 1].y * f1) << (8 * i);
         }
       }
-      if (h >= nkv) continue;
+      if (h >= nkv || page < 0) continue;
       uint8_t* dst = v_pages + place * SX_PAGE * HD + kv8_v_at(key, d);
       if (n == KV8_TOKENS) {                                     // (begins at a multiple of 16)
         *reinterpret_cast<uint4*>(dst) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -368,7 +384,7 @@ extern "C" int sx_kv8_prepare(const void* qkv, void* q_out, void* k_pages, void*
 
 // ---------------------------------------------------------------------------------------
 // Pages read back: page i of the result holds page page_idx[i] of sequence page_seq[i] as [kv heads][64][hd] in T, rows
-// behind the sequence's end as zeros.  A block a (page, kv head) and keys or values, bound by its bytes.  A lane of keys takes 8 codes of a
+// behind the sequence's end as zeros.  A block a (page, kv head), bound by its bytes.  A lane of keys takes 8 codes of a
 // row at a time (16 bytes of bfloat16); a lane of values takes 8 dims of 4 keys, one word a dim, turns the bytes around in registers and
 // stores 16 bytes a key: 8 lanes beside one another read 32 bytes of a dim, 4 write 64 of a key.
 // ---------------------------------------------------------------------------------------
@@ -382,51 +398,77 @@ template <typename T> __device__ __forceinline__ void kv8_store8(T* dst, const u
   }
   Kv8Vec<T>::store8(dst, x);
 }
-template <typename T>
+// HD: the head size where it is 64 or 128 (all loads of a block are then under way at once), 0 for any
+template <typename T, int HD>
 __global__ void __launch_bounds__(256) kv8_read_kernel(
     const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages, const uint8_t* __restrict__ k_exp,
     const uint8_t* __restrict__ v_exp, T* __restrict__ k_out, T* __restrict__ v_out, const int* __restrict__ page_seq,
-    const int* __restrict__ page_idx, const int* __restrict__ seq_lens, const int* __restrict__ block_table, int maxp, int nkv, int hd,
+    const int* __restrict__ page_idx, const int* __restrict__ seq_lens, const int* __restrict__ block_table, int maxp, int nkv, int hd_,
     int n_pages) {
-  __shared__ float s_f[SX_PAGE];
+  __shared__ float s_k[SX_PAGE], s_v[SX_PAGE];
   pdl_wait();
   pdl_trigger();
+  const int hd = HD ? HD : hd_, groups = hd / 8, cb = kv8_block(hd);     // groups of 8 dims
   const int i = blockIdx.x, kvh = blockIdx.y;
-  const bool is_k = blockIdx.z == 0;
   const int s = page_seq[i], j = page_idx[i];
   const int page = block_table[(size_t)s * maxp + j];
   const bool ok = page >= 0 && page < n_pages;
   const int held = ok ? min(SX_PAGE, max(0, seq_lens[s] - j * SX_PAGE)) : 0;
-  const size_t from = (size_t)(ok ? page : 0) * nkv + kvh;
-  const uint8_t* src = (is_k ? k_pages : v_pages) + from * SX_PAGE * hd;
-  T* dst = (is_k ? k_out : v_out) + ((size_t)i * nkv + kvh) * SX_PAGE * hd;
-  if (threadIdx.x < SX_PAGE) s_f[threadIdx.x] = kv8_scale((is_k ? k_exp : v_exp)[from * SX_PAGE + threadIdx.x]);
-  __syncthreads();
-  const int groups = hd / 8;                                     // of 8 dims
-  if (is_k) {
-    const int cb = kv8_block(hd);
-#pragma unroll 4
-    for (int o = threadIdx.x; o < SX_PAGE * groups; o += 256) {
-      const int key = o / groups, d = o % groups * 8;
-      const uint2 w = *reinterpret_cast<const uint2*>(src + kv8_k_at(key, d, cb));
-      const uint32_t pairs[4] = {w.x, w.x >> 16, w.y, w.y >> 16};
-      kv8_store8<T>(dst + key * hd + d, pairs, s_f[key], key < held);
+  const size_t from = (size_t)(ok ? page : 0) * nkv + kvh, to = ((size_t)i * nkv + kvh) * SX_PAGE * hd;
+  const uint8_t *k = k_pages + from * SX_PAGE * hd, *v = v_pages + from * SX_PAGE * hd;
+  constexpr int NK = HD ? HD / 32 : 1, NV = HD == 64 ? 1 : HD / 128;     // items of a thread, where that is known
+  // items of values, by bits: 3 of the word of 4 keys, 2 of the group of dims, 1 of the word, the group's rest
+  auto v_key = [](int o) { return ((o & 7) | (o >> 2 & 8)) * 4; };
+  auto v_group = [](int o) { return (o >> 3 & 3) | (o >> 6) * 4; };
+  uint2 kw[NK];
+  uint32_t vw[NV ? NV : 1][8];
+  if (HD) {
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+      const int o = threadIdx.x + 256 * n;
+      kw[n] = *reinterpret_cast<const uint2*>(k + kv8_k_at(o / groups, o % groups * 8, cb));
     }
-    return;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int o = threadIdx.x + 256 * n;
+      if (o < groups * 16)
+#pragma unroll
+        for (int d = 0; d < 8; ++d) vw[n][d] = *reinterpret_cast<const uint32_t*>(v + kv8_v_at(v_key(o), v_group(o) * 8 + d));
+    }
   }
-  for (int o = threadIdx.x; o < (groups + 3) / 4 * 64; o += 256) {
-    const int key = ((o & 7) | (o >> 2 & 8)) * 4, group = (o >> 3 & 3) | (o >> 6) * 4;      // bits: 3 of the key's word, 2 of the group, 1 of the word, the group's rest
-    if (group >= groups) continue;
-    uint32_t w[8];
+  if (threadIdx.x < SX_PAGE) s_k[threadIdx.x] = kv8_scale(k_exp[from * SX_PAGE + threadIdx.x]);
+  else if (threadIdx.x < 2 * SX_PAGE) s_v[threadIdx.x - SX_PAGE] = kv8_scale(v_exp[from * SX_PAGE + threadIdx.x - SX_PAGE]);
+  __syncthreads();
+  auto put_k = [&](int o, const uint2 w) {
+    const int key = o / groups, d = o % groups * 8;
+    const uint32_t pairs[4] = {w.x, w.x >> 16, w.y, w.y >> 16};
+    kv8_store8<T>(k_out + to + key * hd + d, pairs, s_k[key], key < held);
+  };
+  auto put_v = [&](int o, const uint32_t (&w)[8]) {
+    const int key = v_key(o), group = v_group(o);
 #pragma unroll
-    for (int d = 0; d < 8; ++d) w[d] = *reinterpret_cast<const uint32_t*>(src + kv8_v_at(key, group * 8 + d));
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int n = 0; n < 4; ++n) {
       uint32_t pairs[4];
 #pragma unroll
-      for (int d = 0; d < 4; ++d) pairs[d] = __byte_perm(w[2 * d], w[2 * d + 1], k | (4 + k) << 4);
-      kv8_store8<T>(dst + (key + k) * hd + group * 8, pairs, s_f[key + k], key + k < held);
+      for (int d = 0; d < 4; ++d) pairs[d] = __byte_perm(w[2 * d], w[2 * d + 1], n | (4 + n) << 4);
+      kv8_store8<T>(v_out + to + (key + n) * hd + group * 8, pairs, s_v[key + n], key + n < held);
     }
+  };
+  if (HD) {
+#pragma unroll
+    for (int n = 0; n < NK; ++n) put_k(threadIdx.x + 256 * n, kw[n]);
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+      if (threadIdx.x + 256 * n < groups * 16) put_v(threadIdx.x + 256 * n, vw[n]);
+    return;
+  }
+  for (int o = threadIdx.x; o < SX_PAGE * groups; o += 256) put_k(o, *reinterpret_cast<const uint2*>(k + kv8_k_at(o / groups, o % groups * 8, cb)));
+  for (int o = threadIdx.x; o < (groups + 3) / 4 * 64; o += 256) {
+    if (v_group(o) >= groups) continue;
+    uint32_t w[8];
+#pragma unroll
+    for (int d = 0; d < 8; ++d) w[d] = *reinterpret_cast<const uint32_t*>(v + kv8_v_at(v_key(o), v_group(o) * 8 + d));
+    put_v(o, w);
   }
 }
 
@@ -436,13 +478,12 @@ extern "C" int sx_kv8_read(const void* k_pages, const void* v_pages, const void*
   if (n_out <= 0) return 0;
   if (hd <= 0 || hd % 16 || hd > KV8_MAX_HD || nkv <= 0 || nkv > 65535) return SX_ERR_SIZE;
   if (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) return SX_ERR_ALIGN;
-  const dim3 grid(n_out, nkv, 2);
-  if (dt == SX_F32)
-    return sx_launch(kv8_read_kernel<float>, grid, dim3(256), 0, stream, (const uint8_t*)k_pages, (const uint8_t*)v_pages, (const uint8_t*)k_exp,
-                     (const uint8_t*)v_exp, (float*)k_out, (float*)v_out, page_seq, page_idx, seq_lens, block_table, maxp, nkv, hd, n_pages);
-  if (dt == SX_BF16)
-    return sx_launch(kv8_read_kernel<bf16>, grid, dim3(256), 0, stream, (const uint8_t*)k_pages, (const uint8_t*)v_pages, (const uint8_t*)k_exp,
-                     (const uint8_t*)v_exp, (bf16*)k_out, (bf16*)v_out, page_seq, page_idx, seq_lens, block_table, maxp, nkv, hd, n_pages);
+  const dim3 grid(n_out, nkv);
+#define KV8_READ(T, HD)                                                                                                                            \
+  sx_launch(kv8_read_kernel<T, HD>, grid, dim3(256), 0, stream, (const uint8_t*)k_pages, (const uint8_t*)v_pages, (const uint8_t*)k_exp,             \
+            (const uint8_t*)v_exp, (T*)k_out, (T*)v_out, page_seq, page_idx, seq_lens, block_table, maxp, nkv, hd, n_pages)
+  if (dt == SX_F32) return hd == 64 ? KV8_READ(float, 64) : hd == 128 ? KV8_READ(float, 128) : KV8_READ(float, 0);
+  if (dt == SX_BF16) return hd == 64 ? KV8_READ(bf16, 64) : hd == 128 ? KV8_READ(bf16, 128) : KV8_READ(bf16, 0);
   return SX_ERR_DTYPE;
 }
 
