@@ -97,16 +97,19 @@ __global__ void __launch_bounds__(KV8_WARPS * 32) kv8_prepare_kernel(
   }
 }
 
-// The same for many tokens at head size 64 or 128, the whole head rotated or nothing, as two kernels.  One takes the q and k heads of four
-// tokens a block, 16 elements a lane (8 of either half of the head, so that rotation stays within the lane and a key's codes leave as 8-byte
-// stores); the block makes the four tokens' angles first, one or two a thread.  The other takes values: a value page lies dim by dim, and a token
-// alone would write a byte here and there (measured in all: 338 us for 8,191 tokens of 48 heads of 128, where bytes take 28.6).  There a thread has
-// two dims of up to 16 tokens that share 16 neighbouring places of a page, finds the rows' largest magnitudes with its warp by 31 exchanges for
-// all 16 tokens, and stores 16 bytes a dim.  (As one kernel its 124 registers left two blocks an SM and the q and k heads waited for themselves: 134 us.)
+// The same for many tokens at head size 64 or 128, the whole head rotated or nothing.  Blocks of one kind take the q and k heads of four tokens, 64
+// threads a token and 16 elements a lane (8 of either half of the head, so that rotation stays within the lane and a key's codes leave as 8-byte
+// stores).  Blocks of the other kind take values: a value page lies dim by dim, and a token alone would write a byte here and there (measured in
+// all: 338 us for 8,191 tokens of 48 heads of 128, where bytes take 28.6).  There a thread has two dims of up to 16 tokens that share 16
+// neighbouring places of a page, finds the rows' largest magnitudes with its warp by 31 exchanges for all 16 tokens, and stores 16 bytes a dim.
+// (One kernel: 16 rows of values one behind the other are mostly waiting, 23 us alone.)
 template <typename T> struct Kv8Vec;
 template <> struct Kv8Vec<bf16> {
-  static __device__ __forceinline__ void load8(const bf16* p, float (&x)[8]) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
+  typedef uint4 Raw8;                                            // 8 and 2 elements as they lie in memory
+  typedef uint32_t Raw2;
+  static __device__ __forceinline__ Raw8 zero8() { return make_uint4(0, 0, 0, 0); }
+  static __device__ __forceinline__ Raw2 zero2() { return 0; }
+  static __device__ __forceinline__ void floats8(const Raw8& w, float (&x)[8]) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -114,6 +117,7 @@ template <> struct Kv8Vec<bf16> {
       x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
     }
   }
+  static __device__ __forceinline__ float2 floats2(Raw2 u) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
   static __device__ __forceinline__ void store8(bf16* p, const float (&x)[8]) {
     uint32_t u[4];
 #pragma unroll
@@ -123,24 +127,20 @@ template <> struct Kv8Vec<bf16> {
     }
     *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
   }
-  static __device__ __forceinline__ float2 load2(const bf16* p) {
-    const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
-    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-  }
 };
 template <> struct Kv8Vec<float> {
-  static __device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float4 v = reinterpret_cast<const float4*>(p)[i];
-      x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
-    }
+  struct Raw8 { float4 a, b; };
+  typedef float2 Raw2;
+  static __device__ __forceinline__ Raw8 zero8() { const float4 z = make_float4(0.f, 0.f, 0.f, 0.f); return {z, z}; }
+  static __device__ __forceinline__ Raw2 zero2() { return make_float2(0.f, 0.f); }
+  static __device__ __forceinline__ void floats8(const Raw8& w, float (&x)[8]) {
+    x[0] = w.a.x; x[1] = w.a.y; x[2] = w.a.z; x[3] = w.a.w; x[4] = w.b.x; x[5] = w.b.y; x[6] = w.b.z; x[7] = w.b.w;
   }
+  static __device__ __forceinline__ float2 floats2(Raw2 u) { return u; }
   static __device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) reinterpret_cast<float4*>(p)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
   }
-  static __device__ __forceinline__ float2 load2(const float* p) { return *reinterpret_cast<const float2*>(p); }
 };
 __device__ __forceinline__ uint32_t kv8_magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }   // ordered as the magnitudes are, NaN above infinity
 __device__ __forceinline__ int kv8_exponent_of(uint32_t top) { return kv8_exponent(__uint_as_float(top), top < 0x7f800000u); }
@@ -150,17 +150,114 @@ __device__ __forceinline__ int kv8_page_of(const int* positions, const int* seq_
   return (unsigned)page < (unsigned)n_pages ? page : -1;
 }
 
+#define KV8_TOKENS 16
+// values of the groups that begin in tokens 16 block .. + 15, of heads first_head, first_head + heads_step, .. (a head is one or two warps)
+template <typename T, int HD>
+__device__ __forceinline__ void kv8_prepare_v(const T* __restrict__ qkv, uint8_t* __restrict__ v_pages, uint8_t* __restrict__ v_exp,
+                                              const int* __restrict__ positions, const int* __restrict__ seq_of_token,
+                                              const int* __restrict__ block_table, int maxp, int nh, int nkv, int n_pages, int row, int n_tokens,
+                                              int block, int first, int step, uint32_t (*s_top)[KV8_TOKENS]) {
+  constexpr int HALF = HD / 2;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // ---- values: the groups of tokens that share 16 places of a page and begin in this block's 16 tokens
+  constexpr int WPH = HALF / 32;                                 // warps a head, two dims a lane
+  // a group is a run of one sequence's neighbouring positions within 16 places; lane i looks at token t0 + i
+  const int t0 = block * KV8_TOKENS, t_ = min(t0 + lane, n_tokens - 1), before = max(t0 - 1, 0);
+  const int pos_ = positions[t_], seq_ = seq_of_token[t_];
+  int pos_before = __shfl_up_sync(0xffffffffu, pos_, 1), seq_before = __shfl_up_sync(0xffffffffu, seq_, 1);
+  if (lane == 0) {
+    pos_before = positions[before];
+    seq_before = seq_of_token[before];
+  }
+  const bool starts = t0 + lane == 0 || t0 + lane >= n_tokens || (pos_ & (KV8_TOKENS - 1)) == 0 || seq_ != seq_before || pos_ != pos_before + 1;
+  const uint32_t groups = __ballot_sync(0xffffffffu, starts);    // (a bit set where the tokens end, too)
+  for (uint32_t left = groups & 0xffffu; left; left &= left - 1) {
+    const int i0 = __ffs(left) - 1, t = t0 + i0;
+    if (t >= n_tokens) break;
+    const uint32_t behind = groups >> i0 >> 1;
+    const int n = min(KV8_TOKENS, behind ? __ffs(behind) : KV8_TOKENS), pos = __shfl_sync(0xffffffffu, pos_, i0), key = pos & (SX_PAGE - 1);
+    const int page = kv8_page_of(positions, seq_of_token, block_table, maxp, n_pages, t);
+    for (int h0 = first * (8 / WPH); h0 < nkv; h0 += step * (8 / WPH)) {
+      const int h = h0 + warp / WPH, d = (warp % WPH) * 64 + 2 * lane;
+      typename Kv8Vec<T>::Raw2 x[KV8_TOKENS];
+      uint32_t top[KV8_TOKENS];
+      const T* src = qkv + (size_t)t * row + (size_t)(nh + nkv + h) * HD + d;
+#pragma unroll
+      for (int i = 0; i < KV8_TOKENS; ++i) x[i] = h < nkv && i < n ? *reinterpret_cast<const typename Kv8Vec<T>::Raw2*>(src + (size_t)i * row) : Kv8Vec<T>::zero2();
+#pragma unroll
+      for (int i = 0; i < KV8_TOKENS; ++i) {
+        const float2 y = Kv8Vec<T>::floats2(x[i]);
+        top[i] = max(kv8_magnitude(y.x), kv8_magnitude(y.y));
+      }
+      // the warp's largest of each token: after the exchanges lane's belongs to token lane >> 1
+      int off = 16;
+#pragma unroll
+      for (int m = KV8_TOKENS; m > 1; m >>= 1, off >>= 1) {
+        const bool up = lane & off;
+#pragma unroll
+        for (int i = 0; i < m / 2; ++i) {
+          const uint32_t keep = up ? top[i + m / 2] : top[i], send = up ? top[i] : top[i + m / 2];
+          top[i] = max(keep, __shfl_xor_sync(0xffffffffu, send, off));
+        }
+      }
+      top[0] = max(top[0], __shfl_xor_sync(0xffffffffu, top[0], 1));
+      if (WPH > 1) {
+        __syncthreads();
+        if (!(lane & 1)) s_top[warp][lane >> 1] = top[0];
+        __syncthreads();
+        top[0] = max(s_top[warp & ~(WPH - 1)][lane >> 1], s_top[warp | (WPH - 1)][lane >> 1]);
+      }
+      const int mine = kv8_exponent_of(top[0]);
+      const size_t place = (size_t)max(page, 0) * nkv + min(h, nkv - 1);
+      uint32_t lo[4], hi[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        lo[w] = hi[w] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const int k = 4 * w + i;
+          const float f0 = kv8_inverse(__shfl_sync(0xffffffffu, mine, 2 * k)), f1 = kv8_inverse(__shfl_sync(0xffffffffu, mine, 2 * k + 2));
+          const float2 y0 = Kv8Vec<T>::floats2(x[k]), y1 = Kv8Vec<T>::floats2(x[k + 1]);
+          lo[w] |= kv8_codes2(y0.x * f0, y1.x * f1) << (8 * i);
+          hi[w] |= kv8_codes2(y0.y * f0, y1.y * f1) << (8 * i);
+        }
+      }
+      if (h >= nkv || page < 0) continue;
+      uint8_t* dst = v_pages + place * SX_PAGE * HD + kv8_v_at(key, d);
+      if (n == KV8_TOKENS) {                                     // (begins at a multiple of 16)
+        *reinterpret_cast<uint4*>(dst) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        *reinterpret_cast<uint4*>(dst + SX_PAGE) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < KV8_TOKENS; ++i)
+          if (i < n) {
+            dst[i] = (uint8_t)(lo[i >> 2] >> (8 * (i & 3)));
+            dst[SX_PAGE + i] = (uint8_t)(hi[i >> 2] >> (8 * (i & 3)));
+          }
+      }
+      if (warp % WPH == 0 && !(lane & 1) && (lane >> 1) < n) v_exp[place * SX_PAGE + key + (lane >> 1)] = (uint8_t)mine;
+    }
+  }
+}
+
 #define KV8_QK_TOKENS 4
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) kv8_prepare_qk_kernel(
-    const T* __restrict__ qkv, T* __restrict__ q_out, uint8_t* __restrict__ k_pages, uint8_t* __restrict__ k_exp, const float* __restrict__ wq,
-    const float* __restrict__ wk, const float* __restrict__ inv_freq, float eps, const int* __restrict__ positions,
-    const int* __restrict__ seq_of_token, const int* __restrict__ block_table, int maxp, int nh, int nkv, int n_pages, int row, int n_tokens) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) kv8_prepare_wide_kernel(
+    const T* __restrict__ qkv, T* __restrict__ q_out, uint8_t* __restrict__ k_pages, uint8_t* __restrict__ v_pages, uint8_t* __restrict__ k_exp,
+    uint8_t* __restrict__ v_exp, const float* __restrict__ wq, const float* __restrict__ wk, const float* __restrict__ inv_freq, float eps,
+    const int* __restrict__ positions, const int* __restrict__ seq_of_token, const int* __restrict__ block_table, int maxp, int nh, int nkv,
+    int n_pages, int row, int n_tokens, int v_blocks, int v_shares) {
   constexpr int HALF = HD / 2, LPH = HD / 16, TOK = KV8_QK_TOKENS;       // lanes a head
   __shared__ __align__(16) float s_cs[TOK][HALF], s_sn[TOK][HALF];
+  __shared__ uint32_t s_top[8][KV8_TOKENS];
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31, t0 = blockIdx.x * TOK, tokens = min(TOK, n_tokens - t0);
+  if (blockIdx.x < v_blocks * v_shares) {                        // (first of all: they wait for memory while the others compute)
+    kv8_prepare_v<T, HD>(qkv, v_pages, v_exp, positions, seq_of_token, block_table, maxp, nh, nkv, n_pages, row, n_tokens, blockIdx.x / v_shares,
+                         blockIdx.x % v_shares, v_shares, s_top);
+    return;
+  }
+  const int lane = threadIdx.x & 31, t0 = (blockIdx.x - v_blocks * v_shares) * TOK, tokens = min(TOK, n_tokens - t0);
   if (inv_freq)
     for (int i = threadIdx.x; i < tokens * HALF; i += 256) {
       const float2 r = kv8_turn(positions[t0 + i / HALF], inv_freq[i % HALF]);
@@ -189,16 +286,22 @@ __global__ void __launch_bounds__(256) kv8_prepare_qk_kernel(
       ga[i] = gain ? gain[e0 + i] : 1.f;
       gb[i] = gain ? gain[e0 + HALF + i] : 1.f;
     }
+    typedef typename Kv8Vec<T>::Raw8 Raw;
+    const T* src = qkv + (size_t)t * row + (size_t)kind * nh * HD + e0;
+    Raw next_a = Kv8Vec<T>::zero8(), next_b = next_a;            // the next head's elements are under way while one is worked at
+    if (here && h0 < n) {
+      next_a = *reinterpret_cast<const Raw*>(src + (size_t)h0 * HD);
+      next_b = *reinterpret_cast<const Raw*>(src + (size_t)h0 * HD + HALF);
+    }
 #pragma unroll 1
     for (int head = h0; head < (n + HPT - 1) / HPT * HPT; head += HPT) {
       const bool live = here && head < n;
       float a[8], b[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
-      if (live) {
-        const T* src = qkv + (size_t)t * row + (size_t)(kind * nh + head) * HD + e0;
-        Kv8Vec<T>::load8(src, a);
-        Kv8Vec<T>::load8(src + HALF, b);
+      Kv8Vec<T>::floats8(next_a, a);
+      Kv8Vec<T>::floats8(next_b, b);
+      if (here && head + HPT < n) {
+        next_a = *reinterpret_cast<const Raw*>(src + (size_t)(head + HPT) * HD);
+        next_b = *reinterpret_cast<const Raw*>(src + (size_t)(head + HPT) * HD + HALF);
       }
       if (gain) {
         float ss = 0.f;
@@ -251,93 +354,6 @@ __global__ void __launch_bounds__(256) kv8_prepare_qk_kernel(
   }
 }
 
-#define KV8_TOKENS 16
-template <typename T, int HD>
-__global__ void __launch_bounds__(256) kv8_prepare_v_kernel(
-    const T* __restrict__ qkv, uint8_t* __restrict__ v_pages, uint8_t* __restrict__ v_exp, const int* __restrict__ positions,
-    const int* __restrict__ seq_of_token, const int* __restrict__ block_table, int maxp, int nh, int nkv, int n_pages, int row, int n_tokens) {
-  constexpr int HALF = HD / 2;
-  __shared__ uint32_t s_top[8][KV8_TOKENS];
-  pdl_wait();
-  pdl_trigger();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // ---- values: the groups of tokens that share 16 places of a page and begin in this block's 16 tokens
-  constexpr int WPH = HALF / 32;                                 // warps a head, two dims a lane
-  // a group is a run of one sequence's neighbouring positions within 16 places; lane i looks at token t0 + i
-  const int t0 = blockIdx.x * KV8_TOKENS, t_ = min(t0 + lane, n_tokens - 1), before = max(t0 - 1, 0);
-  const int pos_ = positions[t_], seq_ = seq_of_token[t_];
-  int pos_before = __shfl_up_sync(0xffffffffu, pos_, 1), seq_before = __shfl_up_sync(0xffffffffu, seq_, 1);
-  if (lane == 0) {
-    pos_before = positions[before];
-    seq_before = seq_of_token[before];
-  }
-  const bool starts = t0 + lane == 0 || t0 + lane >= n_tokens || (pos_ & (KV8_TOKENS - 1)) == 0 || seq_ != seq_before || pos_ != pos_before + 1;
-  const uint32_t groups = __ballot_sync(0xffffffffu, starts);    // (a bit set where the tokens end, too)
-  for (uint32_t left = groups & 0xffffu; left; left &= left - 1) {
-    const int i0 = __ffs(left) - 1, t = t0 + i0;
-    if (t >= n_tokens) break;
-    const uint32_t behind = groups >> i0 >> 1;
-    const int n = min(KV8_TOKENS, behind ? __ffs(behind) : KV8_TOKENS), pos = __shfl_sync(0xffffffffu, pos_, i0), key = pos & (SX_PAGE - 1);
-    const int page = kv8_page_of(positions, seq_of_token, block_table, maxp, n_pages, t);
-    for (int h0 = blockIdx.y * (8 / WPH); h0 < nkv; h0 += gridDim.y * (8 / WPH)) {
-      const int h = h0 + warp / WPH, d = (warp % WPH) * 64 + 2 * lane;
-      float2 x[KV8_TOKENS];
-      uint32_t top[KV8_TOKENS];
-      const T* src = qkv + (size_t)t * row + (size_t)(nh + nkv + h) * HD + d;
-#pragma unroll
-      for (int i = 0; i < KV8_TOKENS; ++i) x[i] = h < nkv && i < n ? Kv8Vec<T>::load2(src + (size_t)i * row) : make_float2(0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < KV8_TOKENS; ++i) top[i] = max(kv8_magnitude(x[i].x), kv8_magnitude(x[i].y));
-      // the warp's largest of each token: after the exchanges lane's belongs to token lane >> 1
-      int off = 16;
-#pragma unroll
-      for (int m = KV8_TOKENS; m > 1; m >>= 1, off >>= 1) {
-        const bool up = lane & off;
-#pragma unroll
-        for (int i = 0; i < m / 2; ++i) {
-          const uint32_t keep = up ? top[i + m / 2] : top[i], send = up ? top[i] : top[i + m / 2];
-          top[i] = max(keep, __shfl_xor_sync(0xffffffffu, send, off));
-        }
-      }
-      top[0] = max(top[0], __shfl_xor_sync(0xffffffffu, top[0], 1));
-      if (WPH > 1) {
-        __syncthreads();
-        if (!(lane & 1)) s_top[warp][lane >> 1] = top[0];
-        __syncthreads();
-        top[0] = max(s_top[warp & ~(WPH - 1)][lane >> 1], s_top[warp | (WPH - 1)][lane >> 1]);
-      }
-      const int mine = kv8_exponent_of(top[0]);
-      const size_t place = (size_t)max(page, 0) * nkv + min(h, nkv - 1);
-      uint32_t lo[4], hi[4];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        lo[w] = hi[w] = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          const int k = 4 * w + i;
-          const float f0 = kv8_inverse(__shfl_sync(0xffffffffu, mine, 2 * k)), f1 = kv8_inverse(__shfl_sync(0xffffffffu, mine, 2 * k + 2));
-          lo[w] |= kv8_codes2(x[k].x * f0, x[k + 1].x * f1) << (8 * i);
-          hi[w] |= kv8_codes2(x[k].y * f0, x[k + 1].y * f1) << (8 * i);
-        }
-      }
-      if (h >= nkv || page < 0) continue;
-      uint8_t* dst = v_pages + place * SX_PAGE * HD + kv8_v_at(key, d);
-      if (n == KV8_TOKENS) {                                     // (begins at a multiple of 16)
-        *reinterpret_cast<uint4*>(dst) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        *reinterpret_cast<uint4*>(dst + SX_PAGE) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < KV8_TOKENS; ++i)
-          if (i < n) {
-            dst[i] = (uint8_t)(lo[i >> 2] >> (8 * (i & 3)));
-            dst[SX_PAGE + i] = (uint8_t)(hi[i >> 2] >> (8 * (i & 3)));
-          }
-      }
-      if (warp % WPH == 0 && !(lane & 1) && (lane >> 1) < n) v_exp[place * SX_PAGE + key + (lane >> 1)] = (uint8_t)mine;
-    }
-  }
-}
-
 // qkv: rows of `row` elements, q heads, k heads and v heads first (q heads alone where k_pages is null and nothing is written).
 // wide: by the kernels for many tokens
 extern "C" int sx_kv8_prepare(const void* qkv, void* q_out, void* k_pages, void* v_pages, void* k_exp, void* v_exp, const float* wq,
@@ -354,20 +370,14 @@ extern "C" int sx_kv8_prepare(const void* qkv, void* q_out, void* k_pages, void*
     if ((hd != 64 && hd != 128) || (inv_freq && rotary_dim != hd)) return SX_ERR_SIZE;
     if (dt != SX_F32 && dt != SX_BF16) return SX_ERR_DTYPE;
     if (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)wq | (uintptr_t)wk | row * es) & 15) return SX_ERR_ALIGN;
-    int rc = 0;
-    const dim3 qk((n_tokens + KV8_QK_TOKENS - 1) / KV8_QK_TOKENS), v((n_tokens + KV8_TOKENS - 1) / KV8_TOKENS, (nkv * (hd / 64) + 7) / 8);
+    const int v_blocks = v_pages ? (n_tokens + KV8_TOKENS - 1) / KV8_TOKENS : 0, v_shares = (nkv * (hd / 64) + 7) / 8;
+    const dim3 blocks(v_blocks * v_shares + (n_tokens + KV8_QK_TOKENS - 1) / KV8_QK_TOKENS);
 #define KV8_WIDE(T, HD)                                                                                                                                \
-  rc = sx_launch(kv8_prepare_qk_kernel<T, HD>, qk, dim3(256), 0, stream, (const T*)qkv, (T*)q_out, (uint8_t*)k_pages, (uint8_t*)k_exp, wq, wk, inv_freq,  \
-                 eps, positions, seq_of_token, block_table, maxp, nh, nkv, n_pages, row, n_tokens);                                                     \
-  if (!rc && v_pages)                                                                                                                                  \
-    rc = sx_launch(kv8_prepare_v_kernel<T, HD>, v, dim3(256), 0, stream, (const T*)qkv, (uint8_t*)v_pages, (uint8_t*)v_exp, positions, seq_of_token,     \
-                   block_table, maxp, nh, nkv, n_pages, row, n_tokens);
-    if (dt == SX_F32) {
-      if (hd == 64) { KV8_WIDE(float, 64) } else { KV8_WIDE(float, 128) }
-    } else {
-      if (hd == 64) { KV8_WIDE(bf16, 64) } else { KV8_WIDE(bf16, 128) }
-    }
-    return rc;
+  sx_launch(kv8_prepare_wide_kernel<T, HD>, blocks, dim3(256), 0, stream, (const T*)qkv, (T*)q_out, (uint8_t*)k_pages, (uint8_t*)v_pages,               \
+            (uint8_t*)k_exp, (uint8_t*)v_exp, wq, wk, inv_freq, eps, positions, seq_of_token, block_table, maxp, nh, nkv, n_pages, row, n_tokens,        \
+            v_blocks, v_shares)
+    if (dt == SX_F32) return hd == 64 ? KV8_WIDE(float, 64) : KV8_WIDE(float, 128);
+    return hd == 64 ? KV8_WIDE(bf16, 64) : KV8_WIDE(bf16, 128);
   }
   // few tokens: a block for every eight heads; many: a block walks its token's heads and makes the angles once
   const dim3 grid(n_tokens, n_tokens * groups <= 4 * sx_sm_count() ? groups : 1);
@@ -416,12 +426,12 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(
   const int held = ok ? min(SX_PAGE, max(0, seq_lens[s] - j * SX_PAGE)) : 0;
   const size_t from = (size_t)(ok ? page : 0) * nkv + kvh, to = ((size_t)i * nkv + kvh) * SX_PAGE * hd;
   const uint8_t *k = k_pages + from * SX_PAGE * hd, *v = v_pages + from * SX_PAGE * hd;
-  constexpr int NK = HD ? HD / 32 : 1, NV = HD == 64 ? 1 : HD / 128;     // items of a thread, where that is known
+  constexpr int NK = HD ? HD / 32 : 1, NV = 1;     // items of a thread, where that is known
   // items of values, by bits: 3 of the word of 4 keys, 2 of the group of dims, 1 of the word, the group's rest
   auto v_key = [](int o) { return ((o & 7) | (o >> 2 & 8)) * 4; };
   auto v_group = [](int o) { return (o >> 3 & 3) | (o >> 6) * 4; };
   uint2 kw[NK];
-  uint32_t vw[NV ? NV : 1][8];
+  uint32_t vw[NV][8];
   if (HD) {
 #pragma unroll
     for (int n = 0; n < NK; ++n) {
@@ -454,21 +464,21 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(
       kv8_store8<T>(v_out + to + (key + n) * hd + group * 8, pairs, s_v[key + n], key + n < held);
     }
   };
-  if (HD) {
+  if constexpr (HD != 0) {
 #pragma unroll
     for (int n = 0; n < NK; ++n) put_k(threadIdx.x + 256 * n, kw[n]);
 #pragma unroll
     for (int n = 0; n < NV; ++n)
       if (threadIdx.x + 256 * n < groups * 16) put_v(threadIdx.x + 256 * n, vw[n]);
-    return;
-  }
-  for (int o = threadIdx.x; o < SX_PAGE * groups; o += 256) put_k(o, *reinterpret_cast<const uint2*>(k + kv8_k_at(o / groups, o % groups * 8, cb)));
-  for (int o = threadIdx.x; o < (groups + 3) / 4 * 64; o += 256) {
-    if (v_group(o) >= groups) continue;
-    uint32_t w[8];
+  } else {
+    for (int o = threadIdx.x; o < SX_PAGE * groups; o += 256) put_k(o, *reinterpret_cast<const uint2*>(k + kv8_k_at(o / groups, o % groups * 8, cb)));
+    for (int o = threadIdx.x; o < (groups + 3) / 4 * 64; o += 256) {
+      if (v_group(o) >= groups) continue;
+      uint32_t w[8];
 #pragma unroll
-    for (int d = 0; d < 8; ++d) w[d] = *reinterpret_cast<const uint32_t*>(v + kv8_v_at(v_key(o), v_group(o) * 8 + d));
-    put_v(o, w);
+      for (int d = 0; d < 8; ++d) w[d] = *reinterpret_cast<const uint32_t*>(v + kv8_v_at(v_key(o), v_group(o) * 8 + d));
+      put_v(o, w);
+    }
   }
 }
 

@@ -137,7 +137,7 @@ def kv8_prepare(qkv: torch.Tensor, q_out: Optional[torch.Tensor], pages: Optiona
             and not any(p is not None and p % 16 for p in args))
     check(launcher("kv8", "sx_kv8_prepare")(
         *args, rotary_dim, eps, positions.data_ptr(), seq_of_token.data_ptr(), block_table.data_ptr(), block_table.shape[1], T, nh, nkv, hd, n_pages,
-        row, wide, dt, raw_stream()), "kv8_prepare", launches=0 if not T or (nh == 0 and k is None) else 2 if wide and k is not None else 1)
+        row, wide, dt, raw_stream()), "kv8_prepare", launches=1 if T and (nh or k is not None) else 0)
 
 
 def _read_plan(ctx, width: int, window: Optional[int], chunk: Optional[int], device):
