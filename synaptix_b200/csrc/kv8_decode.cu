@@ -48,11 +48,11 @@ struct KdArgs {
   const bf16* q;
   bf16* out;
   const uint8_t *k, *v, *ke, *ve;
-  const int *seq_lens, *block_table;
+  const int *seq_lens, *row_seq, *block_table;                  // of row s: keys it may see less len_add, its row of the table (null: s)
   const float* sinks;
   float* part;                 // results of pairs' parts [warps, then 2 a block][rows of a kv head][HD + 2]: maximum, sum, the row
   int* status;
-  int maxp, n_pages, S, nh, nkv, window, blocks, warps, by_pair;
+  int len_add, maxp, n_pages, S, nh, nkv, window, blocks, warps, by_pair;
   float scale;
 };
 
@@ -89,7 +89,7 @@ __device__ __forceinline__ uint32_t kd_half2(float lo, float hi) {
 }
 // first visible page of a sequence and one behind its last
 __device__ __forceinline__ int2 kd_range(const KdArgs& a, int s) {
-  const int len = a.seq_lens[s];
+  const int len = a.seq_lens[s] + a.len_add;
   const int first = a.window > 0 ? max(0, len - a.window) >> 6 : 0;
   return make_int2(first, max(first, min((len + 63) >> 6, a.maxp)));
 }
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
   int seq = -1, kvh = -1, unit_first = 0, unit0 = -1, len = 0;  // the pair at work, the item of the warp it began with; the warp's first pair
   auto begin = [&](int s, int h, int i) {
     seq = s; kvh = h; unit_first = i;
-    len = a.seq_lens[s];
+    len = a.seq_lens[s] + a.len_add;
 #pragma unroll
     for (int r = 0; r < RP; ++r) {
       const int row = g + 8 * r;
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
       const int x = i + L::AHEAD + lane;
       if (x < n_items) {
         const int s = kd_seq_of(start, a.S, a.nkv, x0 + x), n = start[s + 1] - start[s], at = x0 + x - start[s] * a.nkv;
-        const int h = at / n, j = kd_range(a, s).x + at - h * n, page = a.block_table[(size_t)s * a.maxp + j];
+        const int h = at / n, j = kd_range(a, s).x + at - h * n, page = a.block_table[(size_t)(a.row_seq ? a.row_seq[s] : s) * a.maxp + j];
         desc[x & (KD_DESC - 1)] = make_int4(s, h, j, (unsigned)page < (unsigned)a.n_pages ? page : 0);
       }
       __syncwarp();
@@ -666,9 +666,10 @@ extern "C" int sx_kv8_decode_plan(int S, int nh, int nkv, int hd, int max_pages,
   return kd_by_pair(S, nkv, max_pages) || blocks == 1 ? 1 : 2;
 }
 
-// max_pages: no sequence has more visible pages
+// A row of q is a sequence's only token (row_seq null, len_add 0), or any token: seq_lens then holds positions, len_add is 1 and row_seq says whose
+// table it reads.  max_pages: no row has more visible pages
 extern "C" int sx_kv8_decode(const void* q, void* out, const void* k, const void* v, const void* k_exp, const void* v_exp, const int* seq_lens,
-                             const int* block_table, int maxp, int S, int nh, int nkv, int hd, int n_pages, float scale, int window,
+                             const int* row_seq, int len_add, const int* block_table, int maxp, int S, int nh, int nkv, int hd, int n_pages, float scale, int window,
                              const float* sinks, float* part, int max_pages, cudaStream_t stream) {
   if (S <= 0) return 0;
   if ((hd != 64 && hd != 128) || nkv <= 0 || nh <= 0 || nh % nkv || nh / nkv > 16 || S >= KD_MAX_SEQS || n_pages <= 0 || maxp <= 0 || max_pages <= 0 ||
@@ -677,8 +678,8 @@ extern "C" int sx_kv8_decode(const void* q, void* out, const void* k, const void
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k | (uintptr_t)v | (uintptr_t)k_exp | (uintptr_t)v_exp | (uintptr_t)part) & 15) return SX_ERR_ALIGN;
   int* status = kd_status();
   if (!status) return SX_ERR_SIZE;
-  const KdArgs a = {(const bf16*)q, (bf16*)out, (const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)k_exp, (const uint8_t*)v_exp, seq_lens, block_table,
-                    sinks, part, status, maxp, n_pages, S, nh, nkv, window, kd_blocks(S, nkv, max_pages), 0, kd_by_pair(S, nkv, max_pages), scale};
+  const KdArgs a = {(const bf16*)q, (bf16*)out, (const uint8_t*)k, (const uint8_t*)v, (const uint8_t*)k_exp, (const uint8_t*)v_exp, seq_lens, row_seq, block_table,
+                    sinks, part, status, len_add, maxp, n_pages, S, nh, nkv, window, kd_blocks(S, nkv, max_pages), 0, kd_by_pair(S, nkv, max_pages), scale};
   if (hd == 64) return nh / nkv > 8 ? kd_launch<64, true>(a, stream) : kd_launch<64, false>(a, stream);
   return nh / nkv > 8 ? kd_launch<128, true>(a, stream) : kd_launch<128, false>(a, stream);
 }

@@ -225,6 +225,8 @@ def kv8_rows(q: torch.Tensor, pages: KV8Pages, seq_lens: torch.Tensor, block_tab
 DECODE_HEAD_DIMS = (64, 128)
 DECODE_MAX_GROUP = 16
 DECODE_MAX_SEQS = 2047
+# Portions of up to this many tokens a sequence: every token attends by itself over the codes
+FEW_NEW_TOKENS = 4
 
 
 def kv8_decode_supported(dtype, nh: int, nkv: int, hd: int, S: int) -> bool:
@@ -236,8 +238,10 @@ _DECODE_PLANS = {}              # of a shape: kernels, floats of scratch
 
 
 def kv8_decode(q: torch.Tensor, pages: KV8Pages, seq_lens: torch.Tensor, block_table: torch.Tensor, nh: int, scale: float,
-               window: Optional[int], max_len: int, sinks: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """One query token a sequence (row ``s`` of ``q``) on the tensor cores; sizes as ``kv8_decode_supported`` says."""
+               window: Optional[int], max_len: int, sinks: Optional[torch.Tensor] = None,
+               row_seq: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One query token a sequence (row ``s`` of ``q``) on the tensor cores; sizes as ``kv8_decode_supported`` says.  With ``row_seq`` a row is any
+    token: ``row_seq`` names its sequence and ``seq_lens`` holds its position."""
     n_pages, nkv, hd = pages.v.shape[:3]
     S = q.shape[0]
     max_pages = min(-(-max_len // PAGE), block_table.shape[1]) if window is None else min(-(-max_len // PAGE), block_table.shape[1], (window + 126) // PAGE)
@@ -250,8 +254,8 @@ def kv8_decode(q: torch.Tensor, pages: KV8Pages, seq_lens: torch.Tensor, block_t
     out = torch.empty_like(q)
     part = torch.empty(plan[1], dtype=torch.float32, device=q.device)
     check(launcher("kv8_decode", "sx_kv8_decode")(
-        q.data_ptr(), out.data_ptr(), *(t.data_ptr() for t in pages), seq_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1], S, nh, nkv, hd,
-        n_pages, scale, window or 0, _ptr(sinks), part.data_ptr(), max_pages, raw_stream()), "kv8_attention", launches=plan[0])
+        q.data_ptr(), out.data_ptr(), *(t.data_ptr() for t in pages), seq_lens.data_ptr(), _ptr(row_seq), 0 if row_seq is None else 1,
+        block_table.data_ptr(), block_table.shape[1], S, nh, nkv, hd, n_pages, scale, window or 0, _ptr(sinks), part.data_ptr(), max_pages, raw_stream()), "kv8_attention", launches=plan[0])
     return out
 
 
@@ -293,6 +297,13 @@ def kv8_attention(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tens
             return kv8_decode(q, pages, ctx.seq_lens, block_table, nh, scale, window, ctx.max_len, sinks)
         return kv8_rows(q, pages, ctx.seq_lens, block_table, nh, scale, window, ctx.max_len, softcap=softcap, sinks=sinks, chunk=chunk,
                         out=out, out_col=out_col, out_scale=out_scale)
+    if (ctx.max_new <= FEW_NEW_TOKENS and out is None and softcap is None and chunk is None and out_scale == 1.0
+            and kv8_decode_supported(q.dtype, nh, nkv, hd, q.shape[0])):
+        T = q.shape[0]
+        if not (ctx.positions.dtype == ctx.seq_of_token.dtype == torch.int32) or min(ctx.positions.numel(), ctx.seq_of_token.numel()) < T or block_table.dim() != 2:
+            raise KernelError("kv8_attention: a position and a sequence per token (int32), and a table [sequences, pages]")
+        _check_device("kv8_attention", q, *pages, ctx.positions, ctx.seq_of_token, block_table, sinks)
+        return kv8_decode(q, pages, ctx.positions, block_table, nh, scale, window, ctx.max_len, sinks, ctx.seq_of_token)
     from . import attention
     _check_host("kv8_attention", ctx, block_table)
     _check_device("kv8_attention", q, *pages, ctx.seq_lens, block_table, sinks, out)
