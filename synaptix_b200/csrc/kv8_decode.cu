@@ -660,10 +660,12 @@ static int kd_blocks(int S, int nkv, int max_pages) {
 }
 // kernels that a launch makes, and floats of `part` it needs
 extern "C" int sx_kv8_decode_plan(int S, int nh, int nkv, int hd, int max_pages, long long* floats) {
+  *floats = 0;
   if (nkv <= 0) return 0;
+  if (kd_by_pair(S, nkv, max_pages)) return 1;                  // (a warp's only part is in shared memory)
   const int blocks = kd_blocks(S, nkv, max_pages);
   *floats = (long long)blocks * (KD_MAX_WARPS + 2) * (nh / nkv) * (hd + 2);
-  return kd_by_pair(S, nkv, max_pages) || blocks == 1 ? 1 : 2;
+  return blocks == 1 ? 1 : 2;
 }
 
 // A row of q is a sequence's only token (row_seq null, len_add 0), or any token: seq_lens then holds positions, len_add is 1 and row_seq says whose
@@ -673,7 +675,7 @@ extern "C" int sx_kv8_decode(const void* q, void* out, const void* k, const void
                              const float* sinks, float* part, int max_pages, cudaStream_t stream) {
   if (S <= 0) return 0;
   if ((hd != 64 && hd != 128) || nkv <= 0 || nh <= 0 || nh % nkv || nh / nkv > 16 || S >= KD_MAX_SEQS || n_pages <= 0 || maxp <= 0 || max_pages <= 0 ||
-      (long long)S * nkv * maxp >= (1ll << 31) || (long long)S * nh >= (1ll << 31) || !part)
+      (long long)S * nkv * maxp >= (1ll << 31) || (long long)S * nh >= (1ll << 31) || (!part && !kd_by_pair(S, nkv, max_pages)))
     return SX_ERR_SIZE;
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k | (uintptr_t)v | (uintptr_t)k_exp | (uintptr_t)v_exp | (uintptr_t)part) & 15) return SX_ERR_ALIGN;
   int* status = kd_status();

@@ -12,7 +12,7 @@ from typing import NamedTuple, Optional, Tuple
 import numpy as np
 import torch
 
-from ._lib import KernelError, c_int, check, dt_code, fn, good, launcher, raw_stream, require_cuda
+from ._lib import KernelError, c_int, check, dt_code, fn, launcher, raw_stream, require_cuda
 from .decode import sm_count
 
 current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
@@ -49,38 +49,47 @@ def kv8_shapes(n_pages: int, nkv: int, hd: int) -> Tuple[tuple, tuple, tuple]:
     return (n_pages, nkv, hd // b, PAGE, b), (n_pages, nkv, hd, PAGE), (n_pages, nkv, PAGE)
 
 
-def _check_pages(pages: KV8Pages, what: str, nkv: Optional[int] = None, hd: Optional[int] = None) -> Tuple[int, int, int]:
+_SHAPES = {}                    # of the values' shape: those of keys and exponents, or what is wrong with it
+
+
+def _shapes_beside(v_shape, what: str):
+    both = _SHAPES.get(v_shape)
+    if both is None:
+        if len(v_shape) != 4 or v_shape[3] != PAGE:
+            raise KernelError(f"{what}: values are [n_pages, kv heads, head size, 64]")
+        n, kv, d = v_shape[:3]
+        if not kv8_supported(d):
+            raise KernelError(f"{what}: head sizes are multiples of 16 up to {MAX_HEAD_DIM}")
+        if n < 1 or kv < 1:
+            raise KernelError(f"{what}: no pages, or no heads")
+        k, _, e = kv8_shapes(n, kv, d)
+        both = _SHAPES[v_shape] = (torch.Size(k), torch.Size(e))
+    return both
+
+
+def _check_pages(pages: KV8Pages, what: str, nkv: Optional[int] = None, hd: Optional[int] = None):
     k, v, ke, ve = pages
     u8 = torch.uint8
-    if not (k.dtype == v.dtype == ke.dtype == ve.dtype == u8):
+    if k.dtype is not u8 or v.dtype is not u8 or ke.dtype is not u8 or ve.dtype is not u8:
         raise KernelError(f"{what}: codes and exponents are uint8")
-    if v.dim() != 4:
-        raise KernelError(f"{what}: values are [n_pages, kv heads, head size, 64]")
-    n, kv, d, page = v.shape
-    if (nkv is not None and nkv != kv) or (hd is not None and hd != d):
-        raise KernelError(f"{what}: the pages hold {kv} heads of {d}, not {nkv} of {hd}")
-    if not kv8_supported(d):
-        raise KernelError(f"{what}: head sizes are multiples of 16 up to {MAX_HEAD_DIM}")
-    b = 64 if d % 64 == 0 else 32 if d % 32 == 0 else 16
-    if page != PAGE or k.shape != (n, kv, d // b, PAGE, b) or ke.shape != (n, kv, PAGE) or ve.shape != (n, kv, PAGE):
-        raise KernelError(f"{what}: codes or exponents have the wrong shape (want %s, %s, %s)" % kv8_shapes(n, kv, d))
-    if n < 1 or kv < 1:
-        raise KernelError(f"{what}: no pages, or no heads")
-    return n, kv, d
+    vs = v.shape
+    ks, es = _SHAPES.get(vs) or _shapes_beside(vs, what)
+    if k.shape != ks or ke.shape != es or ve.shape != es:
+        raise KernelError(f"{what}: codes or exponents have the wrong shape (want %s, %s, %s)" % (tuple(ks), tuple(vs), tuple(es)))
+    if nkv is not None and (nkv != vs[1] or hd != vs[2]):
+        raise KernelError(f"{what}: the pages hold {vs[1]} heads of {vs[2]}, not {nkv} of {hd}")
+    return vs
 
 
 def _check_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
     """Behind all other checks: contiguous tensors of the current CUDA device."""
-    device = None
+    device = tensors[0].get_device()
     for t in tensors:
-        if t is None:
-            continue
-        if not good(t):
+        if t is not None and (t.get_device() != device or not t.is_contiguous()):
             require_cuda(t)
-        if device is None:
-            device = t.get_device()
-        elif t.get_device() != device:
             raise KernelError(f"{what}: tensors lie on several devices")
+    if device < 0:
+        require_cuda(tensors[0])
     if device != current_device():
         raise KernelError(f"{what}: the tensors lie on cuda:{device}, the current device is cuda:{current_device()}")
 
@@ -107,11 +116,12 @@ def kv8_prepare(qkv: torch.Tensor, q_out: Optional[torch.Tensor], pages: Optiona
     k = v = ke = ve = None
     n_pages = 0
     if pages is not None:
-        n_pages, _, _ = _check_pages(pages, "kv8_prepare", nkv, hd)
+        n_pages = _check_pages(pages, "kv8_prepare", nkv, hd)[0]
         k, v, ke, ve = pages
     elif not kv8_supported(hd):
         raise KernelError(f"kv8_prepare: head sizes are multiples of 16 up to {MAX_HEAD_DIM}")
-    if not (positions.dtype == seq_of_token.dtype == block_table.dtype == torch.int32):
+    i32, f32 = torch.int32, torch.float32
+    if positions.dtype is not i32 or seq_of_token.dtype is not i32 or block_table.dtype is not i32:
         raise KernelError("kv8_prepare: index tensors are int32")
     if qkv.dim() != 2 or block_table.dim() != 2:
         raise KernelError("kv8_prepare: qkv is [T, row], with a position and a sequence per token and a table [sequences, pages]")
@@ -122,22 +132,23 @@ def kv8_prepare(qkv: torch.Tensor, q_out: Optional[torch.Tensor], pages: Optiona
         raise KernelError("kv8_prepare: the heads do not fit the rows of qkv")
     if nh and (q_out is None or q_out.dtype != qkv.dtype or q_out.shape != (T, nh * hd)):
         raise KernelError("kv8_prepare: q_out is [T, nh * hd] in qkv's dtype")
-    for w in (wq, wk):
-        if w is not None and (w.dtype != torch.float32 or w.numel() != hd):
-            raise KernelError("kv8_prepare: gains are float32, one per element of a head")
+    if (wq is not None and (wq.dtype is not f32 or wq.numel() != hd)) or (wk is not None and (wk.dtype is not f32 or wk.numel() != hd)):
+        raise KernelError("kv8_prepare: gains are float32, one per element of a head")
     if inv_freq is None:
         rotary_dim = 0
-    elif inv_freq.dtype != torch.float32 or rotary_dim % 2 or not 0 < rotary_dim <= hd or inv_freq.numel() != rotary_dim // 2:
+    elif inv_freq.dtype is not f32 or rotary_dim % 2 or not 0 < rotary_dim <= hd or inv_freq.numel() != rotary_dim // 2:
         raise KernelError("kv8_prepare: inv_freq is float32 with a frequency per rotated pair of the head")
     dt = dt_code(qkv.dtype)
     _check_device("kv8_prepare", qkv, q_out, k, v, ke, ve, wq, wk, inv_freq, positions, seq_of_token, block_table)
-    es = qkv.element_size()
-    args = [qkv.data_ptr() + col * es, _ptr(q_out), _ptr(k), _ptr(v), _ptr(ke), _ptr(ve), _ptr(wq), _ptr(wk), _ptr(inv_freq)]
-    wide = (T >= WIDE_MIN_TOKENS and hd in (64, 128) and (inv_freq is None or rotary_dim == hd) and row * es % 16 == 0
-            and not any(p is not None and p % 16 for p in args))
+    es = 4 if dt == 0 else 2
+    a_qkv, a_q, a_wq, a_wk = qkv.data_ptr() + col * es, _ptr(q_out), _ptr(wq), _ptr(wk)
+    a_k, a_v = _ptr(k), _ptr(v)
+    wide = (T >= WIDE_MIN_TOKENS and hd in (64, 128) and (inv_freq is None or rotary_dim == hd)
+            and not (row * es | a_qkv | (a_q or 0) | (a_k or 0) | (a_v or 0) | (a_wq or 0) | (a_wk or 0)) & 15)
     check(launcher("kv8", "sx_kv8_prepare")(
-        *args, rotary_dim, eps, positions.data_ptr(), seq_of_token.data_ptr(), block_table.data_ptr(), block_table.shape[1], T, nh, nkv, hd, n_pages,
-        row, wide, dt, raw_stream()), "kv8_prepare", launches=1 if T and (nh or k is not None) else 0)
+        a_qkv, a_q, a_k, a_v, _ptr(ke), _ptr(ve), a_wq, a_wk, _ptr(inv_freq), rotary_dim, eps, positions.data_ptr(), seq_of_token.data_ptr(),
+        block_table.data_ptr(), block_table.shape[1], T, nh, nkv, hd, n_pages, row, wide, dt, raw_stream()), "kv8_prepare",
+        launches=1 if T and (nh or k is not None) else 0)
 
 
 def _read_plan(ctx, width: int, window: Optional[int], chunk: Optional[int], device):
@@ -181,7 +192,7 @@ def kv8_read(pages: KV8Pages, ctx, block_table: torch.Tensor, dtype: torch.dtype
     ``k``, ``v`` ``[n, kv heads, 64, hd]`` the pages one sequence after the other and ``table`` int32 ``[sequences, pages]`` the page
     of each.  Rows behind a sequence's end are zero.  With ``window`` or ``chunk`` pages that no token of the step sees are left
     out (their place in the table names another page).  Needs the step's lengths on the host."""
-    n_pages, nkv, hd = _check_pages(pages, "kv8_read")
+    n_pages, nkv, hd, _ = _check_pages(pages, "kv8_read")
     _check_host("kv8_read", ctx, block_table)
     if (window is not None and window < 1) or (chunk is not None and chunk < 1):
         raise KernelError("kv8_read: window and chunk are positive")
@@ -242,20 +253,25 @@ def kv8_decode(q: torch.Tensor, pages: KV8Pages, seq_lens: torch.Tensor, block_t
                row_seq: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One query token a sequence (row ``s`` of ``q``) on the tensor cores; sizes as ``kv8_decode_supported`` says.  With ``row_seq`` a row is any
     token: ``row_seq`` names its sequence and ``seq_lens`` holds its position."""
-    n_pages, nkv, hd = pages.v.shape[:3]
-    S = q.shape[0]
-    max_pages = min(-(-max_len // PAGE), block_table.shape[1]) if window is None else min(-(-max_len // PAGE), block_table.shape[1], (window + 126) // PAGE)
-    shape = (S, nh, nkv, hd, max_pages, q.get_device())
+    k, v, ke, ve = pages
+    n_pages, nkv, hd, _ = v.shape
+    S, maxp = q.shape[0], block_table.shape[1]
+    max_pages = min(-(-max_len // PAGE), maxp)
+    if window is not None:
+        max_pages = min(max_pages, (window + 126) // PAGE)
+    device = q.get_device()
+    shape = (S, nh, nkv, hd, max_pages, device)
     plan = _DECODE_PLANS.get(shape)
     if plan is None:
         floats = ctypes.c_longlong(0)
         launches = fn("kv8_decode", "sx_kv8_decode_plan")(*map(c_int, shape[:5]), ctypes.byref(floats))
         plan = _DECODE_PLANS[shape] = (launches, floats.value)
     out = torch.empty_like(q)
-    part = torch.empty(plan[1], dtype=torch.float32, device=q.device)
+    part = torch.empty(plan[1], dtype=torch.float32, device=q.device) if plan[1] else None
     check(launcher("kv8_decode", "sx_kv8_decode")(
-        q.data_ptr(), out.data_ptr(), *(t.data_ptr() for t in pages), seq_lens.data_ptr(), _ptr(row_seq), 0 if row_seq is None else 1,
-        block_table.data_ptr(), block_table.shape[1], S, nh, nkv, hd, n_pages, scale, window or 0, _ptr(sinks), part.data_ptr(), max_pages, raw_stream()), "kv8_attention", launches=plan[0])
+        q.data_ptr(), out.data_ptr(), k.data_ptr(), v.data_ptr(), ke.data_ptr(), ve.data_ptr(), seq_lens.data_ptr(), _ptr(row_seq),
+        0 if row_seq is None else 1, block_table.data_ptr(), maxp, S, nh, nkv, hd, n_pages, scale, window or 0, _ptr(sinks), _ptr(part), max_pages,
+        raw_stream()), "kv8_attention", plan[0])
     return out
 
 
@@ -276,8 +292,9 @@ def kv8_attention(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tens
     Single tokens attend over the codes.  Portions of prompts read the pages back once (``kv8_read``) and attend over the result
     with the kernels of the 16- and 32-bit cache: a page serves many rows there, and turning its codes again in every block that
     reads it would cost more than writing it out once."""
-    n_pages, _, _ = _check_pages(pages, "kv8_attention", nkv, hd)
-    if not (ctx.seq_lens.dtype == block_table.dtype == torch.int32):
+    _check_pages(pages, "kv8_attention", nkv, hd)
+    seq_lens = ctx.seq_lens
+    if seq_lens.dtype is not torch.int32 or block_table.dtype is not torch.int32:
         raise KernelError("kv8_attention: index tensors are int32")
     dt_code(q.dtype)
     if nh < 1 or nh % nkv or q.dim() != 2 or q.shape[1] != nh * hd:
@@ -290,12 +307,13 @@ def kv8_attention(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tens
                             or out_col + nh * hd > out.shape[1] or not out.is_contiguous()):
         raise KernelError("kv8_attention: the output does not fit")
     if ctx.all_single and ctx.n_seqs == q.shape[0]:
-        if block_table.dim() != 2 or block_table.shape[0] < ctx.n_seqs or ctx.seq_lens.numel() < ctx.n_seqs:
+        if block_table.dim() != 2 or block_table.shape[0] < ctx.n_seqs or seq_lens.numel() < ctx.n_seqs:
             raise KernelError("kv8_attention: a row of the table and a length per sequence")
-        _check_device("kv8_attention", q, *pages, ctx.seq_lens, block_table, sinks, out)
+        k, v, ke, ve = pages
+        _check_device("kv8_attention", q, k, v, ke, ve, seq_lens, block_table, sinks, out)
         if out is None and softcap is None and chunk is None and out_scale == 1.0 and kv8_decode_supported(q.dtype, nh, nkv, hd, q.shape[0]):
-            return kv8_decode(q, pages, ctx.seq_lens, block_table, nh, scale, window, ctx.max_len, sinks)
-        return kv8_rows(q, pages, ctx.seq_lens, block_table, nh, scale, window, ctx.max_len, softcap=softcap, sinks=sinks, chunk=chunk,
+            return kv8_decode(q, pages, seq_lens, block_table, nh, scale, window, ctx.max_len, sinks)
+        return kv8_rows(q, pages, seq_lens, block_table, nh, scale, window, ctx.max_len, softcap=softcap, sinks=sinks, chunk=chunk,
                         out=out, out_col=out_col, out_scale=out_scale)
     if (ctx.max_new <= FEW_NEW_TOKENS and out is None and softcap is None and chunk is None and out_scale == 1.0
             and kv8_decode_supported(q.dtype, nh, nkv, hd, q.shape[0])):
