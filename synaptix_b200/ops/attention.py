@@ -315,6 +315,47 @@ def attn_prefill_tc(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     return out
 
 
+TC_KEY_BLOCK = 128
+
+
+def tc_parts(tiles, nh: int, window: Optional[int], device) -> Tuple[int, int]:
+    """``(blocks of 128 keys a part, parts of the longest tile)`` where the tiles' keys are better cut into parts, else ``(0, 1)``.  ``tiles``:
+    (first position, last position) of each 128-row tile.  A block takes 4.5 us and 1.1 a key block; three parts an SM even the blocks out, and fewer than
+    eight key blocks are not worth a block of their own."""
+    counts = []
+    for first, last in tiles:
+        lo = max(0, first - window + 1) // TC_KEY_BLOCK if window else 0
+        counts.append(last // TC_KEY_BLOCK + 1 - lo)
+    sms = sm_count(device)
+    most, total = max(counts), sum(counts) * nh
+    chunk = max(8, -(-total // (3 * sms)))
+    # whole tiles: the longest one, or all of them dealt out evenly, whatever takes longer (in key blocks; a block's 4.5 us are four of them)
+    whole = max(most + 4, -(-len(counts) * nh // sms) * (total / (len(counts) * nh) + 4))
+    cut = total / sms + 4 * sum(-(-c // chunk) for c in counts) * nh / sms + (chunk + 4) / 2 + 6
+    return (chunk, -(-most // chunk)) if most > chunk and cut < whole else (0, 1)
+
+
+def attn_prefill_tc_parts(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tile_seq: torch.Tensor, tile_q0: torch.Tensor,
+                          seq_of_token: torch.Tensor, cu_seqlens: torch.Tensor, seq_past: torch.Tensor, seq_lens: torch.Tensor,
+                          block_table: torch.Tensor, nh: int, nkv: int, hd: int, scale: float, window: Optional[int], chunk: int, parts: int,
+                          sinks: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``attn_prefill_tc`` with every tile's keys cut into stretches of ``chunk`` blocks of 128, ``parts`` for the longest tile (``tc_parts``), which
+    blocks of their own take and a second kernel joins."""
+    require_cuda(q, k_pages, v_pages, tile_seq, tile_q0, seq_of_token, cu_seqlens, seq_past, seq_lens, block_table, sinks)
+    _check_sinks(sinks, nh)
+    T = q.shape[0]
+    if not tc_prefill_supported(q.dtype, nh, nkv, hd) or k_pages.dtype != q.dtype:
+        raise KernelError("attn_prefill_tc: bfloat16 and head size 128")
+    out = torch.empty((T, nh * hd), dtype=q.dtype, device=q.device)
+    part = torch.empty(parts * T * nh * (hd + 4), dtype=torch.float32, device=q.device)
+    check(launcher("attn_tc", "sx_attn_prefill_tc_parts")(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), part.data_ptr(), T, k_pages.shape[0], tile_seq.data_ptr(),
+        tile_q0.data_ptr(), tile_seq.numel(), seq_of_token.data_ptr(), cu_seqlens.data_ptr(), seq_past.data_ptr(), seq_lens.data_ptr(),
+        block_table.data_ptr(), block_table.shape[1], nh, nkv, hd, scale, 0 if window is None else int(window),
+        None if sinks is None else sinks.data_ptr(), chunk, parts, raw_stream()), "attn_prefill_tc_parts", launches=2)
+    return out
+
+
 def attn_tc_status(reset: bool = False) -> int:
     """0, or which bounded wait of the tcgen05 attention kernel ran out (1 producer, 2-5 MMA issuer, 6-9
     softmax).  No device call (the word lies in host memory the device writes to); it tells of launches the host

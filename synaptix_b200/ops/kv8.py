@@ -236,8 +236,10 @@ def kv8_rows(q: torch.Tensor, pages: KV8Pages, seq_lens: torch.Tensor, block_tab
 DECODE_HEAD_DIMS = (64, 128)
 DECODE_MAX_GROUP = 16
 DECODE_MAX_SEQS = 2047
-# Portions of up to this many tokens a sequence: every token attends by itself over the codes
-FEW_NEW_TOKENS = 4
+# Portions of up to this many tokens a sequence: every token attends by itself over the codes.  Measured, us, reading back and by token, 32 heads over 8
+# of 128: 2 tokens over 2,000 keys 20 and 11.5, over 20,000 80 and 22; 8 tokens 20 and 16, 80 and 48, of 32 sequences with 3,000 keys 260 and 107;
+# 16 tokens 20 and 20, 81 and 80, 260 and 199, but 5 x 16 over 9,000 135 and 118 and 32 tokens 84 and 146
+FEW_NEW_TOKENS = 8
 
 
 def kv8_decode_supported(dtype, nh: int, nkv: int, hd: int, S: int) -> bool:
@@ -322,9 +324,20 @@ def kv8_attention(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tens
             raise KernelError("kv8_attention: a position and a sequence per token (int32), and a table [sequences, pages]")
         _check_device("kv8_attention", q, *pages, ctx.positions, ctx.seq_of_token, block_table, sinks)
         return kv8_decode(q, pages, ctx.positions, block_table, nh, scale, window, ctx.max_len, sinks, ctx.seq_of_token)
-    from . import attention
+    from . import TC_TILE_ROWS, _query_tiles, attention, tc_prefill_supported
+    from .attention import attn_prefill_tc_parts, tc_parts
     _check_host("kv8_attention", ctx, block_table)
     _check_device("kv8_attention", q, *pages, ctx.seq_lens, block_table, sinks, out)
     k, v, table = kv8_read(pages, ctx, block_table, q.dtype, window, chunk)
+    if out is None and softcap is None and chunk is None and out_scale == 1.0 and tc_prefill_supported(q.dtype, nh, nkv, hd):
+        cut = ctx.scratch.get(("kv8_parts", nh, window))
+        if cut is None:
+            cu, past = ctx.host["cu_seqlens"], ctx.host["seq_past"]
+            tiles = [(p + q0, min(p + q0 + TC_TILE_ROWS, p + b - a) - 1) for a, b, p in zip(cu, cu[1:], past) for q0 in range(0, b - a, TC_TILE_ROWS)]
+            cut = ctx.scratch[("kv8_parts", nh, window)] = tc_parts(tiles, nh, window, q.device)
+        if cut[1] > 1:
+            tile_seq, tile_q0 = _query_tiles(ctx, TC_TILE_ROWS, q.device)
+            return attn_prefill_tc_parts(q, k, v, tile_seq, tile_q0, ctx.seq_of_token, ctx.cu_seqlens, ctx.seq_past, ctx.seq_lens, table, nh, nkv, hd,
+                                         scale, window, *cut, sinks=sinks)
     return attention(q, k, v, ctx, table, nh, nkv, hd, scale, window, softcap=softcap, sinks=sinks, chunk=chunk, out=out, out_col=out_col,
                      out_scale=out_scale)

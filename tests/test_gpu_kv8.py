@@ -331,6 +331,38 @@ def test_portions(dtype, nh, nkv, hd, lens, new, options):
         assert ((got[part] - want).abs() <= tol).all(), (s, ((got[part] - want).abs() / tol).max().item())
 
 
+@pytest.mark.parametrize("lens,new", [([6000], [70]), ([7000, 500, 129], [130, 300, 129]), ([8000, 64], [9, 6])])
+@pytest.mark.parametrize("options", [{}, dict(window=4500), dict(sinks=True), dict(window=4001, sinks=True)])
+def test_portions_over_long_caches(lens, new, options):
+    """Few tiles of many keys: cut over the keys (``tc_parts``) and joined."""
+    from synaptix_b200.ops.attention import tc_parts
+    nh, nkv, hd = 16, 2, 128
+    tiles = [(n - m + q0, min(n - m + q0 + 128, n) - 1) for n, m in zip(lens, new) for q0 in range(0, m, 128)]
+    assert tc_parts(tiles, nh, options.get("window"), torch.device("cuda", 0))[1] > 1
+    options = dict(options, sinks=randn(nh, seed=9) * 3) if options.get("sinks") else options
+    check(2 * randn(sum(new), nh, hd, seed=3), filled(lens, nkv, hd), lens, new, nh, hd, torch.bfloat16, True, **options)
+
+
+def test_when_keys_are_cut():
+    from synaptix_b200.ops.attention import tc_parts
+    d = torch.device("cuda", 0)
+    assert tc_parts([(0, 127)], 32, None, d) == (0, 1)                       # one block of keys
+    assert tc_parts([(128 * i, 128 * i + 127) for i in range(64)], 32, None, d) == (0, 1)   # a long prompt fills the SMs as it is
+    chunk, parts = tc_parts([(100000, 100063)], 32, None, d)
+    assert chunk * parts >= 782 > chunk * (parts - 1) and parts * 32 >= 148
+    assert tc_parts([(100000, 100063)], 32, 500, d)[1] == 1                  # a window leaves few
+
+
+@pytest.mark.parametrize("new", [[2], [4, 1, 8], [1, 4], [8, 1, 1]])
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (32, 8, 128), (12, 1, 128), (5, 1, 64)])
+@pytest.mark.parametrize("options", [{}, dict(window=33), dict(sinks=True)])
+def test_a_few_tokens(new, nh, nkv, hd, options):
+    """Portions of up to eight tokens attend over the codes, token by token."""
+    lens = [m + past for m, past in zip(new, (300, 62, 0))]
+    options = dict(options, sinks=randn(nh, seed=9)) if options.get("sinks") else options
+    check(2 * randn(sum(new), nh, hd, seed=3), filled(lens, nkv, hd), lens, new, nh, hd, torch.bfloat16, True, **options)
+
+
 # ---- as a model uses them
 
 def held_rows(engine, slot, layer, n):
