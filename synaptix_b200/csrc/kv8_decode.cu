@@ -8,7 +8,7 @@
 //     block's end, one that several blocks share by a second, small kernel.  Where every pair has a block and no more than two pages a warp,
 //     blocks take pairs instead and there is no second kernel.
 //   * A warp has its own ring of shared memory, filled by untiled bulk copies (K and V tile of a page are one stretch of memory each;
-//     no tensor map; the exponents come by plain loads an item ahead, since a copy of 64 bytes costs as much to ask for as one of 8 KB), and no barrier with other warps on the way.  K and V take turns in the slots, so a slot is free again after half a page.
+//     no tensor map; the exponents come by cp.async three items ahead, since a bulk copy of 64 bytes costs as much to ask for as one of 8 KB), and no barrier with other warps on the way.  K and V take turns in the slots, so a slot is free again after half a page.
 //   * q k^T: m16n8k32 on the codes as they are.  A bfloat16 query (8 bits of mantissa) is the sum of TWO e4m3 numbers of 4 bits each: the
 //     G <= 8 heads' larger parts are the fragment's rows 0-7, the rests rows 8-15 that would be idle, and the two results are added.  Queries
 //     are scaled by a power of two so that the row's largest lies in 2^7 .. 2^8: elements down to 2^-9 of that are exact, smaller ones off by at
@@ -37,10 +37,11 @@ template <int HD, bool MORE> struct KdLayout {
   static constexpr int WARPS = MORE ? 8 : 12;
   static constexpr int TILE = SX_PAGE * HD;
   static constexpr int SLOTS = (MORE ? 3 : 2) * (128 / HD);
-  static constexpr int AHEAD = (SLOTS + 1) / 2;                 // items whose tiles are under way ahead of the one at work
+  static constexpr int AHEAD = 3;                               // items whose exponents (and at most whose tiles) are under way ahead of the one at work
+  static constexpr int EXPS = 2 * SX_PAGE;                      // an item's exponents of keys and values
   static constexpr int PART = HD + 2;                           // a row's maximum, sum and result
   static constexpr int RING = WARPS * SLOTS * TILE;
-  static constexpr int smem() { return RING + WARPS * KD_DESC * (int)sizeof(int4) + KD_MAX_SEQS * (int)sizeof(int); }
+  static constexpr int smem() { return RING + WARPS * (KD_DESC * (int)sizeof(int4) + (AHEAD + 1) * EXPS) + KD_MAX_SEQS * (int)sizeof(int); }
 };
 #define KD_MAX_WARPS 12
 
@@ -149,7 +150,8 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
   __shared__ __align__(8) uint64_t bars[WARPS * L::SLOTS];
   __shared__ int warp_sums[WARPS], first_unit[WARPS], last_unit[WARPS];
   int4* desc_all = reinterpret_cast<int4*>(smem + L::RING);
-  int* start = reinterpret_cast<int*>(smem + L::RING + WARPS * KD_DESC * sizeof(int4));
+  unsigned char* exps = smem + L::RING + WARPS * KD_DESC * sizeof(int4) + (threadIdx.x >> 5) * (L::AHEAD + 1) * L::EXPS;
+  int* start = reinterpret_cast<int*>(smem + L::RING + WARPS * (KD_DESC * sizeof(int4) + (L::AHEAD + 1) * L::EXPS));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   if (lane == 0) {
 #pragma unroll
@@ -287,7 +289,6 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
 
   bool ok = true;
   int done = 0;
-  uint4 ke4 = make_uint4(0, 0, 0, 0), ve4 = ke4, ke4_next = ke4, ve4_next = ke4;       // exponents of the thread's keys 16 t ..
   for (int i = -L::AHEAD; i < n_items; ++i) {
     if (((i + L::AHEAD) & 31) == 0) {                           // the next 32 items
       const int x = i + L::AHEAD + lane;
@@ -300,14 +301,12 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
       if (i == -L::AHEAD)
         for (int n = 0; n < L::SLOTS; ++n) issue(n);
     }
-    ke4 = ke4_next;
-    ve4 = ve4_next;
-    if (i >= -1 && i + 1 < n_items) {
-      const int4 d = desc[(i + 1) & (KD_DESC - 1)];
-      const size_t at = ((size_t)d.w * a.nkv + d.y) * SX_PAGE + 16 * t;
-      ke4_next = *reinterpret_cast<const uint4*>(a.ke + at);
-      ve4_next = *reinterpret_cast<const uint4*>(a.ve + at);
+    if (lane < 8 && i + L::AHEAD < n_items) {                   // exponents: four lanes for the keys', four for the values'
+      const int4 d = desc[(i + L::AHEAD) & (KD_DESC - 1)];
+      const uint8_t* src = (lane < 4 ? a.ke : a.ve) + ((size_t)d.w * a.nkv + d.y) * SX_PAGE + 16 * t;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 16;\n" ::"r"(kd_smem(exps + ((i + L::AHEAD) & L::AHEAD) * L::EXPS + 16 * lane)), "l"(src) : "memory");
     }
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
     if (i < 0) continue;
     done = i;
     const int4 d = desc[i & (KD_DESC - 1)];
@@ -345,8 +344,11 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
 #pragma unroll
       for (int e = 0; e < 2 * RP; ++e) s[j][e] = acc[e] + (MORE ? rest[e] : acc[2 + e]);
     }
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(L::AHEAD) : "memory");      // this item's are there, those of the next ones may be on their way
     __syncwarp();
     issue(n + L::SLOTS);
+    const uint4 ke4 = *reinterpret_cast<const uint4*>(exps + (i & L::AHEAD) * L::EXPS + 16 * t);     // of the thread's keys 16 t ..
+    const uint4 ve4 = *reinterpret_cast<const uint4*>(exps + (i & L::AHEAD) * L::EXPS + SX_PAGE + 16 * t);
     const uint32_t ke[4] = {ke4.x, ke4.y, ke4.z, ke4.w};
     float top[RP];
 #pragma unroll
