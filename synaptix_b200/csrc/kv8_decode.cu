@@ -31,8 +31,9 @@
 #define KD_DESC 64               // items a warp knows ahead: two batches of 32
 #define KD_LOG2E 1.44269504f
 
-// Three warps a scheduler hide one another's latencies (a page takes a warp alone 3,400 clocks, HBM delivers one to an SM every 710); with more
-// than 8 heads a kv head a thread has two rows' registers, and there two warps.
+// Three warps a scheduler hide one another's latencies: a page takes a warp alone 3,400 clocks, and HBM delivers one to an SM every 710 (four at head
+// size 64 and three slots each: 33.0 us for 64 sequences seeing 1,000 keys where three take 31.5).  With more than 8 heads a kv head a thread has two
+// rows' registers, and there are two.
 template <int HD, bool MORE> struct KdLayout {
   static constexpr int WARPS = MORE ? 8 : 12;
   static constexpr int TILE = SX_PAGE * HD;
@@ -500,51 +501,55 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
   const bool met = mine < 0 || (lane < 16 ? k_ > 0 && before == fu : lu == fu);
   const bool alone = mine_from >= first_of(k_) && mine_from + mine_n <= first_of(k_ + 1);      // written by its warp
   const uint32_t joins = __ballot_sync(0xffffffffu, !met && !alone);
+  int turn = warp;                                              // rows go to the warps in turn
 #pragma unroll 1
-  for (int r = warp; r < __popc(joins) * G; r += WARPS) {
-    const int row = r % G;
-    uint32_t left = joins;
-    for (int j = r / G; j > 0; --j) left &= left - 1;
+  for (uint32_t left = joins; left; left &= left - 1) {
     const int from_lane = __ffs(left) - 1;
     const int u = __shfl_sync(0xffffffffu, mine, from_lane), us = __shfl_sync(0xffffffffu, mine_s, from_lane);
     const int from = __shfl_sync(0xffffffffu, mine_from, from_lane), n = __shfl_sync(0xffffffffu, mine_n, from_lane);
-    const int head = __shfl_sync(0xffffffffu, mine_h, from_lane) * G + row;
+    const int head0 = __shfl_sync(0xffffffffu, mine_h, from_lane) * G;
     const bool final = from >= b0 && from + n <= b1, has = lane < WARPS && fu >= 0 && fu <= u && u <= lu;
     const uint32_t have = __ballot_sync(0xffffffffu, has);      // warps with a part of u
-    float2 v[WARPS][HD / 64];
+    const uint32_t inside = have & ~__ballot_sync(0xffffffffu, u == lu);       // those for whom it is not the last one
+#pragma unroll 1
+    for (; turn < G; turn += WARPS) {
+      const int row = turn, head = head0 + row;
+      float2 v[WARPS][HD / 64];
 #pragma unroll
-    for (int k = 0; k < WARPS; ++k) {
-      const float* src = part_of(k, u == last_unit[k]) + row * L::PART + 2 + 2 * lane;
+      for (int k = 0; k < WARPS; ++k) {
+        const float* src = part_of(k, !(inside >> k & 1)) + row * L::PART + 2 + 2 * lane;
 #pragma unroll
-      for (int h = 0; h < HD / 64; ++h) v[k][h] = have >> k & 1 ? *reinterpret_cast<const float2*>(src + 64 * h) : make_float2(0.f, 0.f);
-    }
-    const float2 ml = has ? *reinterpret_cast<const float2*>(part_of(lane, u == lu) + row * L::PART) : make_float2(-INFINITY, 0.f);
-    const float sink = final && a.sinks ? a.sinks[head] * KD_LOG2E : -INFINITY;
-    const float top = fmaxf(warp_max(ml.x), sink), base = top == -INFINITY ? 0.f : top;
-    float w = kd_ex2(ml.x - base);
-    const float sum = warp_sum(ml.y * w) + kd_ex2(sink - base);
-    if (final) w = sum == 0.f ? 0.f : w / sum;
-    float2 x[HD / 64];
+        for (int h = 0; h < HD / 64; ++h) v[k][h] = have >> k & 1 ? *reinterpret_cast<const float2*>(src + 64 * h) : make_float2(0.f, 0.f);
+      }
+      const float2 ml = has ? *reinterpret_cast<const float2*>(part_of(lane, u == lu) + row * L::PART) : make_float2(-INFINITY, 0.f);
+      const float sink = final && a.sinks ? a.sinks[head] * KD_LOG2E : -INFINITY;
+      const float top = fmaxf(warp_max(ml.x), sink), base = top == -INFINITY ? 0.f : top;
+      float w = kd_ex2(ml.x - base);
+      const float sum = warp_sum(ml.y * w) + kd_ex2(sink - base);
+      if (final) w = sum == 0.f ? 0.f : __fdividef(w, sum);
+      float2 x[HD / 64];
 #pragma unroll
-    for (int h = 0; h < HD / 64; ++h) x[h] = make_float2(0.f, 0.f);
+      for (int h = 0; h < HD / 64; ++h) x[h] = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < WARPS; ++k) {
-      const float f = __shfl_sync(0xffffffffu, w, k);
+      for (int k = 0; k < WARPS; ++k) {
+        const float f = __shfl_sync(0xffffffffu, w, k);
+#pragma unroll
+        for (int h = 0; h < HD / 64; ++h) {
+          x[h].x += f * v[k][h].x;
+          x[h].y += f * v[k][h].y;
+        }
+      }
+      // a pair's first stretch goes to the block's second place, one that another block began to its first
+      float* dst = a.part + ((size_t)(gridDim.x * WARPS + blockIdx.x * 2 + (from >= b0 ? 1 : 0)) * G + row) * L::PART;
+      if (!final && lane == 0) *reinterpret_cast<float2*>(dst) = make_float2(top, sum);
 #pragma unroll
       for (int h = 0; h < HD / 64; ++h) {
-        x[h].x += f * v[k][h].x;
-        x[h].y += f * v[k][h].y;
+        const int d = 2 * lane + 64 * h;
+        if (final) *reinterpret_cast<__nv_bfloat162*>(a.out + ((size_t)us * a.nh + head) * HD + d) = __floats2bfloat162_rn(x[h].x, x[h].y);
+        else *reinterpret_cast<float2*>(dst + 2 + d) = x[h];
       }
     }
-    // a pair's first stretch goes to the block's second place, one that another block began to its first
-    float* dst = a.part + ((size_t)(gridDim.x * WARPS + blockIdx.x * 2 + (from >= b0 ? 1 : 0)) * G + row) * L::PART;
-    if (!final && lane == 0) *reinterpret_cast<float2*>(dst) = make_float2(top, sum);
-#pragma unroll
-    for (int h = 0; h < HD / 64; ++h) {
-      const int d = 2 * lane + 64 * h;
-      if (final) *reinterpret_cast<__nv_bfloat162*>(a.out + ((size_t)us * a.nh + head) * HD + d) = __floats2bfloat162_rn(x[h].x, x[h].y);
-      else *reinterpret_cast<float2*>(dst + 2 + d) = x[h];
-    }
+    turn -= G;
   }
 }
 
@@ -655,7 +660,7 @@ static int kd_launch(KdArgs a, cudaStream_t stream) {
 }
 
 // a block a pair: pairs no more than SMs, of no more than two pages a warp
-static bool kd_by_pair(int S, int nkv, int max_pages) { return (long long)S * nkv <= sx_sm_count() && max_pages <= 2 * KD_MAX_WARPS; }
+static bool kd_by_pair(int S, int nkv, int max_pages) { return (long long)S * nkv <= sx_sm_count() && max_pages <= 24; }
 static int kd_blocks(int S, int nkv, int max_pages) {
   const long long items = (long long)S * nkv * max_pages, few = (items + 7) / 8;         // (the fewest warps of a block are 8)
   return kd_by_pair(S, nkv, max_pages) ? S * nkv : (int)max(1ll, min((long long)sx_sm_count(), few));
