@@ -42,7 +42,7 @@ template <int HD, bool MORE> struct KdLayout {
   static constexpr int EXPS = 2 * SX_PAGE;                      // an item's exponents of keys and values
   static constexpr int PART = HD + 2;                           // a row's maximum, sum and result
   static constexpr int RING = WARPS * SLOTS * TILE;
-  static constexpr int smem() { return RING + WARPS * (KD_DESC * (int)sizeof(int4) + (AHEAD + 1) * EXPS) + KD_MAX_SEQS * (int)sizeof(int); }
+  static constexpr int FIXED = RING + WARPS * (KD_DESC * (int)sizeof(int4) + (AHEAD + 1) * EXPS);       // ... and the starts of the sequences' items behind it
 };
 #define KD_MAX_WARPS 12
 
@@ -559,7 +559,8 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
 template <int HD>
 __global__ void __launch_bounds__(256) kv8_decode_merge_kernel(const KdArgs a) {
   constexpr int TEAMS = 256 / (HD / 2);
-  __shared__ int start[KD_MAX_SEQS + 1], warp_sums[8];
+  extern __shared__ int start[];           // (no more than the sequences need: a block of this kernel has to fit beside one of the first)
+  __shared__ int warp_sums[8];
   __shared__ float acc[TEAMS][HD], s_m[TEAMS], s_l[TEAMS];
   kd_starts<256>(a, start, warp_sums);
   const int G = a.nh / a.nkv, row = blockIdx.y, n_all = start[a.S] * a.nkv, workers = n_all ? kd_workers(a, n_all) : 0;
@@ -649,14 +650,14 @@ static int kd_launch(KdArgs a, cudaStream_t stream) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
   if (dev < 0 || dev >= 64 || !opted[dev]) {
-    e = cudaFuncSetAttribute(kv8_decode_kernel<HD, MORE>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem());
+    e = cudaFuncSetAttribute(kv8_decode_kernel<HD, MORE>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::FIXED + KD_MAX_SEQS * (int)sizeof(int));
     if (e != cudaSuccess) return (int)e;
     if (dev >= 0 && dev < 64) opted[dev] = true;
   }
   a.warps = L::WARPS;
-  const int rc = sx_launch(kv8_decode_kernel<HD, MORE>, dim3(a.blocks), dim3(L::WARPS * 32), L::smem(), stream, a);
+  const int rc = sx_launch(kv8_decode_kernel<HD, MORE>, dim3(a.blocks), dim3(L::WARPS * 32), L::FIXED + (a.S + 1) * sizeof(int), stream, a);
   if (rc || a.by_pair || a.blocks == 1) return rc;
-  return sx_launch(kv8_decode_merge_kernel<HD>, dim3(a.blocks - 1, a.nh / a.nkv), dim3(256), 0, stream, a);
+  return sx_launch(kv8_decode_merge_kernel<HD>, dim3(a.blocks - 1, a.nh / a.nkv), dim3(256), (a.S + 1) * sizeof(int), stream, a);
 }
 
 // a block a pair: pairs no more than SMs, of no more than two pages a warp
