@@ -130,8 +130,14 @@ __device__ __forceinline__ void kd_starts(const KdArgs& a, int* start, int* warp
 }
 // the blocks that work (a block of fewer items than warps would leave some idle), and the first item of block b
 __device__ __forceinline__ int kd_workers(const KdArgs& a, int n) { return max(1, min(a.blocks, (n + a.warps - 1) / a.warps)); }
-__device__ __forceinline__ int kd_first(int b, int n, int workers) { return (int)((long long)b * n / workers); }
-__device__ __forceinline__ int kd_worker_of(int item, int n, int workers) { return (int)((((long long)item + 1) * workers - 1) / n); }
+__device__ __forceinline__ int kd_first(int b, int n, int workers) {
+  const int q = n / workers;
+  return b * q + min(b, n - q * workers);
+}
+__device__ __forceinline__ int kd_worker_of(int item, int n, int workers) {
+  const int q = n / workers, longer = (n - q * workers) * (q + 1);        // items of the blocks that have one more
+  return item < longer ? item / (q + 1) : n - q * workers + (item - longer) / q;
+}
 // the sequence of item x: the last s with start[s] * nkv <= x among those that have pages
 __device__ __forceinline__ int kd_seq_of(const int* start, int S, int nkv, int x) {
   int lo = 0, hi = S - 1;
@@ -149,7 +155,7 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
   constexpr int RP = MORE ? 2 : 1, WARPS = L::WARPS;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ __align__(8) uint64_t bars[WARPS * L::SLOTS];
-  __shared__ int warp_sums[WARPS], first_unit[WARPS], last_unit[WARPS];
+  __shared__ int warp_sums[WARPS], first_unit[WARPS], last_unit[WARPS], first_seq;
   int4* desc_all = reinterpret_cast<int4*>(smem + L::RING);
   unsigned char* exps = smem + L::RING + WARPS * KD_DESC * sizeof(int4) + (threadIdx.x >> 5) * (L::AHEAD + 1) * L::EXPS;
   int* start = reinterpret_cast<int*>(smem + L::RING + WARPS * (KD_DESC * sizeof(int4) + (L::AHEAD + 1) * L::EXPS));
@@ -168,21 +174,23 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
     for (size_t i = blockIdx.x * WARPS * 32 + threadIdx.x; i < (size_t)a.S * a.nh * HD; i += gridDim.x * WARPS * 32) a.out[i] = __float2bfloat16_rn(0.f);
     return;
   }
-  // sequences without a visible key are nobody's items
-  for (int s = blockIdx.x * WARPS + warp; s < a.S; s += gridDim.x * WARPS)
-    if (start[s + 1] == start[s])
-      for (int i = lane; i < a.nh * HD; i += 32) a.out[(size_t)s * a.nh * HD + i] = __float2bfloat16_rn(0.f);
-  int b0, b1;                                                   // the block's items
+  // (Every instruction up to the first copy is latency: a kernel's code comes in cold, at some ten clocks an instruction.)
+  int b0 = 0, b1 = 0;                                           // the block's items
   if (a.by_pair) {
     const int s = blockIdx.x / a.nkv, n = start[s + 1] - start[s];
-    b0 = start[s] * a.nkv + (blockIdx.x % a.nkv) * n;
+    b0 = start[s] * a.nkv + (blockIdx.x - s * a.nkv) * n;
     b1 = b0 + n;
+    if (threadIdx.x == 0) first_seq = s;
   } else {
-    const int workers = kd_workers(a, n_all);
-    if (blockIdx.x >= workers) return;
-    b0 = kd_first(blockIdx.x, n_all, workers);
-    b1 = kd_first(blockIdx.x + 1, n_all, workers);
+    const int workers = max(1, min(a.blocks, (n_all + WARPS - 1) / WARPS));      // (as kd_workers)
+    if (blockIdx.x < workers) {
+      b0 = kd_first(blockIdx.x, n_all, workers);
+      b1 = kd_first(blockIdx.x + 1, n_all, workers);
+    }
+    for (int s = threadIdx.x; s < a.S; s += WARPS * 32)
+      if (start[s] * a.nkv <= b0 && b0 < start[s + 1] * a.nkv) first_seq = s;
   }
+  __syncthreads();
   auto first_of = [&](int w) { return b0 + (b1 - b0) * w / WARPS; };
   const int x0 = first_of(warp), n_items = first_of(warp + 1) - x0;
   int4* desc = desc_all + warp * KD_DESC;                       // (sequence, kv head, page of the sequence, page of the pool)
@@ -294,7 +302,9 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
     if (((i + L::AHEAD) & 31) == 0) {                           // the next 32 items
       const int x = i + L::AHEAD + lane;
       if (x < n_items) {
-        const int s = kd_seq_of(start, a.S, a.nkv, x0 + x), n = start[s + 1] - start[s], at = x0 + x - start[s] * a.nkv;
+        int s = first_seq;
+        while (start[s + 1] * a.nkv <= x0 + x) ++s;
+        const int n = start[s + 1] - start[s], at = x0 + x - start[s] * a.nkv;
         const int h = at / n, j = kd_range(a, s).x + at - h * n, page = a.block_table[(size_t)(a.row_seq ? a.row_seq[s] : s) * a.maxp + j];
         desc[x & (KD_DESC - 1)] = make_int4(s, h, j, (unsigned)page < (unsigned)a.n_pages ? page : 0);
       }
@@ -480,6 +490,10 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
       if ((n >> 1) < n_items) kd_wait(bar_a + n % L::SLOTS * 8, (n / L::SLOTS) & 1);
     }
   }
+  // sequences without a visible key are nobody's items
+  for (int s = blockIdx.x * WARPS + warp; s < a.S; s += gridDim.x * WARPS)
+    if (start[s + 1] == start[s])
+      for (int i = lane; i < a.nh * HD; i += 32) a.out[(size_t)s * a.nh * HD + i] = __float2bfloat16_rn(0.f);
   // ---- pairs that several warps worked at, or that go on in another block, are joined: their rows are dealt out to all warps
   const int unit1 = n_items ? seq * a.nkv + kvh : -1;
   if (lane == 0) {
