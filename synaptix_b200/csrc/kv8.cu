@@ -578,12 +578,15 @@ __global__ void __launch_bounds__(KV8_WARPS * 32) kv8_rows_kernel(const T* __res
         float x[16];
         kv8_float16(*reinterpret_cast<const uint4*>(kp + kv8_k_at(key, d, cb)), x);
 #pragma unroll
-        for (int g = 0; g < KV8_HEADS; ++g)
+        for (int g = 0; g < KV8_HEADS; ++g) {
+          float part = 0.f;                                          // (sums of 16, then of those: fewer roundings of large sums)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float4 y = *reinterpret_cast<const float4*>(q_s + g * hd + d + 4 * i);
-            s[h][g] = fmaf(y.x, x[4 * i], fmaf(y.y, x[4 * i + 1], fmaf(y.z, x[4 * i + 2], fmaf(y.w, x[4 * i + 3], s[h][g]))));
+            part = fmaf(y.x, x[4 * i], fmaf(y.y, x[4 * i + 1], fmaf(y.z, x[4 * i + 2], fmaf(y.w, x[4 * i + 3], part))));
           }
+          s[h][g] += part;
+        }
       }
     }
     const float kf[2] = {kv8_scale(a.ke[place * SX_PAGE + lane]), kv8_scale(a.ke[place * SX_PAGE + lane + 32])};
@@ -630,12 +633,15 @@ __global__ void __launch_bounds__(KV8_WARPS * 32) kv8_rows_kernel(const T* __res
             if (c + n < v0 || c + n >= v1) x[n] = 0.f;
         }
 #pragma unroll
-        for (int g = 0; g < KV8_HEADS; ++g)
+        for (int g = 0; g < KV8_HEADS; ++g) {
+          float part = 0.f;
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
             const float4 w = *reinterpret_cast<const float4*>(pw + g * SX_PAGE + c + 4 * n);
-            o[g][i] = fmaf(w.x, x[4 * n], fmaf(w.y, x[4 * n + 1], fmaf(w.z, x[4 * n + 2], fmaf(w.w, x[4 * n + 3], o[g][i]))));
+            part = fmaf(w.x, x[4 * n], fmaf(w.y, x[4 * n + 1], fmaf(w.z, x[4 * n + 2], fmaf(w.w, x[4 * n + 3], part))));
           }
+          o[g][i] += part;
+        }
       }
     }
   }

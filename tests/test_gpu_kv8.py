@@ -363,6 +363,105 @@ def test_a_few_tokens(new, nh, nkv, hd, options):
     check(2 * randn(sum(new), nh, hd, seed=3), filled(lens, nkv, hd), lens, new, nh, hd, torch.bfloat16, True, **options)
 
 
+def test_many_sequences_and_places_that_end_anywhere():
+    """More pairs than blocks, pairs that end within a warp's stretch, empty sequences between: all rows of a batch against the same rows alone."""
+    from synaptix_b200 import ops
+    g = torch.Generator().manual_seed(5)
+    nh, nkv, hd = 8, 4, 128
+    lens = torch.randint(0, 400, (150,), generator=g).tolist()
+    lens[3] = lens[4] = lens[149] = 0
+    held = filled(lens, nkv, hd)
+    q = (2 * randn(len(lens), nh, hd, seed=3)).bfloat16().view(len(lens), -1).cuda()
+    pages, table = held.pages(), held.table.cuda()
+    got = ops.kv8_attention(q, pages, on_gpu(step(lens, [1] * len(lens))), table, nh, nkv, hd, hd ** -0.5)
+    for s in range(0, 150, 7):
+        want, weight = P.attend(q[s:s + 1].cpu().view(1, nh, hd), held.keys[s], held.values[s], torch.tensor([lens[s] - 1]), hd ** -0.5) if lens[s] else (torch.zeros(1, nh * hd).double(),) * 2
+        if lens[s] == 0:
+            assert (got[s] == 0).all()
+            continue
+        tol = bound(q[s:s + 1].cpu().view(1, nh, hd), held, s, want, weight, None, hd ** -0.5, torch.bfloat16, hd, True)
+        assert ((got[s].cpu().double() - want[0]).abs() <= tol[0]).all(), s
+    again = ops.kv8_attention(q, pages, on_gpu(step(lens, [1] * len(lens))), table, nh, nkv, hd, hd ** -0.5)
+    assert torch.equal(got, again)                                 # (no sum depends on which warp is first)
+
+
+@pytest.mark.parametrize("nh,nkv,hd,dtype", [(32, 8, 128, torch.bfloat16), (8, 1, 64, torch.bfloat16), (24, 2, 128, torch.bfloat16), (4, 2, 96, torch.float32)])
+def test_recorded_and_replayed(nh, nkv, hd, dtype):
+    """A step of preparation and attention recorded once, replayed while the sequences grow, two graphs in turn and on two streams at once."""
+    from synaptix_b200 import ops
+    lens = [130, 700, 64]
+    held = filled([n + 8 for n in lens], nkv, hd)
+    pages, table = held.pages(), held.table.cuda()
+    scale = hd ** -0.5
+
+    class Step:
+        def __init__(self, seed):
+            self.ctx = on_gpu(step(lens, [1] * 3, host=None))
+            self.ctx.max_len = table.shape[1] * 64
+            self.pages = ops.KV8Pages(*(t.clone() for t in pages))
+            self.qkv = torch.zeros(3, (nh + 2 * nkv) * hd, dtype=dtype, device="cuda")
+            self.q = torch.zeros(3, nh * hd, dtype=dtype, device="cuda")
+            self.run()
+            torch.cuda.synchronize()
+            self.graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(self.graph):
+                self.out = self.run()
+            self.rows = [randn(3, (nh + 2 * nkv) * hd, seed=seed + i).to(dtype).cuda() for i in range(4)]
+
+        def run(self):
+            ops.kv8_prepare(self.qkv, self.q, self.pages, None, None, None, 0, 0.0, self.ctx.positions, self.ctx.seq_of_token, table, nh, nkv, hd)
+            return ops.kv8_attention(self.q, self.pages, self.ctx, table, nh, nkv, hd, scale)
+
+        def at(self, i):
+            self.qkv.copy_(self.rows[i])
+            self.ctx.seq_lens.copy_(torch.tensor([n + i for n in lens], dtype=torch.int32))
+            self.ctx.positions.copy_(torch.tensor([n + i - 1 for n in lens], dtype=torch.int32))
+
+    a, b = Step(10), Step(20)
+    want = []
+    for s in (a, b):
+        for i in range(4):
+            s.at(i)
+            want.append(s.run().clone())
+    assert not torch.equal(a.pages.k, b.pages.k)
+    for i in range(4):                                             # in turn
+        for s, w in ((a, want[i]), (b, want[4 + i])):
+            s.at(i)
+            s.graph.replay()
+            assert torch.equal(s.out, w)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in (3, 0, 2):                                            # at once
+        for s in (a, b):
+            s.at(i)
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for s, st in zip((a, b), streams):
+                with torch.cuda.stream(st):
+                    s.graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a.out, want[i]) and torch.equal(b.out, want[4 + i])
+
+
+def test_what_is_not_contiguous_or_aligned():
+    from synaptix_b200 import ops
+    nh, nkv, hd, lens = 8, 2, 64, [200]
+    held = filled(lens, nkv, hd)
+    pages, table, ctx = held.pages(), held.table.cuda(), on_gpu(step(lens, [1]))
+    wide = randn(1, 2 * nh * hd).bfloat16().cuda()
+    with pytest.raises(ops.KernelError, match="contiguous"):
+        ops.kv8_attention(wide[:, ::2], pages, ctx, table, nh, nkv, hd, 0.1)
+    # (a row of a larger tensor that begins anywhere is fine for the heads' preparation, and refused where 16 bytes are loaded at once)
+    odd = wide.view(-1)[1:1 + nh * hd].view(1, -1)
+    with pytest.raises(ops.KernelError, match="misaligned"):
+        ops.kv8_attention(odd, pages, ctx, table, nh, nkv, hd, 0.1)
+    x = randn(70, 1 + (nh + 2 * nkv) * hd).bfloat16()
+    held = empty([70], nkv, hd)
+    q, got = prepare(x, held, torch.arange(70), torch.zeros(70), nh, nkv, hd, col=1)
+    assert torch.equal(q, x[:, 1:1 + nh * hd])
+    kc, _, _ = P.quantise(x[:, 1 + nh * hd:1 + (nh + nkv) * hd].reshape(70, nkv, hd))
+    assert torch.equal(written(got, held, 0, 69, nkv, hd)[0], kc[69])
+
+
 # ---- as a model uses them
 
 def held_rows(engine, slot, layer, n):
