@@ -152,25 +152,27 @@ def kv8_prepare(qkv: torch.Tensor, q_out: Optional[torch.Tensor], pages: Optiona
 
 
 def _read_plan(ctx, width: int, window: Optional[int], chunk: Optional[int], device):
-    """Which pages of which sequence are read, in order, and the table that finds them again, made once a step."""
-    key = ("kv8_read", width, window, chunk)
-    plan = ctx.scratch.get(key)
-    if plan is None:
-        past, lens = ctx.host["seq_past"], ctx.host["seq_lens"]
-        seqs, idx, table = [], [], np.zeros((len(lens), width), dtype=np.int32)
-        for s, (p, n) in enumerate(zip(past, lens)):
-            first = max(0, p - window + 1) if window else 0              # the first key that the step's first token sees
-            if chunk:
-                first = max(first, p // chunk * chunk)
-            a, b = first // PAGE, -(-n // PAGE)
-            at = len(idx)
-            table[s, :b] = at + np.maximum(np.arange(b) - a, 0)
-            seqs += [s] * (b - a)
-            idx += range(a, b)
-        flat = np.concatenate([table.reshape(-1), np.asarray(seqs + idx, dtype=np.int32)])
-        dev = torch.from_numpy(flat).to(device, non_blocking=True)
-        n = len(idx)
-        plan = ctx.scratch[key] = (dev[:table.size].view(table.shape), dev[table.size:table.size + n], dev[table.size + n:], n)
+    """Which pages of which sequence are read, in order, and the table that finds them again, made once a step (and anew where a context is used for
+    other lengths)."""
+    past, lens = ctx.host["seq_past"], ctx.host["seq_lens"]
+    plan = ctx.scratch.get(("kv8_read", width, window, chunk))
+    if plan is not None and plan[4] == past and plan[5] == lens:
+        return plan
+    seqs, idx, table = [], [], np.zeros((len(lens), width), dtype=np.int32)
+    for s, (p, n) in enumerate(zip(past, lens)):
+        first = max(0, p - window + 1) if window else 0                  # the first key that the step's first token sees
+        if chunk:
+            first = max(first, p // chunk * chunk)
+        a, b = first // PAGE, -(-n // PAGE)
+        at = len(idx)
+        table[s, :b] = at + np.maximum(np.arange(b) - a, 0)
+        seqs += [s] * (b - a)
+        idx += range(a, b)
+    flat = np.concatenate([table.reshape(-1), np.asarray(seqs + idx, dtype=np.int32)])
+    dev = torch.from_numpy(flat).to(device, non_blocking=True)
+    n = len(idx)
+    plan = ctx.scratch[("kv8_read", width, window, chunk)] = (dev[:table.size].view(table.shape), dev[table.size:table.size + n],
+                                                              dev[table.size + n:], n, list(past), list(lens))
     return plan
 
 
@@ -192,18 +194,26 @@ def kv8_read(pages: KV8Pages, ctx, block_table: torch.Tensor, dtype: torch.dtype
     ``k``, ``v`` ``[n, kv heads, 64, hd]`` the pages one sequence after the other and ``table`` int32 ``[sequences, pages]`` the page
     of each.  Rows behind a sequence's end are zero.  With ``window`` or ``chunk`` pages that no token of the step sees are left
     out (their place in the table names another page).  Needs the step's lengths on the host."""
-    n_pages, nkv, hd, _ = _check_pages(pages, "kv8_read")
+    _check_pages(pages, "kv8_read")
     _check_host("kv8_read", ctx, block_table)
     if (window is not None and window < 1) or (chunk is not None and chunk < 1):
         raise KernelError("kv8_read: window and chunk are positive")
-    dt = dt_code(dtype)
+    dt_code(dtype)
     _check_device("kv8_read", *pages, ctx.seq_lens, block_table)
-    table, seqs, idx, n = _read_plan(ctx, block_table.shape[1], window, chunk, pages.k.device)
-    k = torch.empty((n, nkv, PAGE, hd), dtype=dtype, device=pages.k.device)
+    return _read(pages, ctx, block_table, dtype, window, chunk)
+
+
+def _read(pages: KV8Pages, ctx, block_table: torch.Tensor, dtype: torch.dtype, window: Optional[int], chunk: Optional[int]):
+    """``kv8_read`` of what has been checked."""
+    k8, v8, ke, ve = pages
+    n_pages, nkv, hd, _ = v8.shape
+    device, width = v8.device, block_table.shape[1]
+    table, seqs, idx, n, _, _ = _read_plan(ctx, width, window, chunk, device)
+    k = torch.empty((n, nkv, PAGE, hd), dtype=dtype, device=device)
     v = torch.empty_like(k)
     check(launcher("kv8", "sx_kv8_read")(
-        *(t.data_ptr() for t in pages), k.data_ptr(), v.data_ptr(), seqs.data_ptr(), idx.data_ptr(), n, ctx.seq_lens.data_ptr(),
-        block_table.data_ptr(), block_table.shape[1], nkv, hd, n_pages, dt, raw_stream()), "kv8_read", launches=1 if n else 0)
+        k8.data_ptr(), v8.data_ptr(), ke.data_ptr(), ve.data_ptr(), k.data_ptr(), v.data_ptr(), seqs.data_ptr(), idx.data_ptr(), n,
+        ctx.seq_lens.data_ptr(), block_table.data_ptr(), width, nkv, hd, n_pages, dt_code(dtype), raw_stream()), "kv8_read", 1 if n else 0)
     return k, v, table
 
 
@@ -328,16 +338,16 @@ def kv8_attention(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tens
     from .attention import attn_prefill_tc_parts, tc_parts
     _check_host("kv8_attention", ctx, block_table)
     _check_device("kv8_attention", q, *pages, ctx.seq_lens, block_table, sinks, out)
-    k, v, table = kv8_read(pages, ctx, block_table, q.dtype, window, chunk)
+    k, v, table = _read(pages, ctx, block_table, q.dtype, window, chunk)
     if out is None and softcap is None and chunk is None and out_scale == 1.0 and tc_prefill_supported(q.dtype, nh, nkv, hd):
+        cu, past = ctx.host["cu_seqlens"], ctx.host["seq_past"]
         cut = ctx.scratch.get(("kv8_parts", nh, window))
-        if cut is None:
-            cu, past = ctx.host["cu_seqlens"], ctx.host["seq_past"]
+        if cut is None or cut[2] != cu or cut[3] != past:
             tiles = [(p + q0, min(p + q0 + TC_TILE_ROWS, p + b - a) - 1) for a, b, p in zip(cu, cu[1:], past) for q0 in range(0, b - a, TC_TILE_ROWS)]
-            cut = ctx.scratch[("kv8_parts", nh, window)] = tc_parts(tiles, nh, window, q.device)
+            cut = ctx.scratch[("kv8_parts", nh, window)] = tc_parts(tiles, nh, window, q.device) + (list(cu), list(past))
         if cut[1] > 1:
             tile_seq, tile_q0 = _query_tiles(ctx, TC_TILE_ROWS, q.device)
             return attn_prefill_tc_parts(q, k, v, tile_seq, tile_q0, ctx.seq_of_token, ctx.cu_seqlens, ctx.seq_past, ctx.seq_lens, table, nh, nkv, hd,
-                                         scale, window, *cut, sinks=sinks)
+                                         scale, window, cut[0], cut[1], sinks=sinks)
     return attention(q, k, v, ctx, table, nh, nkv, hd, scale, window, softcap=softcap, sinks=sinks, chunk=chunk, out=out, out_col=out_col,
                      out_scale=out_scale)
