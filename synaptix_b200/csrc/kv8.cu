@@ -269,22 +269,18 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) kv8_prepare_wide_
   constexpr int HPT = 64 / LPH;                                  // heads at a time
   const int tok = threadIdx.x / 64, t = t0 + tok, e0 = (lane % LPH) * 8, h0 = threadIdx.x % 64 / LPH;
   const bool here = tok < tokens;
-  float cs[8], sn[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    cs[i] = inv_freq && here ? s_cs[tok][e0 + i] : 1.f;
-    sn[i] = inv_freq && here ? s_sn[tok][e0 + i] : 0.f;
-  }
   const int pos = here ? positions[t] : 0, page = here && k_pages ? kv8_page_of(positions, seq_of_token, block_table, maxp, n_pages, t) : -1;
 #pragma unroll 1
   for (int kind = 0; kind < (k_pages ? 2 : 1); ++kind) {
     const float* gain = kind ? wk : wq;
     const int n = kind ? nkv : nh;
-    float ga[8], gb[8];
+    // a' = a f[0] - b f[1], b' = a f[2] + b f[3]: gains and rotation in one
+    float f[4][8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      ga[i] = gain ? gain[e0 + i] : 1.f;
-      gb[i] = gain ? gain[e0 + HALF + i] : 1.f;
+      const float ga = gain ? gain[e0 + i] : 1.f, gb = gain ? gain[e0 + HALF + i] : 1.f;
+      const float cs = inv_freq && here ? s_cs[tok][e0 + i] : 1.f, sn = inv_freq && here ? s_sn[tok][e0 + i] : 0.f;
+      f[0][i] = ga * cs; f[1][i] = gb * sn; f[2][i] = ga * sn; f[3][i] = gb * cs;
     }
     typedef typename Kv8Vec<T>::Raw8 Raw;
     const T* src = qkv + (size_t)t * row + (size_t)kind * nh * HD + e0;
@@ -303,25 +299,27 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) kv8_prepare_wide_
         next_a = *reinterpret_cast<const Raw*>(src + (size_t)(head + HPT) * HD);
         next_b = *reinterpret_cast<const Raw*>(src + (size_t)(head + HPT) * HD + HALF);
       }
+      float inv = 1.f;
       if (gain) {
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
 #pragma unroll
         for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float inv = rsqrtf(ss / (float)HD + eps);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          a[i] *= inv * ga[i];
-          b[i] *= inv * gb[i];
-        }
+        inv = rsqrtf(ss / (float)HD + eps);
       }
       if (inv_freq) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float x = a[i] * cs[i] - b[i] * sn[i], y = a[i] * sn[i] + b[i] * cs[i];
-          a[i] = x;
-          b[i] = y;
+          const float x = a[i] * f[0][i] - b[i] * f[1][i], y = a[i] * f[2][i] + b[i] * f[3][i];
+          a[i] = x * inv;
+          b[i] = y * inv;
+        }
+      } else if (gain) {                                         // (apart: an infinite b times 0 would be NaN in a)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          a[i] *= inv * f[0][i];
+          b[i] *= inv * f[3][i];
         }
       }
       if (kind == 0) {

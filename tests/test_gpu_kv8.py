@@ -465,14 +465,16 @@ def test_what_is_not_contiguous_or_aligned():
 # ---- as a model uses them
 
 def held_rows(engine, slot, layer, n):
-    """Keys and values that the engine's cache holds of a sequence, as the doubles they stand for."""
+    """Keys and values that the engine's cache holds of a sequence, as the doubles they stand for (NaN where a window gave the page back)."""
     view = engine.cache.view(layer)
-    at = torch.tensor(engine.cache.slots.table(slot, view.group)[:-(-n // 64)], device="cuda")
+    table = engine.cache.slots.table(slot, view.group)[:-(-n // 64)]
+    at = torch.tensor([max(p, 0) for p in table], device="cuda")
     k, v, ke, ve = (t[at].cpu() for t in (view.pages8.k, view.pages8.v, view.pages8.k_exp, view.pages8.v_exp))
     power = [torch.exp2(e.double() - 127).transpose(1, 2).reshape(-1, e.shape[1], 1) for e in (ke, ve)]
     k = k.view(torch.float8_e4m3fn).double().permute(0, 3, 1, 2, 4).flatten(3).flatten(0, 1)
     v = v.view(torch.float8_e4m3fn).double().permute(0, 3, 1, 2).flatten(0, 1)
-    return (k * power[0])[:n], (v * power[1])[:n]
+    gone = torch.tensor([p < 0 for p in table]).repeat_interleave(64)[:, None, None]
+    return tuple(torch.where(gone, math.nan, x)[:n] for x in (k * power[0], v * power[1]))
 
 
 def oracle8(name, tokens, held, slack):
@@ -483,7 +485,7 @@ def oracle8(name, tokens, held, slack):
     whole, layer = Q.causal_gqa_attention, iter(range(1000))
 
     def attention(q, k, v, *a, **kw):
-        rows = held[next(layer)]
+        rows = [torch.where(got.isnan(), P.quantise(own)[2], got) for got, own in zip(held[next(layer)], (k, v))]
         for got, own in zip(rows, (k, v)):
             top = own.double().abs().amax(-1, keepdim=True)
             assert ((got - own).abs() <= own.abs() * 2.0 ** -4 + top * (2.0 ** -10 / 224 + slack * (1 + 2.0 ** -4))).all()
@@ -495,7 +497,7 @@ def oracle8(name, tokens, held, slack):
         Q.causal_gqa_attention = whole
 
 
-@pytest.mark.parametrize("name", ["A", "F"])
+@pytest.mark.parametrize("name", ["A", "F", "O", "B", "W", "S", "G"])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("graph", [True, False])
 def test_engine(name, dtype, graph):
@@ -520,6 +522,35 @@ def test_engine(name, dtype, graph):
         assert (full - want).abs().max().item() > 1e-3 * scale      # eight bits show
         off = (torch.cat(rows).cpu() - want).abs().max().item() / scale
         assert off <= rel, (cuts, off)
+
+
+def test_a_decoder_of_other_parts():
+    """The Vemedra decoder (chunks, capped scores and sinks beside retention): where its keys and values have one size its cache may be in eight bits, and
+    a prompt gives the same whole, in portions and token by token; where they have not, the engine says so."""
+    import synaptix_b200
+    import tiny_vemedra as V
+    took = 0
+    for name in V.CONFIGS:
+        try:
+            engine = synaptix_b200.LLM(V.folder(name), compute_dtype="f32", max_tokens=1024, kv_dtype="fp8").engine
+        except ValueError as e:
+            assert "eight bits" in str(e)
+            continue
+        took += 1
+        tokens = random_tokens(engine.model.vocab_size, 150, 5)
+        want = V.oracle_logits(name, tuple(tokens))
+        scale = want.abs().max().item()
+        from synaptix_b200.engine import Entry
+        for cuts in ([150], [70, 80], [140] + [1] * 10):
+            s, at, rows = engine.open(), 0, []
+            for n in cuts:
+                rows.append(engine.step([Entry(s, tokens[at:at + n], list(range(n)))]).clone())
+                at += n
+            engine.close(s)
+            off = (torch.cat(rows).cpu() - want).abs().max().item() / scale
+            # eight bits move an element of a key or value by 2^-4 of itself: half of that on average, mostly lost in sums of many
+            assert 1e-6 < off < 2.0 ** -4, (name, cuts, off)
+    assert took == 1
 
 
 def test_generation_and_conversation():
