@@ -567,81 +567,110 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
   }
 }
 
-// Pairs that several blocks shared: block (b, row) looks at the border between the stretches b and b + 1, and where a pair's first border is
-// that one, joins the pair's row.  Lengths are read while the first kernel still runs: it lets this one in behind its own wait, so what was
-// there before it is there.
+// Pairs that several blocks shared: block b looks at the border between the stretches b and b + 1, and where that lies within a pair, takes its share of
+// the pair's rows, dealt to the blocks at its borders.  With few parts a warp takes a row, with more than four the warps share a row's parts.  Lengths are
+// read and the place is found while the first kernel still runs: it lets this one in behind its own wait, so what was there before it is there.
+// (As a block of 256 threads for every border and row: 29.7 us for 64 sequences seeing 1,000 keys where this takes 27.3, 18.3 for 8 x 4,096 where it takes
+// 17.3.  Fewer registers in the first kernel, so that these blocks wait on its SMs, cost it more than that gave: 18.8 for 8 x 4,096, 56.6 for one of 65,536
+// where 52.8 stand.)
+#define KD_MERGE_WARPS 4
 template <int HD>
-__global__ void __launch_bounds__(256) kv8_decode_merge_kernel(const KdArgs a) {
-  constexpr int TEAMS = 256 / (HD / 2);
-  extern __shared__ int start[];           // (no more than the sequences need: a block of this kernel has to fit beside one of the first)
-  __shared__ int warp_sums[8];
+__global__ void __launch_bounds__(KD_MERGE_WARPS * 32) kv8_decode_merge_kernel(const KdArgs a) {
+  constexpr int DIMS = HD / 32, TEAMS = KD_MERGE_WARPS;         // dims a lane
+  extern __shared__ int start[];
+  __shared__ int warp_sums[TEAMS];
   __shared__ float acc[TEAMS][HD], s_m[TEAMS], s_l[TEAMS];
-  kd_starts<256>(a, start, warp_sums);
-  const int G = a.nh / a.nkv, row = blockIdx.y, n_all = start[a.S] * a.nkv, workers = n_all ? kd_workers(a, n_all) : 0;
-  const int w0 = blockIdx.x;
-  int w1 = w0, seq = 0, kvh = 0;
-  if (w0 + 1 < workers) {
-    const int border = kd_first(w0 + 1, n_all, workers);
+  kd_starts<TEAMS * 32>(a, start, warp_sums);
+  const int G = a.nh / a.nkv, n_all = start[a.S] * a.nkv, workers = n_all ? kd_workers(a, n_all) : 0;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int w0 = 0, k = 0, seq = 0, kvh = 0;                          // the pair's first block, and the borders within the pair
+  if ((int)blockIdx.x + 1 < workers) {
+    const int border = kd_first(blockIdx.x + 1, n_all, workers);
     seq = kd_seq_of(start, a.S, a.nkv, border);
     const int n = start[seq + 1] - start[seq], at = border - start[seq] * a.nkv;
     kvh = at / n;
     const int from = start[seq] * a.nkv + kvh * n;
-    if (from < border && kd_worker_of(from, n_all, workers) == w0) w1 = kd_worker_of(from + n - 1, n_all, workers);
+    if (from < border) {
+      w0 = kd_worker_of(from, n_all, workers);
+      k = kd_worker_of(from + n - 1, n_all, workers) - w0;
+    }
   }
   pdl_wait();
   pdl_trigger();
-  if (w1 == w0) return;
-  const int head = kvh * G + row, team = threadIdx.x / (HD / 2), d = threadIdx.x % (HD / 2) * 2;
-  const float* parts = a.part + ((size_t)a.blocks * a.warps * G + row) * (HD + 2);
-  float top = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
-  // (blocks at work are never more than items, so every one from w0 to w1 has a part)
-  for (int w = w0 + team; w <= w1; w += 4 * TEAMS) {
-    float2 ml[4], v[4];
+  if (k == 0) return;
+  const bool shared = k >= TEAMS;                               // (of the pair, so of the block)
+  const int team = shared ? warp : 0, teams = shared ? TEAMS : 1, rows = shared ? 1 : TEAMS, step = 2 * G * (HD + 2);
+  for (int row0 = ((int)blockIdx.x - w0) * rows; row0 < G; row0 += k * rows) {
+    const int row = shared ? row0 : row0 + warp, head = kvh * G + row;
+    if (row >= G) break;                                        // (never where a row is shared)
+    // (blocks at work are never more than items, so every one from w0 to w0 + k has a part; the first block's is in its second place)
+    const float* parts = a.part + ((size_t)(a.blocks * a.warps + 2 * w0) * G + row) * (HD + 2);
+    const float sink = a.sinks ? a.sinks[head] * KD_LOG2E : -INFINITY;
+    float top = -INFINITY, L = 0.f, x[DIMS] = {};
+    for (int w = team; w <= k; w += 4 * teams) {
+      float2 ml[4], v[4][DIMS / 2];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int i = w + k * TEAMS;
-      ml[k] = make_float2(-INFINITY, 0.f);
-      v[k] = make_float2(0.f, 0.f);
-      if (i <= w1) {
-        const float* src = parts + (size_t)(i * 2 + (i == w0 ? 1 : 0)) * G * (HD + 2);
-        ml[k] = *reinterpret_cast<const float2*>(src);
-        v[k] = *reinterpret_cast<const float2*>(src + 2 + d);
+      for (int j = 0; j < 4; ++j) {
+        const int i = w + j * teams;
+        ml[j] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int d = 0; d < DIMS / 2; ++d) v[j][d] = make_float2(0.f, 0.f);
+        if (i <= k) {
+          const float2* src = reinterpret_cast<const float2*>(parts + (ptrdiff_t)i * step + (i == 0 ? step / 2 : 0));
+          ml[j] = src[0];
+#pragma unroll
+          for (int d = 0; d < DIMS / 2; ++d) v[j][d] = src[1 + d * 32 + lane];
+        }
       }
+      const float next = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), top), base = next == -INFINITY ? 0.f : next;
+      const float f = kd_ex2(top - base);
+      L *= f;
+#pragma unroll
+      for (int d = 0; d < DIMS; ++d) x[d] *= f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float h = kd_ex2(ml[j].x - base);
+        L += ml[j].y * h;
+#pragma unroll
+        for (int d = 0; d < DIMS / 2; ++d) {
+          x[2 * d] += v[j][d].x * h;
+          x[2 * d + 1] += v[j][d].y * h;
+        }
+      }
+      top = next;
     }
-    const float next = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), top), base = next == -INFINITY ? 0.f : next;
-    const float f = kd_ex2(top - base);
-    L *= f; x *= f; y *= f;
+    bf16* dst = a.out + ((size_t)seq * a.nh + head) * HD;
+    if (!shared) {
+      const float all = fmaxf(top, sink), base = all == -INFINITY ? 0.f : all, f = kd_ex2(top - base);
+      L = L * f + kd_ex2(sink - base);
+      const float inv = L == 0.f ? 0.f : f / L;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float h = kd_ex2(ml[k].x - base);
-      L += ml[k].y * h;
-      x += v[k].x * h;
-      y += v[k].y * h;
+      for (int d = 0; d < DIMS / 2; ++d) reinterpret_cast<__nv_bfloat162*>(dst)[d * 32 + lane] = __floats2bfloat162_rn(x[2 * d] * inv, x[2 * d + 1] * inv);
+      continue;
     }
-    top = next;
-  }
-  acc[team][d] = x;
-  acc[team][d + 1] = y;
-  if (d == 0) {
-    s_m[team] = top;
-    s_l[team] = L;
-  }
-  __syncthreads();
-  if (threadIdx.x >= HD) return;
-  const float sink = a.sinks ? a.sinks[head] * KD_LOG2E : -INFINITY;
-  top = sink;
 #pragma unroll
-  for (int i = 0; i < TEAMS; ++i) top = fmaxf(top, s_m[i]);
-  const float base = top == -INFINITY ? 0.f : top;
-  L = kd_ex2(sink - base);
-  float O = 0.f;
+    for (int d = 0; d < DIMS / 2; ++d) reinterpret_cast<float2*>(acc[team])[d * 32 + lane] = make_float2(x[2 * d], x[2 * d + 1]);
+    if (lane == 0) {
+      s_m[team] = top;
+      s_l[team] = L;
+    }
+    __syncthreads();
+    if (threadIdx.x < HD) {
+      float all = sink;
 #pragma unroll
-  for (int i = 0; i < TEAMS; ++i) {
-    const float f = kd_ex2(s_m[i] - base);
-    L += s_l[i] * f;
-    O += acc[i][threadIdx.x] * f;
+      for (int i = 0; i < TEAMS; ++i) all = fmaxf(all, s_m[i]);
+      const float base = all == -INFINITY ? 0.f : all;
+      float den = kd_ex2(sink - base), O = 0.f;
+#pragma unroll
+      for (int i = 0; i < TEAMS; ++i) {
+        const float f = kd_ex2(s_m[i] - base);
+        den += s_l[i] * f;
+        O += acc[i][threadIdx.x] * f;
+      }
+      dst[threadIdx.x] = __float2bfloat16_rn(den == 0.f ? 0.f : O / den);
+    }
+    __syncthreads();
   }
-  a.out[((size_t)seq * a.nh + head) * HD + threadIdx.x] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L);
 }
 
 static int* kd_status() {
@@ -671,7 +700,7 @@ static int kd_launch(KdArgs a, cudaStream_t stream) {
   a.warps = L::WARPS;
   const int rc = sx_launch(kv8_decode_kernel<HD, MORE>, dim3(a.blocks), dim3(L::WARPS * 32), L::FIXED + (a.S + 1) * sizeof(int), stream, a);
   if (rc || a.by_pair || a.blocks == 1) return rc;
-  return sx_launch(kv8_decode_merge_kernel<HD>, dim3(a.blocks - 1, a.nh / a.nkv), dim3(256), (a.S + 1) * sizeof(int), stream, a);
+  return sx_launch(kv8_decode_merge_kernel<HD>, dim3(a.blocks - 1), dim3(KD_MERGE_WARPS * 32), (a.S + 1) * sizeof(int), stream, a);
 }
 
 // a block a pair: pairs no more than SMs, of no more than two pages a warp

@@ -60,7 +60,7 @@ def empty(lens, nkv, hd, fill=0xAB, **kw):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("nh,nkv,hd", [(4, 2, 64), (3, 3, 16), (5, 1, 48), (8, 2, 128), (2, 1, 80), (2, 2, 256), (16, 8, 32), (1, 1, 144), (40, 8, 128)])
+@pytest.mark.parametrize("nh,nkv,hd", [(4, 2, 64), (3, 3, 16), (5, 1, 48), (8, 2, 128), (2, 1, 80), (2, 2, 256), (16, 8, 32), (1, 1, 144), (40, 8, 128), (80, 8, 128), (9, 9, 64)])
 @pytest.mark.parametrize("past,new,col", [([0], [1], 0), ([63, 5, 127], [1, 1, 1], 8), ([60, 0], [9, 70], 0), ([0, 3], [300, 129], 24), ([130], [1], 3)])
 def test_write(dtype, nh, nkv, hd, past, new, col):
     """Without norm and rotation: codes and exponents to the bit, queries unchanged, and not a byte beside them."""
