@@ -52,6 +52,7 @@ LIBRARIES: Dict[str, tuple] = {
     "latent": ("latent.cu", []),
     "kv8": ("kv8.cu", []),
     "kv8_decode": ("kv8_decode.cu", []),
+    "kv8_tile": ("kv8_tile.cu", []),
     "moe": ("moe.cu", []),
     "moe_tc": ("moe_tc.cu", []),
     "decode": ("decode.cu", []),

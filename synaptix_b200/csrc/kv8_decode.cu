@@ -72,23 +72,6 @@ __device__ __forceinline__ void kd_copy(uint32_t dst, const void* src, uint32_t 
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
                ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void kd_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void kd_mma8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ float kd_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t kd_half2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 // first visible page of a sequence and one behind its last
 __device__ __forceinline__ int2 kd_range(const KdArgs& a, int s) {
   const int len = a.seq_lens[s] + a.len_add;
@@ -264,11 +247,11 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       // 2^-15 o is 2^-M times sum 2^(x + E) code; times this it is the sum of 2^(x - m) 2^E code
-      float f = m[r] == -INFINITY || M[r] == -INFINITY ? 0.f : kd_ex2(M[r] - m[r]);
+      float f = m[r] == -INFINITY || M[r] == -INFINITY ? 0.f : kv8_ex2(M[r] - m[r]);
       if (whole) {
         const float sink = a.sinks && row < G ? a.sinks[kvh * G + row] * KD_LOG2E : -INFINITY, top = fmaxf(m[r], sink);
-        const float base = top == -INFINITY ? 0.f : top, shrink = kd_ex2(m[r] - base);
-        sum = sum * shrink + kd_ex2(sink - base);
+        const float base = top == -INFINITY ? 0.f : top, shrink = kv8_ex2(m[r] - base);
+        sum = sum * shrink + kv8_ex2(sink - base);
         f = sum == 0.f ? 0.f : f * shrink / sum;
       } else if (row < G && t == 0) {
         *reinterpret_cast<float2*>(part + row * L::PART) = make_float2(m[r], sum);
@@ -345,10 +328,10 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
           const uint32_t b0_ = h ? w.z : w.x, b1_ = h ? w.w : w.y;
           const int k = 4 * b + 2 * h;
           if (MORE) {
-            kd_mma8(acc, qf[k][0][0], qf[k][0][RP - 1], qf[k + 1][0][0], qf[k + 1][0][RP - 1], b0_, b1_);
-            kd_mma8(rest, qf[k][1][0], qf[k][1][RP - 1], qf[k + 1][1][0], qf[k + 1][1][RP - 1], b0_, b1_);
+            kv8_mma_e4m3(acc, qf[k][0][0], qf[k][0][RP - 1], qf[k + 1][0][0], qf[k + 1][0][RP - 1], b0_, b1_);
+            kv8_mma_e4m3(rest, qf[k][1][0], qf[k][1][RP - 1], qf[k + 1][1][0], qf[k + 1][1][RP - 1], b0_, b1_);
           } else {
-            kd_mma8(acc, qf[k][0][0], qf[k][1][0], qf[k + 1][0][0], qf[k + 1][1][0], b0_, b1_);
+            kv8_mma_e4m3(acc, qf[k][0][0], qf[k][1][0], qf[k + 1][0][0], qf[k + 1][1][0], b0_, b1_);
           }
         }
       }
@@ -394,10 +377,10 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
       top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
       top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
       const float base = top[r] == -INFINITY ? 0.f : top[r];
-      float sum = l[r] * kd_ex2(m[r] - base);
+      float sum = l[r] * kv8_ex2(m[r] - base);
       m[r] = top[r];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum += kd_ex2(s[j][2 * r] - base) + kd_ex2(s[j][2 * r + 1] - base);
+      for (int j = 0; j < 8; ++j) sum += kv8_ex2(s[j][2 * r] - base) + kv8_ex2(s[j][2 * r + 1] - base);
       l[r] = sum;
     }
     // ---- weights with the values' powers of two, p v
@@ -448,7 +431,7 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
       for (int r = 0; r < RP; ++r) {
-        const float2 shrink = of_heads(Top[r] == -INFINITY ? 1.f : kd_ex2(M[r] - Top[r]));
+        const float2 shrink = of_heads(Top[r] == -INFINITY ? 1.f : kv8_ex2(M[r] - Top[r]));
         M[r] = Top[r];
 #pragma unroll
         for (int d2 = 0; d2 < HD / 16; ++d2) {
@@ -462,7 +445,7 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
     for (int r = 0; r < RP; ++r) {
       const float base = M[r] == -INFINITY ? 0.f : M[r] - 15.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[j][r] = kd_half2(kd_ex2(s[j][2 * r] - base), kd_ex2(s[j][2 * r + 1] - base));
+      for (int j = 0; j < 8; ++j) p[j][r] = kv8_pack2(kv8_ex2(s[j][2 * r] - base), kv8_ex2(s[j][2 * r + 1] - base));
     }
 #pragma unroll
     for (int d2 = 0; d2 < HD / 16; ++d2) {
@@ -475,7 +458,7 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
         kv8_half4(u0[k], a0, a2);
         kv8_half4(u1[k], a1, a3);
 #pragma unroll
-        for (int r = 0; r < RP; ++r) kd_mma(o[d2][r], a0, a1, a2, a3, p[2 * k][r], p[2 * k + 1][r]);
+        for (int r = 0; r < RP; ++r) kv8_mma_f16(o[d2][r], a0, a1, a2, a3, p[2 * k][r], p[2 * k + 1][r]);
       }
     }
     __syncwarp();
@@ -538,8 +521,8 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
       const float2 ml = has ? *reinterpret_cast<const float2*>(part_of(lane, u == lu) + row * L::PART) : make_float2(-INFINITY, 0.f);
       const float sink = final && a.sinks ? a.sinks[head] * KD_LOG2E : -INFINITY;
       const float top = fmaxf(warp_max(ml.x), sink), base = top == -INFINITY ? 0.f : top;
-      float w = kd_ex2(ml.x - base);
-      const float sum = warp_sum(ml.y * w) + kd_ex2(sink - base);
+      float w = kv8_ex2(ml.x - base);
+      const float sum = warp_sum(ml.y * w) + kv8_ex2(sink - base);
       if (final) w = sum == 0.f ? 0.f : __fdividef(w, sum);
       float2 x[HD / 64];
 #pragma unroll
@@ -623,13 +606,13 @@ __global__ void __launch_bounds__(KD_MERGE_WARPS * 32) kv8_decode_merge_kernel(c
         }
       }
       const float next = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), top), base = next == -INFINITY ? 0.f : next;
-      const float f = kd_ex2(top - base);
+      const float f = kv8_ex2(top - base);
       L *= f;
 #pragma unroll
       for (int d = 0; d < DIMS; ++d) x[d] *= f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float h = kd_ex2(ml[j].x - base);
+        const float h = kv8_ex2(ml[j].x - base);
         L += ml[j].y * h;
 #pragma unroll
         for (int d = 0; d < DIMS / 2; ++d) {
@@ -641,8 +624,8 @@ __global__ void __launch_bounds__(KD_MERGE_WARPS * 32) kv8_decode_merge_kernel(c
     }
     bf16* dst = a.out + ((size_t)seq * a.nh + head) * HD;
     if (!shared) {
-      const float all = fmaxf(top, sink), base = all == -INFINITY ? 0.f : all, f = kd_ex2(top - base);
-      L = L * f + kd_ex2(sink - base);
+      const float all = fmaxf(top, sink), base = all == -INFINITY ? 0.f : all, f = kv8_ex2(top - base);
+      L = L * f + kv8_ex2(sink - base);
       const float inv = L == 0.f ? 0.f : f / L;
 #pragma unroll
       for (int d = 0; d < DIMS / 2; ++d) reinterpret_cast<__nv_bfloat162*>(dst)[d * 32 + lane] = __floats2bfloat162_rn(x[2 * d] * inv, x[2 * d + 1] * inv);
@@ -660,10 +643,10 @@ __global__ void __launch_bounds__(KD_MERGE_WARPS * 32) kv8_decode_merge_kernel(c
 #pragma unroll
       for (int i = 0; i < TEAMS; ++i) all = fmaxf(all, s_m[i]);
       const float base = all == -INFINITY ? 0.f : all;
-      float den = kd_ex2(sink - base), O = 0.f;
+      float den = kv8_ex2(sink - base), O = 0.f;
 #pragma unroll
       for (int i = 0; i < TEAMS; ++i) {
-        const float f = kd_ex2(s_m[i] - base);
+        const float f = kv8_ex2(s_m[i] - base);
         den += s_l[i] * f;
         O += acc[i][threadIdx.x] * f;
       }

@@ -294,6 +294,50 @@ def kv8_decode_status(reset: bool = False) -> int:
     return int(v.value)
 
 
+TILE_HEAD_DIMS = (64, 128)
+TILE_ROWS = 64                  # query heads of a kv head x tokens that a block of csrc/kv8_tile.cu serves
+# float32 portions of any length attend over the codes: us, 32 heads over 8 of 128, reading back (with FFMA products) and so: 150 tokens of two
+# sequences 57 and 17.5, 64 over 6,000 keys 447 and 52, a prompt of 1,500 638 and 160.  bfloat16 ones of up to one tile of rows a kv head at head size 128
+# (16 tokens of 4 heads a kv head over 2,000 keys 17.9 and 16.5, over 20,000 91 and 48, of 32 sequences with 3,000 260 and 156), two at head size 64 (32
+# tokens of 4 heads 44 and 13, 374 and 47, 159 and 147); with more the tcgen05 products are worth the pages' way through memory (5 x 32 over 9,000
+# at head size 128 135 and 164, 5 x 64 at 64 229 and 252).
+TILE_BF16_ROWS = {128: 64, 64: 128}
+
+
+def kv8_tile_supported(q: torch.Tensor, nh: int, nkv: int, hd: int, S: int) -> bool:
+    """Whether portions of these sizes attend over the codes (``csrc/kv8_tile.cu``)."""
+    return hd in TILE_HEAD_DIMS and nh // nkv <= TILE_ROWS and q.shape[0] > 0 and S <= 65535 and q.data_ptr() % 16 == 0
+
+
+def _tile_splits(S: int, max_new: int, nh: int, nkv: int, max_pages: int, device) -> int:
+    """Shares of a tile's pages: as many as fit the GPU at once (two blocks an SM), of four pages or more."""
+    blocks = S * nkv * -(-max_new // (TILE_ROWS // (nh // nkv)))
+    return max(1, min(-(-max_pages // 4), 2 * sm_count(device) // blocks))
+
+
+def kv8_tile(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tensor, nh: int, scale: float, window: Optional[int], *,
+             softcap: Optional[float] = None, sinks: Optional[torch.Tensor] = None, chunk: Optional[int] = None,
+             out: Optional[torch.Tensor] = None, out_col: int = 0, out_scale: float = 1.0) -> torch.Tensor:
+    """Packed queries of portions over the codes; sizes as ``kv8_tile_supported`` says."""
+    k, v, ke, ve = pages
+    n_pages, nkv, hd, _ = v.shape
+    T, S, maxp = q.shape[0], ctx.n_seqs, block_table.shape[1]
+    max_pages = min(-(-ctx.max_len // PAGE), maxp)
+    if window is not None:
+        max_pages = min(max_pages, (window + TILE_ROWS + 125) // PAGE)
+    splits = _tile_splits(S, ctx.max_new, nh, nkv, max_pages, q.device)
+    if out is None:
+        out = torch.empty_like(q)
+    part = torch.empty(T * nh * splits * (hd + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+    part_o = _ptr(part)
+    check(launcher("kv8_tile", "sx_kv8_tile")(
+        q.data_ptr(), out.data_ptr() + out_col * out.element_size(), k.data_ptr(), v.data_ptr(), ke.data_ptr(), ve.data_ptr(),
+        ctx.cu_seqlens.data_ptr(), ctx.seq_past.data_ptr(), block_table.data_ptr(), maxp, S, T, ctx.max_new, nh, nkv, hd, n_pages, scale, window or 0,
+        softcap or 0.0, _ptr(sinks), chunk or 0, out.shape[1], out_scale, splits, part_o, part_o + 4 * T * nh * splits * hd if part_o else 0,
+        dt_code(q.dtype), raw_stream()), "kv8_attention", 2 if splits > 1 else 1)
+    return out
+
+
 def kv8_attention(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tensor, nh: int, nkv: int, hd: int, scale: float,
                   window: Optional[int] = None, *, softcap: Optional[float] = None, sinks: Optional[torch.Tensor] = None,
                   chunk: Optional[int] = None, out: Optional[torch.Tensor] = None, out_col: int = 0,
@@ -301,9 +345,9 @@ def kv8_attention(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tens
     """Causal attention of the step's packed queries ``q [T, nh * hd]`` over a cache in eight bits that already holds the step's
     keys and values: ``[T, nh * hd]`` in ``q``'s dtype.  The options are those of ``ops.attention``.
 
-    Single tokens attend over the codes.  Portions of prompts read the pages back once (``kv8_read``) and attend over the result
-    with the kernels of the 16- and 32-bit cache: a page serves many rows there, and turning its codes again in every block that
-    reads it would cost more than writing it out once."""
+    Single tokens, portions of a few tokens and float32 portions attend over the codes.  Longer portions read the pages back once
+    (``kv8_read``) and attend over the result with the kernels of the 16- and 32-bit cache: a page serves many rows there, and
+    turning its codes again in every block that reads it would cost more than writing it out once."""
     _check_pages(pages, "kv8_attention", nkv, hd)
     seq_lens = ctx.seq_lens
     if seq_lens.dtype is not torch.int32 or block_table.dtype is not torch.int32:
@@ -334,9 +378,18 @@ def kv8_attention(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tens
             raise KernelError("kv8_attention: a position and a sequence per token (int32), and a table [sequences, pages]")
         _check_device("kv8_attention", q, *pages, ctx.positions, ctx.seq_of_token, block_table, sinks)
         return kv8_decode(q, pages, ctx.positions, block_table, nh, scale, window, ctx.max_len, sinks, ctx.seq_of_token)
+    _check_host("kv8_attention", ctx, block_table)
+    if kv8_tile_supported(q, nh, nkv, hd, ctx.n_seqs) and (q.dtype == torch.float32 or ctx.max_new * (nh // nkv) <= TILE_BF16_ROWS[hd]):
+        S = ctx.n_seqs
+        if not (ctx.cu_seqlens.dtype == ctx.seq_past.dtype == torch.int32) or ctx.cu_seqlens.numel() <= S or ctx.seq_past.numel() < S:
+            raise KernelError("kv8_attention: a first token and a length before the step per sequence (int32)")
+        if ctx.host["cu_seqlens"][S] > q.shape[0]:
+            raise KernelError("kv8_attention: fewer rows of queries than the step has tokens")
+        _check_device("kv8_attention", q, *pages, ctx.cu_seqlens, ctx.seq_past, block_table, sinks, out)
+        return kv8_tile(q, pages, ctx, block_table, nh, scale, window, softcap=softcap, sinks=sinks, chunk=chunk, out=out, out_col=out_col,
+                        out_scale=out_scale)
     from . import TC_TILE_ROWS, _query_tiles, attention, tc_prefill_supported
     from .attention import attn_prefill_tc_parts, tc_parts
-    _check_host("kv8_attention", ctx, block_table)
     _check_device("kv8_attention", q, *pages, ctx.seq_lens, block_table, sinks, out)
     k, v, table = _read(pages, ctx, block_table, q.dtype, window, chunk)
     if out is None and softcap is None and chunk is None and out_scale == 1.0 and tc_prefill_supported(q.dtype, nh, nkv, hd):

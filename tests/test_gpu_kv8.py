@@ -363,6 +363,88 @@ def test_a_few_tokens(new, nh, nkv, hd, options):
     check(2 * randn(sum(new), nh, hd, seed=3), filled(lens, nkv, hd), lens, new, nh, hd, torch.bfloat16, True, **options)
 
 
+@pytest.fixture
+def over_the_codes(monkeypatch):
+    """All portions attend over the codes, whatever is faster."""
+    from synaptix_b200.ops import kv8
+    calls, tile = [], kv8.kv8_tile
+    monkeypatch.setattr(kv8, "FEW_NEW_TOKENS", 0)
+    monkeypatch.setattr(kv8, "TILE_BF16_ROWS", {64: 1 << 30, 128: 1 << 30})
+    monkeypatch.setattr(kv8, "kv8_tile", lambda *a, **kw: calls.append(1) or tile(*a, **kw))
+    yield
+    assert calls
+
+
+# Bounds of portions over the codes.  bfloat16: those of single tokens (queries as two codes, weights as halves).  float32: queries and weights are two
+# halves, off by 2^-22 of themselves; products are summed in chains of four instructions, each of which may drop 2^-22 of the sum so far, and chains by
+# plain additions: a score is off by less than (4 + 2) 2^-22 + 8 2^-24, under (hd + 8) 2^-24, of its spread, the sum over keys by (2 + 4) 2^-22 + (n / 64 + 64) 2^-24.
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (32, 8, 128), (64, 1, 128), (7, 1, 64), (24, 2, 128), (3, 3, 128)])
+@pytest.mark.parametrize("lens,new", [([1], [1]), ([2, 65], [2, 1]), ([5000], [3]), ([64, 300, 1, 131], [2, 33, 1, 131]), ([2000, 64, 70], [150, 64, 0])])
+@pytest.mark.parametrize("options", [{}, dict(window=1), dict(window=70, sinks=True), dict(softcap=4.0, chunk=96)])
+def test_portions_over_the_codes(over_the_codes, dtype, nh, nkv, hd, lens, new, options):
+    options = dict(options, sinks=randn(nh, seed=9) * 3) if options.get("sinks") else options
+    held, ctx = filled(lens, nkv, hd, seed=nh), step(lens, new)
+    ctx.all_single = False
+    q = (2 * randn(sum(new), nh, hd, seed=3)).to(dtype)
+    pages, table = held.pages(), held.table.cuda()
+    from synaptix_b200 import ops
+    kw = {k: (v.cuda() if isinstance(v, torch.Tensor) else v) for k, v in options.items()}
+    got, again = (ops.kv8_attention(q.view(q.shape[0], -1).cuda(), pages, on_gpu(ctx), table, nh, nkv, hd, hd ** -0.5, **kw).cpu() for _ in range(2))
+    assert torch.equal(got, again)
+    at = 0
+    for s, (n, m) in enumerate(zip(lens, new)):
+        part = slice(at, at + m)
+        at += m
+        if m:
+            pos = torch.arange(n - m, n)
+            want, weight = P.attend(q[part], held.keys[s], held.values[s], pos, hd ** -0.5, **options)
+            tol = bound(q[part], held, s, want, weight, pos, hd ** -0.5, dtype, hd, dtype == torch.bfloat16, options.get("softcap"))
+            assert ((got[part].double() - want).abs() <= tol).all(), (s, ((got[part].double() - want).abs() / tol).max().item())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("past", [0, 3000])
+@pytest.mark.parametrize("window", [None, 50])
+def test_portions_with_rows_that_are_not_finite(over_the_codes, dtype, past, window):
+    """A key or value that was not finite shows in the tokens of a portion that see it, and leaves the others' results as they are without it."""
+    from synaptix_b200 import ops
+    hd, nh, new = 128, 4, 150
+    ks, vs = ([randn(past + new, 2, hd, seed=i + 7 * w) for i in range(3)] for w in (1, 2))
+    q = randn(3 * new, nh, hd).to(dtype)
+    res = []
+    for spoil in (False, True):
+        if spoil:
+            ks[0][past + 40, 0, 3], vs[1][past + 70, 1, 5] = math.inf, math.nan
+            q = q.clone()
+            q[2 * new + 9, 2, 1] = math.inf
+        held = P.Held(ks, vs)
+        ctx = step([past + new] * 3, [new] * 3)
+        res.append(ops.kv8_attention(q.view(3 * new, -1).cuda(), held.pages(), on_gpu(ctx), held.table.cuda(), nh, 2, hd, 0.1, window).cpu().view(3, new, nh, hd))
+    until = new if window is None else window
+    bad = torch.zeros(3, new, nh, dtype=torch.bool)
+    bad[0, 40:40 + until, :2] = bad[1, 70:70 + until, 2:] = bad[2, 9, 2] = True
+    assert torch.equal(res[1].isnan().any(-1), bad) and torch.equal(res[1].isnan().all(-1), bad)
+    assert torch.equal(res[0][~bad], res[1][~bad]) and not res[0].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scale_k,scale_v,scale_q", [(1e-20, 1e20, 1e18), (1e15, 1e-30, 1e-16), (1e-8, 1e-8, 1.0)])
+def test_portions_of_magnitudes_far_from_one(over_the_codes, dtype, scale_k, scale_v, scale_q):
+    lens, new, nh, hd = [300, 70], [40, 70], 8, 128
+    ks, vs = ([randn(n, 2, hd, seed=i + 7 * w) * f for i, n in enumerate(lens)] for w, f in ((1, scale_k), (2, scale_v)))
+    check(randn(110, nh, hd) * scale_q, P.Held(ks, vs), lens, new, nh, hd, dtype, dtype == torch.bfloat16, scale=hd ** -0.5 / (scale_k * scale_q))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_portions_where_one_value_outweighs_all_others(over_the_codes, dtype):
+    nh, hd = 4, 64
+    ks, vs = randn(260, 1, hd, seed=1), randn(260, 1, hd, seed=2)
+    ks[77] = -6.0                                                  # score -48 below zero: weight 1e-21
+    vs[77] *= 2.0 ** 40
+    check(torch.ones(120, nh, hd), P.Held([ks], [vs]), [260], [120], nh, hd, dtype, dtype == torch.bfloat16, scale=1 / 8)
+
+
 def test_many_sequences_and_places_that_end_anywhere():
     """More pairs than blocks, pairs that end within a warp's stretch, empty sequences between: all rows of a batch against the same rows alone."""
     from synaptix_b200 import ops

@@ -122,7 +122,9 @@ def test_attention_refuses(new):
            dict(out=torch.zeros(new + 1, 4 * 64)), dict(out=torch.zeros(new, 4 * 64), out_col=8), dict(out=torch.zeros(new, 8 * 64)[:, ::2]),
            dict(block_table=torch.zeros((1, 2))), dict(block_table=torch.zeros((0, 2), dtype=torch.int32))]
     if new > 1:
-        bad.append(dict(ctx=step([70], [new], host=None)))
+        bad += [dict(ctx=step([70], [new], host=None)), dict(ctx=step([70], [new], cu_seqlens=torch.tensor([0.0, 5.0]))),
+                dict(ctx=step([70], [new], seq_past=torch.tensor([65]))), dict(ctx=step([70], [new], cu_seqlens=torch.zeros(1, dtype=torch.int32))),
+                dict(ctx=step([70], [new + 1])), dict(ctx=step([129], [new]))]
     for change in bad:
         with pytest.raises(KernelError):
             ops.kv8_attention(**{**ok, **change})
