@@ -10,6 +10,7 @@
 //   k heads: the same, then quantised into the sequence's page;   v heads: quantised.
 // The rotation's angle is position * inv_freq in about 48 bits: the product rounded to 32 bits and what that left out, by which
 // sine and cosine are moved on.  (In 32 bits alone an angle at position 100,000 is off by up to 0.004.)
+// One token of 48 heads of 128 3.7 us, 48 tokens 4.8: a launch, the page's number from the table, a row, its sums.
 // ---------------------------------------------------------------------------------------
 #define KV8_WARPS 8
 // cosine and sine of pos * f: the angle is hi + lo with |lo| <= 2^-24 |hi|, up to 2^-8 at position 131,072, so the series in lo needs its
@@ -103,6 +104,8 @@ __global__ void __launch_bounds__(KV8_WARPS * 32) kv8_prepare_kernel(
 // all: 338 us for 8,191 tokens of 48 heads of 128, where bytes take 28.6).  There a thread has two dims of up to 16 tokens that share 16
 // neighbouring places of a page, finds the rows' largest magnitudes with its warp by 31 exchanges for all 16 tokens, and stores 16 bytes a dim.
 // (One kernel: 16 rows of values one behind the other are mostly waiting, 23 us alone.)
+// 8,191 tokens of 48 heads of 128 in bfloat16: 48 us, 3.8 TB/s.  It issues two instructions a clock and SM (80 registers, three blocks an SM): what
+// bounds it is the arithmetic of a row (norm, rotation, quantising: some 16 instructions an element) as much as its loads' latency, which the few warps do not hide.
 template <typename T> struct Kv8Vec;
 template <> struct Kv8Vec<bf16> {
   typedef uint4 Raw8;                                            // 8 and 2 elements as they lie in memory
@@ -395,6 +398,7 @@ extern "C" int sx_kv8_prepare(const void* qkv, void* q_out, void* k_pages, void*
 // behind the sequence's end as zeros.  A block a (page, kv head), bound by its bytes.  A lane of keys takes 8 codes of a
 // row at a time (16 bytes of bfloat16); a lane of values takes 8 dims of 4 keys, one word a dim, turns the bytes around in registers and
 // stores 16 bytes a key: 8 lanes beside one another read 32 bytes of a dim, 4 write 64 of a key.
+// Eight sequences of 4,969 to 12,000 tokens, 8 heads of 128, to bfloat16: 70 to 73 us for 411 MB moved, 5.6 to 5.8 TB/s: HBM, nine tenths of a plain copy's rate.
 // ---------------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ void kv8_store8(T* dst, const uint32_t (&pairs)[4], float f, bool held) {
   float x[8];

@@ -4,7 +4,7 @@
 // the row's largest magnitude, a = m 2^x and 1 <= m < 2, e - 127 is x - 8 where m <= 1.75 and x - 7 above (448 = 1.75 2^8 is
 // the largest e4m3 number), kept in -117 .. 119; codes are rounded to nearest even and saturate.  e = 255: the row was not
 // finite and reads as NaN; its codes are e4m3's NaN (0x7f) too, so a kernel may look at either.  A scale that is a power of two takes nothing from a floating format: all
-// magnitudes within 2^15 of the row's largest keep their three bits of mantissa, as with any other scale, and in return x / scale and
+// magnitudes within 2^13 of the row's largest keep their three bits of mantissa, as with any other scale, and in return x / scale and
 // code * scale are exact in bfloat16, float16 (within its range) and float32.  So writing rounds once, whatever
 // else a kernel does in which order, and reading back rounds never.
 //

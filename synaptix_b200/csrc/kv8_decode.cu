@@ -22,6 +22,11 @@
 //     the denominator, and 2^(x + E - M + 15) in half precision beside the codes, with M the running maximum of x + E.  So a large value
 //     of next to no weight takes nothing from the precision of the others; weights from 1 down to 2^-29 of the row's largest x + E keep all 11 bits.
 //
+// Measured (replayed graphs, other inputs each time; 32 heads over 8 of 128 unless said): one sequence of 131,072 keys 53 us, 5.1 TB/s; 8 x 4,096 keys 17.2;
+// one of 301 keys 7.8; 64 sequences seeing 1,000 keys, 64 heads over 8 of 64, 27.2.  With parts left out in a copy, us of these four: copies alone 41.8, 10.5, 3.9, 15.3;
+// without the products and the softmax 45.9, 15.6, 5.1, 24.3.  So a long line of pages is bound by HBM, a short one by its start (lengths, places, the first
+// pages: 3 us, cold code), the joins (1 to 1.5 us in the block, 1.5 to 3 of the second kernel) and what a warp does once a pair (its query's two parts, its end).
+//
 // Every wait on an mbarrier is bounded; one that runs out sets the library's status word (sx_kv8_decode_status).
 #include "kv8.cuh"
 
