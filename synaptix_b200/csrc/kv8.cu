@@ -398,6 +398,8 @@ extern "C" int sx_kv8_prepare(const void* qkv, void* q_out, void* k_pages, void*
 // behind the sequence's end as zeros.  A block a (page, kv head), bound by its bytes.  A lane of keys takes 8 codes of a
 // row at a time (16 bytes of bfloat16); a lane of values takes 8 dims of 4 keys, one word a dim, turns the bytes around in registers and
 // stores 16 bytes a key: 8 lanes beside one another read 32 bytes of a dim, 4 write 64 of a key.
+// for_attention: a value row that is not finite comes back as zeros and its key row as NaN instead.  Kernels that multiply a page's values with weights of
+// several tokens then give NaN to the tokens that see the row, by their scores, and to no others (a weight of zero times NaN would).
 // Eight sequences of 4,969 to 12,000 tokens, 8 heads of 128, to bfloat16: 70 to 73 us for 411 MB moved, 5.6 to 5.8 TB/s: HBM, nine tenths of a plain copy's rate.
 // ---------------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ void kv8_store8(T* dst, const uint32_t (&pairs)[4], float f, bool held) {
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(
     const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages, const uint8_t* __restrict__ k_exp,
     const uint8_t* __restrict__ v_exp, T* __restrict__ k_out, T* __restrict__ v_out, const int* __restrict__ page_seq,
     const int* __restrict__ page_idx, const int* __restrict__ seq_lens, const int* __restrict__ block_table, int maxp, int nkv, int hd_,
-    int n_pages) {
+    int n_pages, int for_attention) {
   __shared__ float s_k[SX_PAGE], s_v[SX_PAGE];
   pdl_wait();
   pdl_trigger();
@@ -448,8 +450,12 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(
         for (int d = 0; d < 8; ++d) vw[n][d] = *reinterpret_cast<const uint32_t*>(v + kv8_v_at(v_key(o), v_group(o) * 8 + d));
     }
   }
-  if (threadIdx.x < SX_PAGE) s_k[threadIdx.x] = kv8_scale(k_exp[from * SX_PAGE + threadIdx.x]);
-  else if (threadIdx.x < 2 * SX_PAGE) s_v[threadIdx.x - SX_PAGE] = kv8_scale(v_exp[from * SX_PAGE + threadIdx.x - SX_PAGE]);
+  if (threadIdx.x < 2 * SX_PAGE) {
+    const int key = threadIdx.x & (SX_PAGE - 1), ve = v_exp[from * SX_PAGE + key];
+    const bool gone = for_attention && ve == KV8_NAN;
+    if (threadIdx.x < SX_PAGE) s_k[key] = kv8_scale(gone ? KV8_NAN : k_exp[from * SX_PAGE + key]);
+    else s_v[key] = gone ? 0.f : kv8_scale(ve);
+  }
   __syncthreads();
   auto put_k = [&](int o, const uint2 w) {
     const int key = o / groups, d = o % groups * 8;
@@ -463,7 +469,7 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(
       uint32_t pairs[4];
 #pragma unroll
       for (int d = 0; d < 4; ++d) pairs[d] = __byte_perm(w[2 * d], w[2 * d + 1], n | (4 + n) << 4);
-      kv8_store8<T>(v_out + to + (key + n) * hd + group * 8, pairs, s_v[key + n], key + n < held);
+      kv8_store8<T>(v_out + to + (key + n) * hd + group * 8, pairs, s_v[key + n], key + n < held && s_v[key + n] != 0.f);
     }
   };
   if constexpr (HD != 0) {
@@ -486,14 +492,14 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(
 
 extern "C" int sx_kv8_read(const void* k_pages, const void* v_pages, const void* k_exp, const void* v_exp, void* k_out, void* v_out,
                            const int* page_seq, const int* page_idx, int n_out, const int* seq_lens, const int* block_table, int maxp,
-                           int nkv, int hd, int n_pages, int dt, cudaStream_t stream) {
+                           int nkv, int hd, int n_pages, int for_attention, int dt, cudaStream_t stream) {
   if (n_out <= 0) return 0;
   if (hd <= 0 || hd % 16 || hd > KV8_MAX_HD || nkv <= 0 || nkv > 65535) return SX_ERR_SIZE;
   if (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) return SX_ERR_ALIGN;
   const dim3 grid(n_out, nkv);
 #define KV8_READ(T, HD)                                                                                                                            \
   sx_launch(kv8_read_kernel<T, HD>, grid, dim3(256), 0, stream, (const uint8_t*)k_pages, (const uint8_t*)v_pages, (const uint8_t*)k_exp,             \
-            (const uint8_t*)v_exp, (T*)k_out, (T*)v_out, page_seq, page_idx, seq_lens, block_table, maxp, nkv, hd, n_pages)
+            (const uint8_t*)v_exp, (T*)k_out, (T*)v_out, page_seq, page_idx, seq_lens, block_table, maxp, nkv, hd, n_pages, for_attention)
   if (dt == SX_F32) return hd == 64 ? KV8_READ(float, 64) : hd == 128 ? KV8_READ(float, 128) : KV8_READ(float, 0);
   if (dt == SX_BF16) return hd == 64 ? KV8_READ(bf16, 64) : hd == 128 ? KV8_READ(bf16, 128) : KV8_READ(bf16, 0);
   return SX_ERR_DTYPE;

@@ -200,11 +200,11 @@ def kv8_read(pages: KV8Pages, ctx, block_table: torch.Tensor, dtype: torch.dtype
         raise KernelError("kv8_read: window and chunk are positive")
     dt_code(dtype)
     _check_device("kv8_read", *pages, ctx.seq_lens, block_table)
-    return _read(pages, ctx, block_table, dtype, window, chunk)
+    return _read(pages, ctx, block_table, dtype, window, chunk, False)
 
 
-def _read(pages: KV8Pages, ctx, block_table: torch.Tensor, dtype: torch.dtype, window: Optional[int], chunk: Optional[int]):
-    """``kv8_read`` of what has been checked."""
+def _read(pages: KV8Pages, ctx, block_table: torch.Tensor, dtype: torch.dtype, window: Optional[int], chunk: Optional[int], for_attention: bool):
+    """``kv8_read`` of what has been checked.  ``for_attention``: value rows that are not finite are zeros, and their keys NaN."""
     k8, v8, ke, ve = pages
     n_pages, nkv, hd, _ = v8.shape
     device, width = v8.device, block_table.shape[1]
@@ -213,7 +213,7 @@ def _read(pages: KV8Pages, ctx, block_table: torch.Tensor, dtype: torch.dtype, w
     v = torch.empty_like(k)
     check(launcher("kv8", "sx_kv8_read")(
         k8.data_ptr(), v8.data_ptr(), ke.data_ptr(), ve.data_ptr(), k.data_ptr(), v.data_ptr(), seqs.data_ptr(), idx.data_ptr(), n,
-        ctx.seq_lens.data_ptr(), block_table.data_ptr(), width, nkv, hd, n_pages, dt_code(dtype), raw_stream()), "kv8_read", 1 if n else 0)
+        ctx.seq_lens.data_ptr(), block_table.data_ptr(), width, nkv, hd, n_pages, for_attention, dt_code(dtype), raw_stream()), "kv8_read", 1 if n else 0)
     return k, v, table
 
 
@@ -391,7 +391,7 @@ def kv8_attention(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tens
     from . import TC_TILE_ROWS, _query_tiles, attention, tc_prefill_supported
     from .attention import attn_prefill_tc_parts, tc_parts
     _check_device("kv8_attention", q, *pages, ctx.seq_lens, block_table, sinks, out)
-    k, v, table = _read(pages, ctx, block_table, q.dtype, window, chunk)
+    k, v, table = _read(pages, ctx, block_table, q.dtype, window, chunk, True)
     if out is None and softcap is None and chunk is None and out_scale == 1.0 and tc_prefill_supported(q.dtype, nh, nkv, hd):
         cu, past = ctx.host["cu_seqlens"], ctx.host["seq_past"]
         cut = ctx.scratch.get(("kv8_parts", nh, window))

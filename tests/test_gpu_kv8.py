@@ -428,6 +428,24 @@ def test_portions_with_rows_that_are_not_finite(over_the_codes, dtype, past, win
     assert torch.equal(res[0][~bad], res[1][~bad]) and not res[0].isnan().any()
 
 
+@pytest.mark.parametrize("dtype,nh,nkv,hd,past", [(torch.bfloat16, 4, 2, 128, 0), (torch.bfloat16, 32, 2, 128, 3000), (torch.bfloat16, 4, 2, 128, 9000), (torch.bfloat16, 4, 2, 64, 70),
+                                                  (torch.bfloat16, 4, 2, 32, 70), (torch.bfloat16, 4, 2, 96, 70), (torch.float32, 4, 2, 80, 70), (torch.float32, 4, 2, 32, 70)])
+@pytest.mark.parametrize("window", [None, 50])
+def test_portions_read_back_with_rows_that_are_not_finite(dtype, nh, nkv, hd, past, window):
+    """The same where pages are read back: a row that is not finite shows in the tokens that see it and in no others."""
+    from synaptix_b200 import ops
+    new, G = 150, nh // nkv
+    ks, vs = ([randn(past + new, nkv, hd, seed=i + 7 * w) for i in range(2)] for w in (1, 2))
+    ks[0][past + 40, 0, 3], vs[1][past + 70, 1, 5] = math.inf, math.nan
+    held = P.Held(ks, vs)
+    got = ops.kv8_attention(randn(2 * new, nh * hd).to(dtype).cuda(), held.pages(), on_gpu(step([past + new] * 2, [new] * 2)), held.table.cuda(), nh, nkv, hd, 0.1, window)
+    got = got.cpu().view(2, new, nh, hd)
+    until = new if window is None else window
+    bad = torch.zeros(2, new, nh, dtype=torch.bool)
+    bad[0, 40:40 + until, :G] = bad[1, 70:70 + until, G:] = True
+    assert torch.equal(got.isnan().any(-1), bad) and torch.equal(got.isnan().all(-1), bad)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("scale_k,scale_v,scale_q", [(1e-20, 1e20, 1e18), (1e15, 1e-30, 1e-16), (1e-8, 1e-8, 1.0)])
 def test_portions_of_magnitudes_far_from_one(over_the_codes, dtype, scale_k, scale_v, scale_q):
