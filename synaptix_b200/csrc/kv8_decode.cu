@@ -31,6 +31,7 @@
 #include "kv8.cuh"
 
 #define KD_MAX_SEQS 2048
+#define KD_FEW_SEQS 128          // every warp looks at all lengths by itself
 #define KD_SPIN_LIMIT (1u << 26)
 #define KD_DOWN 3.0517578125e-5f      // 2^-15
 #define KD_DESC 64               // items a warp knows ahead: two batches of 32
@@ -116,6 +117,30 @@ __device__ __forceinline__ void kd_starts(const KdArgs& a, int* start, int* warp
   if (threadIdx.x == 0) start[a.S] = before;
   __syncthreads();
 }
+// the same by a warp for itself
+__device__ __forceinline__ void kd_starts_warp(const KdArgs& a, int* start) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+#pragma unroll 1
+  for (int s0 = 0; s0 < a.S; s0 += 32) {
+    const int s = s0 + lane;
+    int n = 0;
+    if (s < a.S) {
+      const int2 r = kd_range(a, s);
+      n = r.y - r.x;
+    }
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (s < a.S) start[s] = before + x - n;
+    before += __shfl_sync(0xffffffffu, x, 31);
+  }
+  if (lane == 0) start[a.S] = before;
+  __syncwarp();
+}
 // the blocks that work (a block of fewer items than warps would leave some idle), and the first item of block b
 __device__ __forceinline__ int kd_workers(const KdArgs& a, int n) { return max(1, min(a.blocks, (n + a.warps - 1) / a.warps)); }
 __device__ __forceinline__ int kd_first(int b, int n, int workers) {
@@ -140,7 +165,7 @@ __device__ __forceinline__ int kd_seq_of(const int* start, int S, int nkv, int x
 template <int HD, bool MORE>
 __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_kernel(const KdArgs a) {
   using L = KdLayout<HD, MORE>;
-  constexpr int RP = MORE ? 2 : 1, WARPS = L::WARPS;
+  constexpr int RP = MORE ? 2 : 1, WARPS = L::WARPS, FIRST = (L::SLOTS + 1) / 2;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ __align__(8) uint64_t bars[WARPS * L::SLOTS];
   __shared__ int warp_sums[WARPS], first_unit[WARPS], last_unit[WARPS], first_seq;
@@ -156,7 +181,13 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
   }
   pdl_wait();
   pdl_trigger();
-  kd_starts<WARPS * 32>(a, start, warp_sums);
+  const bool few = a.S <= KD_FEW_SEQS;
+  if (few) {
+    start += warp * (a.S + 1);                                  // (a copy a warp)
+    kd_starts_warp(a, start);
+  } else {
+    kd_starts<WARPS * 32>(a, start, warp_sums);
+  }
   const int G = a.nh / a.nkv, n_all = start[a.S] * a.nkv;
   if (n_all == 0) {                                             // nobody sees anything
     for (size_t i = blockIdx.x * WARPS * 32 + threadIdx.x; i < (size_t)a.S * a.nh * HD; i += gridDim.x * WARPS * 32) a.out[i] = __float2bfloat16_rn(0.f);
@@ -168,19 +199,27 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
     const int s = blockIdx.x / a.nkv, n = start[s + 1] - start[s];
     b0 = start[s] * a.nkv + (blockIdx.x - s * a.nkv) * n;
     b1 = b0 + n;
-    if (threadIdx.x == 0) first_seq = s;
   } else {
     const int workers = max(1, min(a.blocks, (n_all + WARPS - 1) / WARPS));      // (as kd_workers)
     if (blockIdx.x < workers) {
       b0 = kd_first(blockIdx.x, n_all, workers);
       b1 = kd_first(blockIdx.x + 1, n_all, workers);
     }
-    for (int s = threadIdx.x; s < a.S; s += WARPS * 32)
-      if (start[s] * a.nkv <= b0 && b0 < start[s + 1] * a.nkv) first_seq = s;
   }
-  __syncthreads();
   auto first_of = [&](int w) { return b0 + (b1 - b0) * w / WARPS; };
   const int x0 = first_of(warp), n_items = first_of(warp + 1) - x0;
+  int seq0 = 0;                                                 // a sequence at or before the first item's
+  if (a.by_pair) {
+    seq0 = blockIdx.x / a.nkv;
+  } else if (few) {
+#pragma unroll 1
+    for (int s0 = 0; s0 < a.S; s0 += 32) seq0 += __popc(__ballot_sync(0xffffffffu, s0 + lane < a.S && start[s0 + lane + 1] * a.nkv <= x0));
+  } else {
+    for (int s = threadIdx.x; s < a.S; s += WARPS * 32)
+      if (start[s] * a.nkv <= b0 && b0 < start[s + 1] * a.nkv) first_seq = s;
+    __syncthreads();
+    seq0 = first_seq;
+  }
   int4* desc = desc_all + warp * KD_DESC;                       // (sequence, kv head, page of the sequence, page of the pool)
   unsigned char* ring = smem + warp * L::SLOTS * L::TILE;
   const uint32_t ring_a = kd_smem(ring), bar_a = kd_smem(&bars[warp * L::SLOTS]);
@@ -290,15 +329,17 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
     if (((i + L::AHEAD) & 31) == 0) {                           // the next 32 items
       const int x = i + L::AHEAD + lane;
       if (x < n_items) {
-        int s = first_seq;
+        int s = seq0;
         while (start[s + 1] * a.nkv <= x0 + x) ++s;
         const int n = start[s + 1] - start[s], at = x0 + x - start[s] * a.nkv;
         const int h = at / n, j = kd_range(a, s).x + at - h * n, page = a.block_table[(size_t)(a.row_seq ? a.row_seq[s] : s) * a.maxp + j];
         desc[x & (KD_DESC - 1)] = make_int4(s, h, j, (unsigned)page < (unsigned)a.n_pages ? page : 0);
       }
       __syncwarp();
+      // the first tiles: half of the slots before the query is looked at, half behind it, so that a warp's first keys do not wait for all others' rings
       if (i == -L::AHEAD)
-        for (int n = 0; n < L::SLOTS; ++n) issue(n);
+#pragma unroll 1
+        for (int n = 0; n < FIRST; ++n) issue(n);
     }
     if (lane < 8 && i + L::AHEAD < n_items) {                   // exponents: four lanes for the keys', four for the values'
       const int4 d = desc[(i + L::AHEAD) & (KD_DESC - 1)];
@@ -311,7 +352,11 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
     const int4 d = desc[i & (KD_DESC - 1)];
     if (d.x != seq || d.y != kvh) {
       begin(d.x, d.y, i);
-      if (i == 0) unit0 = d.x * a.nkv + d.y;
+      if (i == 0) {
+        unit0 = d.x * a.nkv + d.y;
+#pragma unroll 1
+        for (int n = FIRST; n < L::SLOTS; ++n) issue(n);
+      }
     }
     const int v0 = a.window > 0 ? max(0, len - a.window - d.z * SX_PAGE) : 0, v1 = len - d.z * SX_PAGE;   // visible keys of the page: v0 <= key < v1
     const bool edge = v0 > 0 || v1 < SX_PAGE;
@@ -686,7 +731,7 @@ static int kd_launch(KdArgs a, cudaStream_t stream) {
     if (dev >= 0 && dev < 64) opted[dev] = true;
   }
   a.warps = L::WARPS;
-  const int rc = sx_launch(kv8_decode_kernel<HD, MORE>, dim3(a.blocks), dim3(L::WARPS * 32), L::FIXED + (a.S + 1) * sizeof(int), stream, a);
+  const int rc = sx_launch(kv8_decode_kernel<HD, MORE>, dim3(a.blocks), dim3(L::WARPS * 32), L::FIXED + (a.S <= KD_FEW_SEQS ? L::WARPS : 1) * (a.S + 1) * sizeof(int), stream, a);
   if (rc || a.by_pair || a.blocks == 1) return rc;
   return sx_launch(kv8_decode_merge_kernel<HD>, dim3(a.blocks - 1), dim3(KD_MERGE_WARPS * 32), (a.S + 1) * sizeof(int), stream, a);
 }
