@@ -22,9 +22,9 @@
 //     the denominator, and 2^(x + E - M + 15) in half precision beside the codes, with M the running maximum of x + E.  So a large value
 //     of next to no weight takes nothing from the precision of the others; weights from 1 down to 2^-29 of the row's largest x + E keep all 11 bits.
 //
-// Measured (replayed graphs, other inputs each time; 32 heads over 8 of 128 unless said): one sequence of 131,072 keys 53 us, 5.1 TB/s; 8 x 4,096 keys 17.2;
-// one of 301 keys 7.8; 64 sequences seeing 1,000 keys, 64 heads over 8 of 64, 27.2.  With parts left out in a copy, us of these four: copies alone 41.8, 10.5, 3.9, 15.3;
-// without the products and the softmax 45.9, 15.6, 5.1, 24.3.  So a long line of pages is bound by HBM, a short one by its start (lengths, places, the first
+// Measured (replayed graphs, other inputs each time; 32 heads over 8 of 128 unless said): one sequence of 131,072 keys 52.5 us, 5.2 TB/s; 8 x 4,096 keys 16.3;
+// one of 301 keys 7.9; 64 sequences seeing 1,000 keys, 64 heads over 8 of 64, 26.0.  With parts left out in a copy (of a state that took 53.1, 18.4, 7.8 and 29.7), us of these
+// four: copies alone 41.8, 10.5, 3.9, 15.3; without the products and the softmax 45.9, 15.6, 5.1, 24.3.  So a long line of pages is bound by HBM, a short one by its start (lengths, places, the first
 // pages: 3 us, cold code), the joins (1 to 1.5 us in the block, 1.5 to 3 of the second kernel) and what a warp does once a pair (its query's two parts, its end).
 //
 // Every wait on an mbarrier is bounded; one that runs out sets the library's status word (sx_kv8_decode_status).
@@ -78,9 +78,8 @@ __device__ __forceinline__ void kd_copy(uint32_t dst, const void* src, uint32_t 
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
                ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-// first visible page of a sequence and one behind its last
-__device__ __forceinline__ int2 kd_range(const KdArgs& a, int s) {
-  const int len = a.seq_lens[s] + a.len_add;
+// first visible page of a sequence of that length and one behind its last
+__device__ __forceinline__ int2 kd_range(const KdArgs& a, int len) {
   const int first = a.window > 0 ? max(0, len - a.window) >> 6 : 0;
   return make_int2(first, max(first, min((len + 63) >> 6, a.maxp)));
 }
@@ -93,7 +92,7 @@ __device__ __forceinline__ void kd_starts(const KdArgs& a, int* start, int* warp
     const int s = s0 + threadIdx.x;
     int n = 0;
     if (s < a.S) {
-      const int2 r = kd_range(a, s);
+      const int2 r = kd_range(a, a.seq_lens[s] + a.len_add);
       n = r.y - r.x;
     }
     int x = n;
@@ -120,15 +119,15 @@ __device__ __forceinline__ void kd_starts(const KdArgs& a, int* start, int* warp
 // the same by a warp for itself
 __device__ __forceinline__ void kd_starts_warp(const KdArgs& a, int* start) {
   const int lane = threadIdx.x & 31;
-  int before = 0;
-#pragma unroll 1
-  for (int s0 = 0; s0 < a.S; s0 += 32) {
-    const int s = s0 + lane;
-    int n = 0;
-    if (s < a.S) {
-      const int2 r = kd_range(a, s);
-      n = r.y - r.x;
-    }
+  int len[KD_FEW_SEQS / 32], before = 0;
+#pragma unroll
+  for (int i = 0; i < KD_FEW_SEQS / 32; ++i) len[i] = 32 * i + lane < a.S ? a.seq_lens[32 * i + lane] : 0;
+#pragma unroll
+  for (int i = 0; i < KD_FEW_SEQS / 32; ++i) {
+    const int s = 32 * i + lane;
+    if (32 * i >= a.S) break;
+    const int2 r = kd_range(a, len[i] + a.len_add);
+    const int n = s < a.S ? r.y - r.x : 0;
     int x = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -332,11 +331,12 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
         int s = seq0;
         while (start[s + 1] * a.nkv <= x0 + x) ++s;
         const int n = start[s + 1] - start[s], at = x0 + x - start[s] * a.nkv;
-        const int h = at / n, j = kd_range(a, s).x + at - h * n, page = a.block_table[(size_t)(a.row_seq ? a.row_seq[s] : s) * a.maxp + j];
+        const int h = at / n, j = kd_range(a, a.seq_lens[s] + a.len_add).x + at - h * n, page = a.block_table[(size_t)(a.row_seq ? a.row_seq[s] : s) * a.maxp + j];
         desc[x & (KD_DESC - 1)] = make_int4(s, h, j, (unsigned)page < (unsigned)a.n_pages ? page : 0);
       }
       __syncwarp();
       // the first tiles: half of the slots before the query is looked at, half behind it, so that a warp's first keys do not wait for all others' rings
+      // (all at once: 17.4 us for 8 x 4,096 keys where this takes 16.3)
       if (i == -L::AHEAD)
 #pragma unroll 1
         for (int n = 0; n < FIRST; ++n) issue(n);
@@ -603,9 +603,9 @@ __global__ void __launch_bounds__(KdLayout<HD, MORE>::WARPS * 32, 1) kv8_decode_
 // Pairs that several blocks shared: block b looks at the border between the stretches b and b + 1, and where that lies within a pair, takes its share of
 // the pair's rows, dealt to the blocks at its borders.  With few parts a warp takes a row, with more than four the warps share a row's parts.  Lengths are
 // read and the place is found while the first kernel still runs: it lets this one in behind its own wait, so what was there before it is there.
-// (As a block of 256 threads for every border and row: 29.7 us for 64 sequences seeing 1,000 keys where this takes 27.3, 18.3 for 8 x 4,096 where it takes
-// 17.3.  Fewer registers in the first kernel, so that these blocks wait on its SMs, cost it more than that gave: 18.8 for 8 x 4,096, 56.6 for one of 65,536
-// where 52.8 stand.)
+// (As a block of 256 threads for every border and row: 29.7 us for 64 sequences seeing 1,000 keys where this took 27.3, 18.3 for 8 x 4,096 where it took
+// 17.3.  Fewer registers in the first kernel, so that these blocks wait on its SMs, cost it more than that gave: 18.8 for 8 x 4,096, 56.6 for one of 131,072
+// where 52.8 stood.)
 #define KD_MERGE_WARPS 4
 template <int HD>
 __global__ void __launch_bounds__(KD_MERGE_WARPS * 32) kv8_decode_merge_kernel(const KdArgs a) {
