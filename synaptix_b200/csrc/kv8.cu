@@ -245,13 +245,13 @@ __device__ __forceinline__ void kv8_prepare_v(const T* __restrict__ qkv, uint8_t
 
 #define KV8_QK_TOKENS 4
 template <typename T, int HD>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) kv8_prepare_wide_kernel(
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) kv8_prepare_wide_kernel(
     const T* __restrict__ qkv, T* __restrict__ q_out, uint8_t* __restrict__ k_pages, uint8_t* __restrict__ v_pages, uint8_t* __restrict__ k_exp,
     uint8_t* __restrict__ v_exp, const float* __restrict__ wq, const float* __restrict__ wk, const float* __restrict__ inv_freq, float eps,
     const int* __restrict__ positions, const int* __restrict__ seq_of_token, const int* __restrict__ block_table, int maxp, int nh, int nkv,
     int n_pages, int row, int n_tokens, int v_blocks, int v_shares) {
   constexpr int HALF = HD / 2, LPH = HD / 16, TOK = KV8_QK_TOKENS;       // lanes a head
-  __shared__ __align__(16) float s_cs[TOK][HALF], s_sn[TOK][HALF];
+  __shared__ __align__(16) float s_cs[TOK][HALF], s_sn[TOK][HALF], s_gain[2][HD];
   __shared__ uint32_t s_top[8][KV8_TOKENS];
   pdl_wait();
   pdl_trigger();
@@ -267,24 +267,26 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) kv8_prepare_wide_
       s_cs[i / HALF][i % HALF] = r.x;
       s_sn[i / HALF][i % HALF] = r.y;
     }
+  if (threadIdx.x < 2 * HD) {
+    const float* gain = threadIdx.x < HD ? wq : wk;
+    if (gain) s_gain[threadIdx.x / HD][threadIdx.x % HD] = gain[threadIdx.x % HD];
+  }
   __syncthreads();
-  // 64 threads a token: its angles stay in registers over all heads, the gains over all q and over all k heads
+  // 64 threads a token: its angles stay in registers over all heads (the gains with them would cost a block an SM)
   constexpr int HPT = 64 / LPH;                                  // heads at a time
   const int tok = threadIdx.x / 64, t = t0 + tok, e0 = (lane % LPH) * 8, h0 = threadIdx.x % 64 / LPH;
   const bool here = tok < tokens;
   const int pos = here ? positions[t] : 0, page = here && k_pages ? kv8_page_of(positions, seq_of_token, block_table, maxp, n_pages, t) : -1;
+  float cs[8], sn[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    cs[i] = inv_freq && here ? s_cs[tok][e0 + i] : 1.f;
+    sn[i] = inv_freq && here ? s_sn[tok][e0 + i] : 0.f;
+  }
 #pragma unroll 1
   for (int kind = 0; kind < (k_pages ? 2 : 1); ++kind) {
-    const float* gain = kind ? wk : wq;
+    const bool gain = kind ? wk != nullptr : wq != nullptr;
     const int n = kind ? nkv : nh;
-    // a' = a f[0] - b f[1], b' = a f[2] + b f[3]: gains and rotation in one
-    float f[4][8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float ga = gain ? gain[e0 + i] : 1.f, gb = gain ? gain[e0 + HALF + i] : 1.f;
-      const float cs = inv_freq && here ? s_cs[tok][e0 + i] : 1.f, sn = inv_freq && here ? s_sn[tok][e0 + i] : 0.f;
-      f[0][i] = ga * cs; f[1][i] = gb * sn; f[2][i] = ga * sn; f[3][i] = gb * cs;
-    }
     typedef typename Kv8Vec<T>::Raw8 Raw;
     const T* src = qkv + (size_t)t * row + (size_t)kind * nh * HD + e0;
     Raw next_a = Kv8Vec<T>::zero8(), next_b = next_a;            // the next head's elements are under way while one is worked at
@@ -302,27 +304,26 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) kv8_prepare_wide_
         next_a = *reinterpret_cast<const Raw*>(src + (size_t)(head + HPT) * HD);
         next_b = *reinterpret_cast<const Raw*>(src + (size_t)(head + HPT) * HD + HALF);
       }
-      float inv = 1.f;
       if (gain) {
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
 #pragma unroll
         for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        inv = rsqrtf(ss / (float)HD + eps);
+        const float inv = rsqrtf(ss / (float)HD + eps);
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+          const float4 ga = *reinterpret_cast<const float4*>(&s_gain[kind][e0 + i]), gb = *reinterpret_cast<const float4*>(&s_gain[kind][e0 + HALF + i]);
+          a[i] *= inv * ga.x; a[i + 1] *= inv * ga.y; a[i + 2] *= inv * ga.z; a[i + 3] *= inv * ga.w;
+          b[i] *= inv * gb.x; b[i + 1] *= inv * gb.y; b[i + 2] *= inv * gb.z; b[i + 3] *= inv * gb.w;
+        }
       }
       if (inv_freq) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float x = a[i] * f[0][i] - b[i] * f[1][i], y = a[i] * f[2][i] + b[i] * f[3][i];
-          a[i] = x * inv;
-          b[i] = y * inv;
-        }
-      } else if (gain) {                                         // (apart: an infinite b times 0 would be NaN in a)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          a[i] *= inv * f[0][i];
-          b[i] *= inv * f[3][i];
+          const float x = a[i] * cs[i] - b[i] * sn[i], y = a[i] * sn[i] + b[i] * cs[i];
+          a[i] = x;
+          b[i] = y;
         }
       }
       if (kind == 0) {
