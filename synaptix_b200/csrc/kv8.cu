@@ -104,8 +104,8 @@ __global__ void __launch_bounds__(KV8_WARPS * 32) kv8_prepare_kernel(
 // all: 338 us for 8,191 tokens of 48 heads of 128, where bytes take 28.6).  There a thread has two dims of up to 16 tokens that share 16
 // neighbouring places of a page, finds the rows' largest magnitudes with its warp by 31 exchanges for all 16 tokens, and stores 16 bytes a dim.
 // (One kernel: 16 rows of values one behind the other are mostly waiting, 23 us alone.)
-// 8,191 tokens of 48 heads of 128 in bfloat16: 48 us, 3.8 TB/s.  It issues two instructions a clock and SM (80 registers, three blocks an SM): what
-// bounds it is the arithmetic of a row (norm, rotation, quantising: some 16 instructions an element) as much as its loads' latency, which the few warps do not hide.
+// 8,191 tokens of 48 heads of 128 in bfloat16: 43 us, 4.3 TB/s (float32 65 us).  What counts is how many rows are under way: two blocks an SM take 60 us,
+// three (gains in registers beside the angles) 48, four 43, five with registers spilled 48; packed arithmetic, two elements an instruction, changes nothing.
 template <typename T> struct Kv8Vec;
 template <> struct Kv8Vec<bf16> {
   typedef uint4 Raw8;                                            // 8 and 2 elements as they lie in memory
@@ -245,7 +245,7 @@ __device__ __forceinline__ void kv8_prepare_v(const T* __restrict__ qkv, uint8_t
 
 #define KV8_QK_TOKENS 4
 template <typename T, int HD>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) kv8_prepare_wide_kernel(
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) kv8_prepare_wide_kernel(
     const T* __restrict__ qkv, T* __restrict__ q_out, uint8_t* __restrict__ k_pages, uint8_t* __restrict__ v_pages, uint8_t* __restrict__ k_exp,
     uint8_t* __restrict__ v_exp, const float* __restrict__ wq, const float* __restrict__ wk, const float* __restrict__ inv_freq, float eps,
     const int* __restrict__ positions, const int* __restrict__ seq_of_token, const int* __restrict__ block_table, int maxp, int nh, int nkv,
