@@ -314,8 +314,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) kv8_prepare_wide_
 #pragma unroll
         for (int i = 0; i < 8; i += 4) {
           const float4 ga = *reinterpret_cast<const float4*>(&s_gain[kind][e0 + i]), gb = *reinterpret_cast<const float4*>(&s_gain[kind][e0 + HALF + i]);
-          a[i] *= inv * ga.x; a[i + 1] *= inv * ga.y; a[i + 2] *= inv * ga.z; a[i + 3] *= inv * ga.w;
-          b[i] *= inv * gb.x; b[i + 1] *= inv * gb.y; b[i + 2] *= inv * gb.z; b[i + 3] *= inv * gb.w;
+          a[i] = a[i] * inv * ga.x; a[i + 1] = a[i + 1] * inv * ga.y; a[i + 2] = a[i + 2] * inv * ga.z; a[i + 3] = a[i + 3] * inv * ga.w;
+          b[i] = b[i] * inv * gb.x; b[i + 1] = b[i + 1] * inv * gb.y; b[i + 2] = b[i + 2] * inv * gb.z; b[i + 3] = b[i + 3] * inv * gb.w;
         }
       }
       if (inv_freq) {

@@ -302,11 +302,29 @@ TILE_ROWS = 64                  # query heads of a kv head x tokens that a block
 # tokens of 4 heads 44 and 13, 374 and 47, 159 and 147); with more the tcgen05 products are worth the pages' way through memory (5 x 32 over 9,000
 # at head size 128 135 and 164, 5 x 64 at 64 229 and 252).
 TILE_BF16_ROWS = {128: 64, 64: 128}
+# And where the pages of all tiles together are few: one launch is 17 us for the host (21 with a cut), reading back and attending 33.  Device time of both, 32
+# heads over 8 of 128: a prompt of 128 (128 pages of tiles) 9.4 and 12.0, of 200 (416) 11.0 and 14.9, five of 60 behind 60 (320) 14.8 and 15.0, but 300
+# (760) 12.3 and 22.0; at head size 64 300 tokens (760) 11.5 and 13.5, 64 behind 2,000 (1,056) 60 and 17.6, 500 behind 200 (2,816) 23.8 and 26.5, 1,024 (8,192) 36 and 52.
+TILE_BF16_PAGES = {128: 512, 64: 2816}
 
 
 def kv8_tile_supported(q: torch.Tensor, nh: int, nkv: int, hd: int, S: int) -> bool:
     """Whether portions of these sizes attend over the codes (``csrc/kv8_tile.cu``)."""
     return hd in TILE_HEAD_DIMS and nh // nkv <= TILE_ROWS and q.shape[0] > 0 and S <= 65535 and q.data_ptr() % 16 == 0
+
+
+def _tile_better(S: int, max_new: int, nh: int, nkv: int, hd: int, max_len: int, window: Optional[int]) -> bool:
+    """Whether bfloat16 portions go by ``kv8_tile`` (else pages are read back)."""
+    if max_new * (nh // nkv) <= TILE_BF16_ROWS[hd]:
+        return True
+    tokens = TILE_ROWS // (nh // nkv)
+    return S * nkv * -(-max_new // tokens) * _tile_pages(max_len, tokens, window) <= TILE_BF16_PAGES[hd]
+
+
+def _tile_pages(max_len: int, tokens: int, window: Optional[int]) -> int:
+    """Pages of a tile of ``tokens`` tokens at most."""
+    pages = -(-max_len // PAGE)
+    return pages if window is None else min(pages, (window + tokens + 125) // PAGE)
 
 
 def _tile_splits(S: int, max_new: int, nh: int, nkv: int, max_pages: int, device) -> int:
@@ -322,9 +340,7 @@ def kv8_tile(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tensor, n
     k, v, ke, ve = pages
     n_pages, nkv, hd, _ = v.shape
     T, S, maxp = q.shape[0], ctx.n_seqs, block_table.shape[1]
-    max_pages = min(-(-ctx.max_len // PAGE), maxp)
-    if window is not None:
-        max_pages = min(max_pages, (window + TILE_ROWS + 125) // PAGE)
+    max_pages = min(_tile_pages(ctx.max_len, TILE_ROWS // (nh // nkv), window), maxp)
     splits = _tile_splits(S, ctx.max_new, nh, nkv, max_pages, q.device)
     if out is None:
         out = torch.empty_like(q)
@@ -379,7 +395,7 @@ def kv8_attention(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tens
         _check_device("kv8_attention", q, *pages, ctx.positions, ctx.seq_of_token, block_table, sinks)
         return kv8_decode(q, pages, ctx.positions, block_table, nh, scale, window, ctx.max_len, sinks, ctx.seq_of_token)
     _check_host("kv8_attention", ctx, block_table)
-    if kv8_tile_supported(q, nh, nkv, hd, ctx.n_seqs) and (q.dtype == torch.float32 or ctx.max_new * (nh // nkv) <= TILE_BF16_ROWS[hd]):
+    if kv8_tile_supported(q, nh, nkv, hd, ctx.n_seqs) and (q.dtype == torch.float32 or _tile_better(ctx.n_seqs, ctx.max_new, nh, nkv, hd, ctx.max_len, window)):
         S = ctx.n_seqs
         if not (ctx.cu_seqlens.dtype == ctx.seq_past.dtype == torch.int32) or ctx.cu_seqlens.numel() <= S or ctx.seq_past.numel() < S:
             raise KernelError("kv8_attention: a first token and a length before the step per sequence (int32)")
