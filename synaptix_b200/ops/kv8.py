@@ -361,6 +361,8 @@ def kv8_attention(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tens
     """Causal attention of the step's packed queries ``q [T, nh * hd]`` over a cache in eight bits that already holds the step's
     keys and values: ``[T, nh * hd]`` in ``q``'s dtype.  The options are those of ``ops.attention``.
 
+    ``q`` has a row for every token of the step; places of the cache that the step's tokens do not see may hold anything.
+
     Single tokens, portions of a few tokens and float32 portions attend over the codes.  Longer portions read the pages back once
     (``kv8_read``) and attend over the result with the kernels of the 16- and 32-bit cache: a page serves many rows there, and
     turning its codes again in every block that reads it would cost more than writing it out once."""
@@ -387,20 +389,21 @@ def kv8_attention(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tens
             return kv8_decode(q, pages, seq_lens, block_table, nh, scale, window, ctx.max_len, sinks)
         return kv8_rows(q, pages, seq_lens, block_table, nh, scale, window, ctx.max_len, softcap=softcap, sinks=sinks, chunk=chunk,
                         out=out, out_col=out_col, out_scale=out_scale)
+    T = q.shape[0]
+    if ctx.host is not None and ctx.host["cu_seqlens"][ctx.n_seqs] != T:
+        raise KernelError("kv8_attention: q has a row for every token of the step and no others")
     if (ctx.max_new <= FEW_NEW_TOKENS and out is None and softcap is None and chunk is None and out_scale == 1.0
             and kv8_decode_supported(q.dtype, nh, nkv, hd, q.shape[0])):
-        T = q.shape[0]
         if not (ctx.positions.dtype == ctx.seq_of_token.dtype == torch.int32) or min(ctx.positions.numel(), ctx.seq_of_token.numel()) < T or block_table.dim() != 2:
             raise KernelError("kv8_attention: a position and a sequence per token (int32), and a table [sequences, pages]")
         _check_device("kv8_attention", q, *pages, ctx.positions, ctx.seq_of_token, block_table, sinks)
         return kv8_decode(q, pages, ctx.positions, block_table, nh, scale, window, ctx.max_len, sinks, ctx.seq_of_token)
     _check_host("kv8_attention", ctx, block_table)
-    if kv8_tile_supported(q, nh, nkv, hd, ctx.n_seqs) and (q.dtype == torch.float32 or _tile_better(ctx.n_seqs, ctx.max_new, nh, nkv, hd, ctx.max_len, window)):
-        S = ctx.n_seqs
-        if not (ctx.cu_seqlens.dtype == ctx.seq_past.dtype == torch.int32) or ctx.cu_seqlens.numel() <= S or ctx.seq_past.numel() < S:
-            raise KernelError("kv8_attention: a first token and a length before the step per sequence (int32)")
-        if ctx.host["cu_seqlens"][S] > q.shape[0]:
-            raise KernelError("kv8_attention: fewer rows of queries than the step has tokens")
+    S = ctx.n_seqs
+    if (not (ctx.cu_seqlens.dtype == ctx.seq_past.dtype == ctx.seq_of_token.dtype == torch.int32) or ctx.cu_seqlens.numel() <= S
+            or ctx.seq_past.numel() < S or ctx.seq_of_token.numel() < T):
+        raise KernelError("kv8_attention: a first token and a length before the step per sequence, and a sequence per token (int32)")
+    if kv8_tile_supported(q, nh, nkv, hd, S) and (q.dtype == torch.float32 or _tile_better(S, ctx.max_new, nh, nkv, hd, ctx.max_len, window)):
         _check_device("kv8_attention", q, *pages, ctx.cu_seqlens, ctx.seq_past, block_table, sinks, out)
         return kv8_tile(q, pages, ctx, block_table, nh, scale, window, softcap=softcap, sinks=sinks, chunk=chunk, out=out, out_col=out_col,
                         out_scale=out_scale)

@@ -124,7 +124,8 @@ def test_attention_refuses(new):
     if new > 1:
         bad += [dict(ctx=step([70], [new], host=None)), dict(ctx=step([70], [new], cu_seqlens=torch.tensor([0.0, 5.0]))),
                 dict(ctx=step([70], [new], seq_past=torch.tensor([65]))), dict(ctx=step([70], [new], cu_seqlens=torch.zeros(1, dtype=torch.int32))),
-                dict(ctx=step([70], [new + 1])), dict(ctx=step([129], [new]))]
+                dict(ctx=step([70], [new + 1])), dict(ctx=step([70], [new - 1])), dict(ctx=step([129], [new])),
+                dict(ctx=step([70], [new], seq_of_token=torch.zeros(new - 1, dtype=torch.int32)))]
     for change in bad:
         with pytest.raises(KernelError):
             ops.kv8_attention(**{**ok, **change})
