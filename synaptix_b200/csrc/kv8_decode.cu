@@ -38,7 +38,7 @@
 #define KD_LOG2E 1.44269504f
 
 // Three warps a scheduler hide one another's latencies: a page takes a warp alone 3,400 clocks, and HBM delivers one to an SM every 710 (four at head
-// size 64 and three slots each: 33.0 us for 64 sequences seeing 1,000 keys where three take 31.5).  With more than 8 heads a kv head a thread has two
+// size 64 and three slots each: 33.0 us for 64 sequences seeing 1,000 keys where three took 31.5, 26.0 by now).  With more than 8 heads a kv head a thread has two
 // rows' registers, and there are two.
 template <int HD, bool MORE> struct KdLayout {
   static constexpr int WARPS = MORE ? 8 : 12;
