@@ -798,7 +798,9 @@ __global__ void __launch_bounds__(256) attn_tc_parts_merge_kernel(const float* _
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const float g = ft_ex2(ml[k].x - base);
-      if (g == 0.f) continue;                                    // (a part without a visible key has zeros, or what stood there)
+      // A part without a visible key has nothing to add.  One of no weight is added all the same: its sum is NaN where a key it saw is, also where its
+      // maximum, which leaves NaN out, is minus infinity or far below the row's.
+      if (ml[k].y == 0.f) continue;
       L += ml[k].y * g;
       x.x += v[k].x * g; x.y += v[k].y * g; x.z += v[k].z * g; x.w += v[k].w * g;
     }

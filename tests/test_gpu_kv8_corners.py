@@ -1,0 +1,68 @@
+"""Attention over a cache in eight bits where its parts meet: rows that are not finite at the border of a stretch of keys.  Bounds as in ``test_gpu_kv8``."""
+import importlib
+import math
+
+import pytest
+import torch
+
+import plain_kv8 as P
+from test_gpu_kv8 import on_gpu, randn
+from test_kv8_cpu import step
+
+pytestmark = pytest.mark.gpu
+
+
+def attend(q, held, ctx, nh, nkv, hd, scale, window=None, **kw):
+    from synaptix_b200 import ops
+    return ops.kv8_attention(q.view(q.shape[0], -1).cuda(), held.pages(), on_gpu(ctx), held.table.cuda(), nh, nkv, hd, scale, window, **kw).cpu().view(-1, nh, hd)
+
+
+# ---- cut tiles (csrc/attn_tc.cu)
+
+@pytest.mark.parametrize("what", ["key", "value"])
+@pytest.mark.parametrize("sinks", [False, True])
+def test_a_row_that_is_not_finite_begins_a_stretch_of_keys(what, sinks):
+    """The first key of a stretch is the only one that its own token sees there."""
+    from synaptix_b200.ops.attention import tc_parts
+    past, new, nh, nkv, hd = 9156, 150, 4, 2, 128
+    tiles = [(past + q0, min(past + q0 + 128, past + new) - 1) for _ in range(2) for q0 in (0, 128)]
+    chunk, parts = tc_parts(tiles, nh, None, torch.device("cuda", 0))
+    token = 60
+    assert parts > 1 and (past + token) % (chunk * 128) == 0
+    ks, vs = ([randn(past + new, nkv, hd, seed=i + 7 * w) for i in range(2)] for w in (1, 2))
+    q, s, res = randn(2 * new, nh, hd).bfloat16(), randn(nh, seed=9).cuda() if sinks else None, []
+    for spoil in (False, True):
+        if spoil:
+            (ks if what == "key" else vs)[1][past + token, 1, 5] = math.nan
+        res.append(attend(q, P.Held(ks, vs), step([past + new] * 2, [new] * 2), nh, nkv, hd, 0.1, sinks=s).view(2, new, nh, hd))
+    bad = torch.zeros(2, new, nh, dtype=torch.bool)
+    bad[1, token:, 2:] = True
+    assert torch.equal(res[1].isnan().any(-1), bad) and torch.equal(res[1].isnan().all(-1), bad)
+    assert torch.equal(res[0][~bad], res[1][~bad]) and not res[0].isnan().any()
+
+
+@pytest.mark.parametrize("window", [None, 130, 200])
+def test_rows_that_are_not_finite_in_short_stretches(monkeypatch, window):
+    """Stretches of 128 keys: spoiled keys at the first and the last place of a stretch, so that a window's lower end leaves that one key of it, and
+    one among keys whose weights are nothing beside the others'."""
+    cut = []
+    monkeypatch.setattr(importlib.import_module("synaptix_b200.ops.attention"), "tc_parts", lambda *a: cut.append(1) or (1, 6))
+    past, new, nh, nkv, hd = 500, 150, 16, 2, 128
+    n = past + new
+    ks, vs = ([randn(n, nkv, hd, seed=i + 7 * w) for i in range(4)] for w in (1, 2))
+    q = randn(4 * new, nh, hd).bfloat16()
+    q[3 * new:] = 1.0
+    ks[3][:128], ks[3][128:] = -4.0, 0.0                           # scores of -256 and 0: weights of 2^-369 and 1
+    spoiled = [512, 511, 383, 77]
+    res = []
+    for spoil in (False, True):
+        if spoil:
+            for s, j in enumerate(spoiled):
+                (vs if s == 2 else ks)[s][j, 0, 3] = math.inf
+        res.append(attend(q, P.Held(ks, vs), step([n] * 4, [new] * 4), nh, nkv, hd, 0.5, window).view(4, new, nh, hd))
+    pos = torch.arange(past, n)
+    bad = torch.zeros(4, new, nh, dtype=torch.bool)
+    for s, j in enumerate(spoiled):
+        bad[s, :, :8] = ((pos >= j) & (pos - (window or n) < j))[:, None]
+    assert cut and torch.equal(res[1].isnan().any(-1), bad) and torch.equal(res[1].isnan().all(-1), bad)
+    assert torch.equal(res[0][~bad], res[1][~bad]) and not res[0].isnan().any()
