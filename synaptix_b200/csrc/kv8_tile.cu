@@ -11,7 +11,8 @@
 //     of one dim is one 16-byte load: nothing moves between lanes.  In float32 weights are two halves as well.
 //   * Powers of two.  With x the score (base 2) and E a value's exponent, p = 2^(x - m) goes into the denominator, and p 2^E 2^(15 + m - M) into the half
 //     precision beside the codes.  m is the running maximum of x and M that of x + E, each rounded UP to an integer: changing either multiplies by exact powers of two,
-//     and one exponential serves both.  Weights down to 2^-29 of the row's largest keep 11 bits (22 in float32).
+//     and one exponential serves both.  Weights down to 2^-29 of the row's largest keep 11 bits (22 in float32);
+//     down to 2^-24 where all values that a row sees have the format's lowest powers.
 // A key that is not finite (exponent 255), or whose place nobody has written, has its codes replaced by zeros before the products, and rows that see such a key
 // become NaN by their scores: rows that do not see it keep their values.
 //
@@ -284,7 +285,8 @@ __global__ void __launch_bounds__(KT_WARPS * 32, 2) kv8_tile_kernel(const KtArgs
     for (int r = 0; r < 2; ++r) {
       most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], 1));
       most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], 2));
-      const float next = fmaxf(M[r], m[r] + (float)((__float_as_int(most[r]) >> 23) - 126));
+      // (M stays within 112 of m: 2^(15 + m - M) is then a float32 number, and weights are no smaller for values whose powers are all below 2^-112)
+      const float next = fmaxf(M[r], m[r] + (float)max((__float_as_int(most[r]) >> 23) - 126, -112));
       shrink[r] = M[r] == next ? 1.f : kt_pow2(M[r] - next);
       moved = moved || M[r] != next;
       M[r] = next;

@@ -1,4 +1,5 @@
-"""Attention over a cache in eight bits where its parts meet: rows that are not finite at the border of a stretch of keys.  Bounds as in ``test_gpu_kv8``."""
+"""Attention over a cache in eight bits where its parts meet: rows that are not finite at the border of a stretch of keys, values at the format's
+smallest powers.  Bounds as in ``test_gpu_kv8``."""
 import importlib
 import math
 
@@ -6,7 +7,7 @@ import pytest
 import torch
 
 import plain_kv8 as P
-from test_gpu_kv8 import on_gpu, randn
+from test_gpu_kv8 import check, filled, on_gpu, over_the_codes, randn  # noqa: F401
 from test_kv8_cpu import step
 
 pytestmark = pytest.mark.gpu
@@ -66,3 +67,37 @@ def test_rows_that_are_not_finite_in_short_stretches(monkeypatch, window):
         bad[s, :, :8] = ((pos >= j) & (pos - (window or n) < j))[:, None]
     assert cut and torch.equal(res[1].isnan().any(-1), bad) and torch.equal(res[1].isnan().all(-1), bad)
     assert torch.equal(res[0][~bad], res[1][~bad]) and not res[0].isnan().any()
+
+
+# ---- the format's ends
+
+def values_of_exponents(lens, nkv, hd, exponents, seed=0):
+    """Sequences whose value rows have these exponent bytes in turn."""
+    held = filled(lens, nkv, hd, seed=seed, loud=False)
+    vs = []
+    for s, n in enumerate(lens):
+        x = torch.clamp(randn(n, nkv, hd, seed=seed + 50 + s) / 4, -1, 1).double()
+        x[..., 3] = 1.0
+        e = torch.tensor(exponents)[torch.arange(n) % len(exponents)]
+        vs.append((x * torch.exp2(e.double() - 127 + 8)[:, None, None]).float())       # a row of largest magnitude 2^x has e - 127 = x - 8
+    ks = [k.float() for k in held.keys]
+    held = P.Held(ks, vs, seed=seed)
+    for s, n in enumerate(lens):
+        for j in range(min(n, len(exponents))):
+            assert int(held.v_exp[int(held.table[s, j // 64]), 0, j % 64]) == exponents[j]
+    return held
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("exponents", [[e] for e in range(10, 18)] + [[10, 15], [10, 12, 30], [11, 127]])
+@pytest.mark.parametrize("lens,new", [([40], [40]), ([2000, 70], [20, 12])])
+def test_portions_over_values_at_the_formats_lower_end(over_the_codes, dtype, exponents, lens, new):  # noqa: F811
+    nh, nkv, hd = 8, 2, 64
+    check(2 * randn(sum(new), nh, hd, seed=3), values_of_exponents(lens, nkv, hd, exponents), lens, new, nh, hd, dtype, dtype == torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 64), (torch.bfloat16, 96), (torch.float32, 64)])
+@pytest.mark.parametrize("exponents", [[10], [12], [16], [10, 30]])
+def test_single_tokens_over_values_at_the_formats_lower_end(dtype, hd, exponents):
+    lens, nh, nkv = [40, 700], 8, 2
+    check(2 * randn(2, nh, hd, seed=3), values_of_exponents(lens, nkv, hd, exponents), lens, [1, 1], nh, hd, dtype, dtype == torch.bfloat16)
