@@ -340,14 +340,16 @@ def attention_from_projection(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages:
 
 
 def _query_tiles(ctx, rows: int, device):
-    """The step's query tiles of ``rows`` rows as two device arrays (sequence, first row), made once a step."""
-    tiles = ctx.scratch.get(("query_tiles", rows))
-    if tiles is None:
+    """The step's query tiles of ``rows`` rows as two device arrays (sequence, first row), made once a step (and anew where a
+    context is used for other portions)."""
+    cu = ctx.host["cu_seqlens"]
+    made = ctx.scratch.get(("query_tiles", rows))
+    if made is None or made[1] != cu:
         import numpy as np
-        ts, t0 = query_tiles(ctx.host["cu_seqlens"], rows)
+        ts, t0 = query_tiles(cu, rows)
         both = torch.from_numpy(np.asarray([ts, t0], dtype=np.int32)).to(device, non_blocking=True)
-        tiles = ctx.scratch[("query_tiles", rows)] = (both[0], both[1])
-    return tiles
+        made = ctx.scratch[("query_tiles", rows)] = ((both[0], both[1]), list(cu))
+    return made[0]
 
 
 def attn_scored(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, ctx, block_table: torch.Tensor, H: int,
@@ -375,14 +377,15 @@ def attn_scored(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, c
 
 
 def _portions(ctx):
-    """What each sequence brings and had before, as ``attn_generic`` takes it, made once a step; ``None`` where the host does not
-    know."""
+    """What each sequence brings and had before, as ``attn_generic`` takes it, made once a step (and anew where a context is used
+    for other lengths); ``None`` where the host does not know."""
     if ctx.host is None:
         return None
-    both = ctx.scratch.get("portions")
-    if both is None:
-        both = ctx.scratch["portions"] = tuple((ctypes.c_int * len(x))(*x) for x in (ctx.host["cu_seqlens"], ctx.host["seq_past"]))
-    return both
+    cu, past = ctx.host["cu_seqlens"], ctx.host["seq_past"]
+    made = ctx.scratch.get("portions")
+    if made is None or made[1] != cu or made[2] != past:
+        made = ctx.scratch["portions"] = (tuple((ctypes.c_int * len(x))(*x) for x in (cu, past)), list(cu), list(past))
+    return made[0]
 
 
 def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, ctx, block_table: torch.Tensor,

@@ -1,5 +1,5 @@
 """Attention over a cache in eight bits where its parts meet: rows that are not finite at the border of a stretch of keys, values at the format's
-smallest powers.  Bounds as in ``test_gpu_kv8``."""
+smallest powers, a context that comes back with other lengths.  Bounds as in ``test_gpu_kv8``."""
 import importlib
 import math
 
@@ -7,8 +7,9 @@ import pytest
 import torch
 
 import plain_kv8 as P
-from test_gpu_kv8 import check, filled, on_gpu, over_the_codes, randn  # noqa: F401
+from test_gpu_kv8 import bound, check, filled, on_gpu, over_the_codes, randn  # noqa: F401
 from test_kv8_cpu import step
+from test_kv8_corners_cpu import comes_back
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +102,32 @@ def test_portions_over_values_at_the_formats_lower_end(over_the_codes, dtype, ex
 def test_single_tokens_over_values_at_the_formats_lower_end(dtype, hd, exponents):
     lens, nh, nkv = [40, 700], 8, 2
     check(2 * randn(2, nh, hd, seed=3), values_of_exponents(lens, nkv, hd, exponents), lens, [1, 1], nh, hd, dtype, dtype == torch.bfloat16)
+
+
+# ---- a context that comes back
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd,cut", [(torch.bfloat16, 32, 2, 128, False), (torch.bfloat16, 32, 2, 128, True), (torch.bfloat16, 64, 2, 64, False),
+                                                 (torch.bfloat16, 4, 2, 96, False), (torch.float32, 4, 2, 80, False)])
+def test_a_context_that_comes_back_with_other_portions(monkeypatch, dtype, nh, nkv, hd, cut):
+    """As many tokens in all, dealt to the sequences in another way: what the first call made for the context is made anew."""
+    from synaptix_b200 import ops
+    module = importlib.import_module("synaptix_b200.ops.attention")
+    if cut:
+        monkeypatch.setattr(module, "tc_parts", lambda *a: (2, 6))
+    read, reads = ops.kv8._read, []
+    monkeypatch.setattr(ops.kv8, "_read", lambda *a: reads.append(1) or read(*a))
+    ctx, scale = None, hd ** -0.5
+    for lens, new in (([700, 1200], [150, 280]), ([800, 1100], [280, 150]), ([430, 900], [429, 1])):
+        held = filled(lens, nkv, hd, seed=lens[0])
+        ctx = step(lens, new) if ctx is None else comes_back(ctx, lens, new)
+        q = (2 * randn(sum(new), nh, hd, seed=3)).to(dtype)
+        got = attend(q, held, ctx, nh, nkv, hd, scale)
+        assert torch.equal(got, attend(q, held, step(lens, new), nh, nkv, hd, scale))
+        at = 0
+        for s, (n, m) in enumerate(zip(lens, new)):
+            part = slice(at, at + m)
+            at += m
+            want, weight = P.attend(q[part], held.keys[s], held.values[s], torch.arange(n - m, n), scale)
+            tol = bound(q[part], held, s, want, weight, None, scale, dtype, hd, dtype == torch.bfloat16, portions=True)
+            assert ((got[part].reshape(m, -1).double() - want).abs() <= tol).all(), (lens, s)
+    assert len(reads) == 6
