@@ -399,8 +399,9 @@ extern "C" int sx_kv8_prepare(const void* qkv, void* q_out, void* k_pages, void*
 // behind the sequence's end as zeros.  A block a (page, kv head), bound by its bytes.  A lane of keys takes 8 codes of a
 // row at a time (16 bytes of bfloat16); a lane of values takes 8 dims of 4 keys, one word a dim, turns the bytes around in registers and
 // stores 16 bytes a key: 8 lanes beside one another read 32 bytes of a dim, 4 write 64 of a key.
-// for_attention: a value row that is not finite comes back as zeros and its key row as NaN instead.  Kernels that multiply a page's values with weights of
-// several tokens then give NaN to the tokens that see the row, by their scores, and to no others (a weight of zero times NaN would).
+// page_from (attention): page i's rows before page_from[i], which no token of the step sees, are zeros, too, and a value row that is not finite comes back as zeros
+// and its key row as NaN instead.  Kernels that multiply a page's values with weights of several tokens then give NaN to the tokens that see the
+// row, by their scores, and to no others (a weight of zero times NaN would).
 // Eight sequences of 4,969 to 12,000 tokens, 8 heads of 128, to bfloat16: 70 to 73 us for 411 MB moved, 5.6 to 5.8 TB/s: HBM, nine tenths of a plain copy's rate.
 // ---------------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ void kv8_store8(T* dst, const uint32_t (&pairs)[4], float f, bool held) {
@@ -418,8 +419,8 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(256) kv8_read_kernel(
     const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages, const uint8_t* __restrict__ k_exp,
     const uint8_t* __restrict__ v_exp, T* __restrict__ k_out, T* __restrict__ v_out, const int* __restrict__ page_seq,
-    const int* __restrict__ page_idx, const int* __restrict__ seq_lens, const int* __restrict__ block_table, int maxp, int nkv, int hd_,
-    int n_pages, int for_attention) {
+    const int* __restrict__ page_idx, const int* __restrict__ page_from, const int* __restrict__ seq_lens, const int* __restrict__ block_table,
+    int maxp, int nkv, int hd_, int n_pages) {
   __shared__ float s_k[SX_PAGE], s_v[SX_PAGE];
   pdl_wait();
   pdl_trigger();
@@ -428,7 +429,7 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(
   const int s = page_seq[i], j = page_idx[i];
   const int page = block_table[(size_t)s * maxp + j];
   const bool ok = page >= 0 && page < n_pages;
-  const int held = ok ? min(SX_PAGE, max(0, seq_lens[s] - j * SX_PAGE)) : 0;
+  const int held = ok ? min(SX_PAGE, max(0, seq_lens[s] - j * SX_PAGE)) : 0, from_key = page_from ? page_from[i] : 0;
   const size_t from = (size_t)(ok ? page : 0) * nkv + kvh, to = ((size_t)i * nkv + kvh) * SX_PAGE * hd;
   const uint8_t *k = k_pages + from * SX_PAGE * hd, *v = v_pages + from * SX_PAGE * hd;
   constexpr int NK = HD ? HD / 32 : 1, NV = 1;     // items of a thread, where that is known
@@ -453,7 +454,7 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(
   }
   if (threadIdx.x < 2 * SX_PAGE) {
     const int key = threadIdx.x & (SX_PAGE - 1), ve = v_exp[from * SX_PAGE + key];
-    const bool gone = for_attention && ve == KV8_NAN;
+    const bool gone = page_from && ve == KV8_NAN;
     if (threadIdx.x < SX_PAGE) s_k[key] = kv8_scale(gone ? KV8_NAN : k_exp[from * SX_PAGE + key]);
     else s_v[key] = gone ? 0.f : kv8_scale(ve);
   }
@@ -461,7 +462,7 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(
   auto put_k = [&](int o, const uint2 w) {
     const int key = o / groups, d = o % groups * 8;
     const uint32_t pairs[4] = {w.x, w.x >> 16, w.y, w.y >> 16};
-    kv8_store8<T>(k_out + to + key * hd + d, pairs, s_k[key], key < held);
+    kv8_store8<T>(k_out + to + key * hd + d, pairs, s_k[key], key < held && key >= from_key);
   };
   auto put_v = [&](int o, const uint32_t (&w)[8]) {
     const int key = v_key(o), group = v_group(o);
@@ -470,7 +471,7 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(
       uint32_t pairs[4];
 #pragma unroll
       for (int d = 0; d < 4; ++d) pairs[d] = __byte_perm(w[2 * d], w[2 * d + 1], n | (4 + n) << 4);
-      kv8_store8<T>(v_out + to + (key + n) * hd + group * 8, pairs, s_v[key + n], key + n < held && s_v[key + n] != 0.f);
+      kv8_store8<T>(v_out + to + (key + n) * hd + group * 8, pairs, s_v[key + n], key + n < held && key + n >= from_key && s_v[key + n] != 0.f);
     }
   };
   if constexpr (HD != 0) {
@@ -492,15 +493,15 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(
 }
 
 extern "C" int sx_kv8_read(const void* k_pages, const void* v_pages, const void* k_exp, const void* v_exp, void* k_out, void* v_out,
-                           const int* page_seq, const int* page_idx, int n_out, const int* seq_lens, const int* block_table, int maxp,
-                           int nkv, int hd, int n_pages, int for_attention, int dt, cudaStream_t stream) {
+                           const int* page_seq, const int* page_idx, const int* page_from, int n_out, const int* seq_lens,
+                           const int* block_table, int maxp, int nkv, int hd, int n_pages, int dt, cudaStream_t stream) {
   if (n_out <= 0) return 0;
   if (hd <= 0 || hd % 16 || hd > KV8_MAX_HD || nkv <= 0 || nkv > 65535) return SX_ERR_SIZE;
   if (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) return SX_ERR_ALIGN;
   const dim3 grid(n_out, nkv);
 #define KV8_READ(T, HD)                                                                                                                            \
   sx_launch(kv8_read_kernel<T, HD>, grid, dim3(256), 0, stream, (const uint8_t*)k_pages, (const uint8_t*)v_pages, (const uint8_t*)k_exp,             \
-            (const uint8_t*)v_exp, (T*)k_out, (T*)v_out, page_seq, page_idx, seq_lens, block_table, maxp, nkv, hd, n_pages, for_attention)
+            (const uint8_t*)v_exp, (T*)k_out, (T*)v_out, page_seq, page_idx, page_from, seq_lens, block_table, maxp, nkv, hd, n_pages)
   if (dt == SX_F32) return hd == 64 ? KV8_READ(float, 64) : hd == 128 ? KV8_READ(float, 128) : KV8_READ(float, 0);
   if (dt == SX_BF16) return hd == 64 ? KV8_READ(bf16, 64) : hd == 128 ? KV8_READ(bf16, 128) : KV8_READ(bf16, 0);
   return SX_ERR_DTYPE;

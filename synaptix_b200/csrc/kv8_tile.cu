@@ -13,8 +13,9 @@
 //     precision beside the codes.  m is the running maximum of x and M that of x + E, each rounded UP to an integer: changing either multiplies by exact powers of two,
 //     and one exponential serves both.  Weights down to 2^-29 of the row's largest keep 11 bits (22 in float32);
 //     down to 2^-24 where all values that a row sees have the format's lowest powers.
-// A key that is not finite (exponent 255), or whose place nobody has written, has its codes replaced by zeros before the products, and rows that see such a key
-// become NaN by their scores: rows that do not see it keep their values.
+// A value that is not finite (exponent 255) has its codes replaced by zeros before the products, and rows that see its key become NaN by their scores: rows
+// that do not see it keep their values.  So have values of keys that no token of the tile sees, before its window or chunk and behind its last
+// token: what lies there may be anything, a code that is NaN beside any exponent.
 //
 // Few tiles are cut: a block takes a share of its tile's pages, and a second kernel joins the shares.
 //
@@ -59,7 +60,7 @@ __global__ void __launch_bounds__(KT_WARPS * 32, 2) kv8_tile_kernel(const KtArgs
   const int G = a.nh / a.nkv, tokens = KT_ROWS / G, t0 = a.cu[seq], n_new = a.cu[seq + 1] - t0, q0 = tile * tokens;
   if (q0 >= n_new) return;
   const int n_tok = min(tokens, n_new - q0), first = a.past[seq] + q0, end = first + n_tok;     // positions of the tile: first .. end - 1
-  const int page0 = kt_lo(a, first) >> 6, n_pages = max(0, min((end + 63) >> 6, a.maxp) - page0);
+  const int begin = kt_lo(a, first), page0 = begin >> 6, n_pages = max(0, min((end + 63) >> 6, a.maxp) - page0);       // (no token of the tile sees a key before)
   const int per = (n_pages + a.n_splits - 1) / a.n_splits, p0 = page0 + min(split * per, n_pages), p1 = min(p0 + per, page0 + n_pages);
   // the rows of the thread (g, g + 8 of the warp's) and the keys they see
   int tok[2], head[2], lo[2], hi[2];
@@ -172,13 +173,13 @@ __global__ void __launch_bounds__(KT_WARPS * 32, 2) kv8_tile_kernel(const KtArgs
     uint32_t nan[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) nan[i] = __vcmpeq4(ve[i], 0xffffffffu);
-    const bool mend = __any_sync(0xffffffffu, (nan[0] | nan[1] | nan[2] | nan[3]) != 0) || key0 + SX_PAGE > end;     // (the same in every warp)
+    const bool mend = __any_sync(0xffffffffu, (nan[0] | nan[1] | nan[2] | nan[3]) != 0) || key0 + SX_PAGE > end || key0 < begin;     // (the same in every warp)
     if (mend) {
       uint32_t keep[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int n = min(max(end - key0 - 16 * t - 4 * i, 0), 4);      // keys of these four that somebody of the tile may see
-        keep[i] = (n == 4 ? ~0u : (1u << (8 * n)) - 1u) & ~nan[i];
+        const int key = key0 + 16 * t + 4 * i, n = min(max(end - key, 0), 4), m = min(max(begin - key, 0), 4);      // of these four: m <= i < n are keys that somebody of the tile may see
+        keep[i] = (n == 4 ? ~0u : (1u << (8 * n)) - 1u) & (m == 4 ? 0u : ~0u << (8 * m)) & ~nan[i];
         ve[i] &= ~nan[i];
       }
       for (int at = threadIdx.x * 16; at < TILE; at += KT_WARPS * 512) {            // (a thread's chunks are all of its 16 keys)

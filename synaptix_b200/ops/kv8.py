@@ -152,13 +152,13 @@ def kv8_prepare(qkv: torch.Tensor, q_out: Optional[torch.Tensor], pages: Optiona
 
 
 def _read_plan(ctx, width: int, window: Optional[int], chunk: Optional[int], device):
-    """Which pages of which sequence are read, in order, and the table that finds them again, made once a step (and anew where a context is used for
-    other lengths)."""
+    """The table that finds the pages read again, which pages of which sequence they are, in order, and from which row on tokens of the step
+    see them, made once a step (and anew where a context is used for other lengths)."""
     past, lens = ctx.host["seq_past"], ctx.host["seq_lens"]
     plan = ctx.scratch.get(("kv8_read", width, window, chunk))
     if plan is not None and plan[4] == past and plan[5] == lens:
         return plan
-    seqs, idx, table = [], [], np.zeros((len(lens), width), dtype=np.int32)
+    seqs, idx, rows, table = [], [], [], np.zeros((len(lens), width), dtype=np.int32)
     for s, (p, n) in enumerate(zip(past, lens)):
         first = max(0, p - window + 1) if window else 0                  # the first key that the step's first token sees
         if chunk:
@@ -168,11 +168,12 @@ def _read_plan(ctx, width: int, window: Optional[int], chunk: Optional[int], dev
         table[s, :b] = at + np.maximum(np.arange(b) - a, 0)
         seqs += [s] * (b - a)
         idx += range(a, b)
-    flat = np.concatenate([table.reshape(-1), np.asarray(seqs + idx, dtype=np.int32)])
+        rows += [max(0, first - PAGE * i) for i in range(a, b)]
+    flat = np.concatenate([table.reshape(-1), np.asarray(seqs + idx + rows, dtype=np.int32)])
     dev = torch.from_numpy(flat).to(device, non_blocking=True)
-    n = len(idx)
-    plan = ctx.scratch[("kv8_read", width, window, chunk)] = (dev[:table.size].view(table.shape), dev[table.size:table.size + n],
-                                                              dev[table.size + n:], n, list(past), list(lens))
+    n, at = len(idx), table.size
+    plan = ctx.scratch[("kv8_read", width, window, chunk)] = (dev[:at].view(table.shape), dev[at:at + n], dev[at + n:at + 2 * n], dev[at + 2 * n:], list(past),
+                                                              list(lens))
     return plan
 
 
@@ -204,16 +205,19 @@ def kv8_read(pages: KV8Pages, ctx, block_table: torch.Tensor, dtype: torch.dtype
 
 
 def _read(pages: KV8Pages, ctx, block_table: torch.Tensor, dtype: torch.dtype, window: Optional[int], chunk: Optional[int], for_attention: bool):
-    """``kv8_read`` of what has been checked.  ``for_attention``: value rows that are not finite are zeros, and their keys NaN."""
+    """``kv8_read`` of what has been checked.  ``for_attention``: rows that no token of the step sees are zeros; so are value rows that are not
+    finite, and their keys are NaN."""
     k8, v8, ke, ve = pages
     n_pages, nkv, hd, _ = v8.shape
     device, width = v8.device, block_table.shape[1]
-    table, seqs, idx, n, _, _ = _read_plan(ctx, width, window, chunk, device)
+    table, seqs, idx, rows, _, _ = _read_plan(ctx, width, window, chunk, device)
+    n = idx.numel()
     k = torch.empty((n, nkv, PAGE, hd), dtype=dtype, device=device)
     v = torch.empty_like(k)
     check(launcher("kv8", "sx_kv8_read")(
-        k8.data_ptr(), v8.data_ptr(), ke.data_ptr(), ve.data_ptr(), k.data_ptr(), v.data_ptr(), seqs.data_ptr(), idx.data_ptr(), n,
-        ctx.seq_lens.data_ptr(), block_table.data_ptr(), width, nkv, hd, n_pages, for_attention, dt_code(dtype), raw_stream()), "kv8_read", 1 if n else 0)
+        k8.data_ptr(), v8.data_ptr(), ke.data_ptr(), ve.data_ptr(), k.data_ptr(), v.data_ptr(), seqs.data_ptr(), idx.data_ptr(),
+        rows.data_ptr() if for_attention else None, n, ctx.seq_lens.data_ptr(), block_table.data_ptr(), width, nkv, hd, n_pages, dt_code(dtype),
+        raw_stream()), "kv8_read", 1 if n else 0)
     return k, v, table
 
 

@@ -1,5 +1,5 @@
 """Attention over a cache in eight bits where its parts meet: rows that are not finite at the border of a stretch of keys, values at the format's
-smallest powers, a context that comes back with other lengths.  Bounds as in ``test_gpu_kv8``."""
+smallest powers, places nobody sees, a context that comes back with other lengths.  Bounds as in ``test_gpu_kv8``."""
 import importlib
 import math
 
@@ -131,3 +131,67 @@ def test_a_context_that_comes_back_with_other_portions(monkeypatch, dtype, nh, n
             tol = bound(q[part], held, s, want, weight, None, scale, dtype, hd, dtype == torch.bfloat16, portions=True)
             assert ((got[part].reshape(m, -1).double() - want).abs() <= tol).all(), (lens, s)
     assert len(reads) == 6
+
+
+# ---- places that nobody sees
+
+def littered(lens, new, nkv, hd, window=None, chunk=None, seed=0):
+    """Sequences where the places that no token of the step sees hold arbitrary codes and exponents: NaN codes, powers up to 2^127."""
+    held = filled(lens, nkv, hd, seed=seed)
+    g = torch.Generator().manual_seed(seed + 1)
+    for s, (n, m) in enumerate(zip(lens, new)):
+        p = n - m
+        first = max(max(0, p - window + 1) if window else 0, p // chunk * chunk if chunk else 0)
+        for j in [*range(first), *range(n, -(-n // 64) * 64)]:
+            page, r = int(held.table[s, j // 64]), j % 64
+            for t in (held.k, held.v, held.k_exp, held.v_exp):
+                where = t[page, :, :, r] if t is held.k else t[page, ..., r]
+                where.copy_(torch.randint(0, 256, where.shape, generator=g).byte())
+            held.v[page, :, ::3, r] = 0x7f if j % 2 else 0xff
+            held.v_exp[page, :, r] = 100 + (j * 7) % 155
+    return held
+
+
+@pytest.fixture
+def read_back(monkeypatch):
+    """All portions go through pages read back, whatever is faster."""
+    from synaptix_b200.ops import kv8
+    monkeypatch.setattr(kv8, "FEW_NEW_TOKENS", 0)
+    for name in ("TILE_BF16_ROWS", "TILE_BF16_PAGES"):
+        monkeypatch.setattr(kv8, name, {64: 0, 128: 0})
+
+
+OPTIONS = [{}, dict(window=50), dict(window=64), dict(window=200, chunk=96)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("options", OPTIONS)
+def test_portions_over_the_codes_beside_places_nobody_sees(over_the_codes, dtype, hd, options):  # noqa: F811
+    lens, new, nh, nkv = [300, 131, 1000], [33, 20, 100], 8, 2
+    held = littered(lens, new, nkv, hd, **options)
+    check(2 * randn(sum(new), nh, hd, seed=3), held, lens, new, nh, hd, dtype, dtype == torch.bfloat16, **options)
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", [(torch.bfloat16, 8, 2, 128), (torch.bfloat16, 8, 2, 64), (torch.bfloat16, 4, 2, 32), (torch.bfloat16, 4, 2, 96),
+                                             (torch.float32, 4, 2, 80), (torch.float32, 4, 2, 32)])
+@pytest.mark.parametrize("options", OPTIONS)
+def test_portions_read_back_beside_places_nobody_sees(read_back, dtype, nh, nkv, hd, options):
+    lens, new = [300, 131, 1000], [33, 20, 100]
+    held = littered(lens, new, nkv, hd, **options)
+    check(2 * randn(sum(new), nh, hd, seed=3), held, lens, new, nh, hd, dtype, dtype == torch.bfloat16, **options)
+
+
+def test_cut_tiles_beside_places_nobody_sees(read_back):
+    lens, new, nh, nkv, hd = [6000, 300], [70, 300], 16, 2, 128
+    options = dict(window=4500)
+    check(2 * randn(sum(new), nh, hd, seed=3), littered(lens, new, nkv, hd, **options), lens, new, nh, hd, torch.bfloat16, True, **options)
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.bfloat16, 96), (torch.float32, 64)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [2, 8, 1]])
+@pytest.mark.parametrize("options", OPTIONS)
+def test_a_few_tokens_beside_places_nobody_sees(dtype, hd, new, options):
+    lens, nh, nkv = [300, 131, 1000], 8, 2
+    held = littered(lens, new, nkv, hd, **options)
+    check(2 * randn(sum(new), nh, hd, seed=3), held, lens, new, nh, hd, dtype, dtype == torch.bfloat16, **options)
