@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(KV8_WARPS * 32) kv8_rows_kernel(const T* __res
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int key = lane + 32 * h;
-        float z = s[h][g] * kf[h] * s_r[g];
+        float z = s[h][g] * (kf[h] * s_r[g]);                        // (up to 2^18 times a power of up to 2^119: the powers go together first)
         if (a.softcap > 0.f) z = a.softcap * tanhf(z / a.softcap);
         s[h][g] = key >= v0 && key < v1 ? z : -INFINITY;
         top = fmaxf(top, s[h][g]);

@@ -1,5 +1,5 @@
-"""Attention over a cache in eight bits where its parts meet: rows that are not finite at the border of a stretch of keys, values at the format's
-smallest powers, places nobody sees, a context that comes back with other lengths.  Bounds as in ``test_gpu_kv8``."""
+"""Attention over a cache in eight bits where its parts meet: rows that are not finite at the border of a stretch of keys, values and keys at the
+format's smallest and largest powers, places nobody sees, a context that comes back with other lengths.  Bounds as in ``test_gpu_kv8``."""
 import importlib
 import math
 
@@ -102,6 +102,17 @@ def test_portions_over_values_at_the_formats_lower_end(over_the_codes, dtype, ex
 def test_single_tokens_over_values_at_the_formats_lower_end(dtype, hd, exponents):
     lens, nh, nkv = [40, 700], 8, 2
     check(2 * randn(2, nh, hd, seed=3), values_of_exponents(lens, nkv, hd, exponents), lens, [1, 1], nh, hd, dtype, dtype == torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 64), (torch.bfloat16, 256), (torch.float32, 128)])
+def test_single_tokens_over_keys_at_the_formats_upper_end(dtype, hd):
+    """Keys of up to 3e38 and queries so small that scores are ordinary: codes times query elements times the power alone would pass float32's range."""
+    lens, nh, nkv = [300, 70], 8, 2
+    ks, vs = ([randn(n, nkv, hd, seed=i + 7 * w) for i, n in enumerate(lens)] for w in (1, 2))
+    for k in ks:
+        k.clamp_(-1, 1).mul_(3e38)
+    scale = hd ** -0.5 * 2.0 ** -31                                # (powers of two beside the queries', which bfloat16 products hold from 2^-99 on)
+    check(randn(2, nh, hd) * 2.0 ** -97, P.Held(ks, vs), lens, [1, 1], nh, hd, dtype, dtype == torch.bfloat16, scale=scale)
 
 
 # ---- a context that comes back
