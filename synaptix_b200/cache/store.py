@@ -121,6 +121,8 @@ class Cache:
             if r is None:
                 return None
             if isinstance(r, KVRequest):
+                if kv_dtype is not None and not r.eight_bit:     # (of every request: equal ones may differ in this)
+                    raise ValueError("kv_dtype='fp8': the model has layers whose keys cannot be held in eight bits")
                 if r not in kv_keys:
                     kv_keys.append(r)
                     kv_counts.append(0)
@@ -140,8 +142,8 @@ class Cache:
 
         for r in requests:
             self._entry.append(place(r))
-        if kv_dtype is not None and not (kv_keys and all(r.eight_bit for r in kv_keys)):
-            raise ValueError("kv_dtype='fp8': the model has " + ("layers whose keys cannot be held in eight bits" if kv_keys else "no keys"))
+        if kv_dtype is not None and not kv_keys:
+            raise ValueError("kv_dtype='fp8': the model has no keys")
         self.kv_groups = kv_keys
         self.state_groups = st_keys
 

@@ -1,7 +1,10 @@
-"""A cache in eight bits, as far as it goes without a GPU: a context that comes back with other lengths."""
+"""A cache in eight bits, as far as it goes without a GPU: a context that comes back with other lengths, refusals."""
+import pytest
 import torch
 
 from synaptix_b200 import ops
+from synaptix_b200.cache import Cache, KVRequest
+from synaptix_b200.cache.store import BundleRequest, StateRequest
 from test_kv8_cpu import step
 
 
@@ -30,3 +33,18 @@ def test_what_is_made_of_a_steps_lengths_is_made_anew_for_others():
     assert [list(x) for x in ops._portions(ctx)] == [[0, 200, 500], [400, 400]]
     ctx.host["seq_past"] = [1, 2]
     assert list(ops._portions(ctx)[1]) == [1, 2]
+
+
+@pytest.mark.parametrize("others_first", [False, True])
+@pytest.mark.parametrize("bundled", [False, True])
+def test_a_request_that_cannot_be_held_in_eight_bits_is_refused_beside_an_equal_one_that_can(others_first, bundled):
+    takes, does_not = KVRequest(2, 64, eight_bit=True), KVRequest(2, 64)
+    state = StateRequest((4,), torch.float32)
+    requests = [takes, BundleRequest((state, BundleRequest((does_not,)))) if bundled else does_not]
+    if others_first:
+        requests.reverse()
+    kw = dict(max_tokens=64, max_seqs=1, dtype=torch.bfloat16, device="cpu")
+    with pytest.raises(ValueError, match="eight bits"):
+        Cache(requests, kv_dtype="fp8", **kw)
+    assert len(Cache(requests, **kw).kv_groups) == 1                  # (in the compute dtype they share a group)
+    assert len(Cache([takes, BundleRequest((state, takes))], kv_dtype="fp8", **kw).kv_groups) == 1
