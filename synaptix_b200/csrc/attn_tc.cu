@@ -183,8 +183,10 @@ enum { FT_B_QFULL = 0, FT_B_KVFULL = 1, FT_B_KVEMPTY = 1 + FT_KV_STAGES, FT_B_SF
        FT_B_PREADY = FT_B_QREADY + 1, FT_B_PVDONE = FT_B_PREADY + 1, FT_B_XCH = FT_B_PVDONE + 1, FT_NBARS = FT_B_XCH + 12 };
 
 // PARTS: block z takes the key blocks z * chunk .. + chunk - 1 of its tile alone and leaves its un-normalised sums with their reference point and
-// denominator in `part` [z][T][nh][FT_PART] (attn_tc_parts_merge_kernel joins them): short portions over long caches have few tiles, and
+// denominator in `part`, rows of FT_PART floats, where row r of tile i has place tile_row[i] + z * (rows of the tile) + r for each head in turn
+// (attn_tc_parts_merge_kernel joins them): short portions over long caches have few tiles, and
 // those of the longest sequence would run long after the others (5 portions of up to 127 tokens over up to 9,000 keys are 160 blocks of 148 SMs).
+// A tile of one part (tile_row[i] < 0) is written as without PARTS and has no place in `part`: beside one long tile a step may have many such.
 #define FT_PART (FT_HD + 4)              // the sums, then reference point (in the exponent's units) and denominator
 template <bool PARTS>
 __global__ void __launch_bounds__(FT_THREADS, 1) attn_tc_prefill_kernel(
@@ -193,7 +195,7 @@ __global__ void __launch_bounds__(FT_THREADS, 1) attn_tc_prefill_kernel(
     const int* __restrict__ tile_q0, const int* __restrict__ cu_seqlens, const int* __restrict__ seq_past,
     const int* __restrict__ seq_lens, const int* __restrict__ block_table, int maxp, int nh, int nkv,
     float scale_log2, int window, const float* __restrict__ sinks, int* __restrict__ status, float* __restrict__ part, int chunk,
-    long long T) {
+    const int* __restrict__ tile_row) {
   extern __shared__ unsigned char ft_smem_raw[];
   unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ft_smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* kv_s = tiles;                                   // [FT_KV_STAGES][K tile, V tile]
@@ -219,6 +221,8 @@ __global__ void __launch_bounds__(FT_THREADS, 1) attn_tc_prefill_kernel(
   const int nb = PARTS ? min(chunk, (last_pos + 1 - kb0 + FT_BN - 1) / FT_BN) : (last_pos + 1 - kb0 + FT_BN - 1) / FT_BN;       // >= 1
   const int* bt = block_table + (size_t)seq * maxp;
   if (PARTS && nb <= 0) return;                                  // (the merge counts a tile's parts as this does)
+  const int place = PARTS ? tile_row[tile] : -1;
+  const bool whole = !PARTS || place < 0;
 
   if (threadIdx.x == 0) {
     ft_mbar_init(bar(FT_B_QFULL), 1);
@@ -336,7 +340,7 @@ __global__ void __launch_bounds__(FT_THREADS, 1) attn_tc_prefill_kernel(
     const uint32_t t_row = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
     const int pos = r < rows ? past + q0 + r : -1;
     float m = -INFINITY, l = 0.f;                                 // l: this thread's columns only
-    if (sinks != nullptr) {                // a sink: a term exp(sink) of the denominator without a key, counted by one half
+    if (sinks != nullptr && whole) {       // a sink: a term exp(sink) of the denominator without a key, counted by one half
       m = sinks[h] * 1.4426950408889634f / scale_log2;
       l = hf == 0 ? 1.f : 0.f;
     }
@@ -449,19 +453,19 @@ __global__ void __launch_bounds__(FT_THREADS, 1) attn_tc_prefill_kernel(
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
       const float inv = l > 0.f ? 1.f / l : 0.f;
       bf16* dst = out + ((size_t)(t_begin + q0 + r) * nh + h) * FT_HD + hf * FT_HALF;
-      float* sums = PARTS ? part + (((size_t)blockIdx.z * T + t_begin + q0 + r) * nh + h) * FT_PART : nullptr;
-      if (PARTS && r < rows && hf == 0) *reinterpret_cast<float2*>(sums + FT_HD) = make_float2(m == -INFINITY ? m : m * scale_log2, l);
+      float* sums = whole ? nullptr : part + (((size_t)place + (size_t)blockIdx.z * rows + r) * nh + h) * FT_PART;
+      if (!whole && r < rows && hf == 0) *reinterpret_cast<float2*>(sums + FT_HD) = make_float2(m == -INFINITY ? m : m * scale_log2, l);
 #pragma unroll 1
       for (int c = 0; c < FT_HALF / 32; ++c) {
         float o[32];
         ft_ld32(t_row + FT_COL_O + hf * FT_HALF + c * 32, o);
         asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-        if (PARTS && r < rows) {
+        if (!whole && r < rows) {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             reinterpret_cast<float4*>(sums + hf * FT_HALF + c * 32)[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         }
-        if (!PARTS && r < rows) {
+        if (whole && r < rows) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint4 v;
@@ -762,22 +766,22 @@ __global__ void __launch_bounds__(FP_THREADS, 1) attn_tc_prefill_pair_kernel(
   }
 }
 
-// A warp a (token, head): its tile's parts joined, a lane four dims.
-__global__ void __launch_bounds__(256) attn_tc_parts_merge_kernel(const float* __restrict__ part, bf16* __restrict__ out, const int* __restrict__ seq_of_token,
+// A warp a (row of a tile, head): the tile's parts joined, a lane four dims.
+__global__ void __launch_bounds__(256) attn_tc_parts_merge_kernel(const float* __restrict__ part, bf16* __restrict__ out, const int* __restrict__ tile_seq,
+                                                                  const int* __restrict__ tile_q0, const int* __restrict__ tile_row,
                                                                   const int* __restrict__ cu_seqlens, const int* __restrict__ seq_past,
-                                                                  int n_tokens, long long T, int nh, int chunk, int window, const float* __restrict__ sinks) {
+                                                                  int nh, int chunk, int window, const float* __restrict__ sinks) {
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31;
-  const long long at = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (at >= (long long)n_tokens * nh) return;
-  const int t = (int)(at / nh), h = (int)(at - (long long)t * nh);
-  const int seq = seq_of_token[t], t_begin = cu_seqlens[seq], n_new = cu_seqlens[seq + 1] - t_begin;
-  const int q0 = (t - t_begin) / FT_BM * FT_BM, first_pos = seq_past[seq] + q0, last_pos = first_pos + min(FT_BM, n_new - q0) - 1;
+  const int lane = threadIdx.x & 31, tile = blockIdx.y, at = (int)blockIdx.x * 8 + (threadIdx.x >> 5), r = at / nh, h = at - r * nh, place = tile_row[tile];
+  if (place < 0) return;
+  const int seq = tile_seq[tile], q0 = tile_q0[tile], t_begin = cu_seqlens[seq], rows = min(FT_BM, cu_seqlens[seq + 1] - t_begin - q0);
+  if (r >= rows) return;
+  const int t = t_begin + q0 + r, first_pos = seq_past[seq] + q0, last_pos = first_pos + rows - 1;
   const int kb0 = (window > 0 ? max(0, first_pos - window + 1) : 0) / FT_BN * FT_BN;
   const int parts = ((last_pos + 1 - kb0 + FT_BN - 1) / FT_BN + chunk - 1) / chunk;
-  const float* src = part + ((size_t)t * nh + h) * FT_PART;
-  const size_t step = (size_t)T * nh * FT_PART;
+  const float* src = part + (((size_t)place + r) * nh + h) * FT_PART;
+  const size_t step = (size_t)rows * nh * FT_PART;
   float top = sinks ? sinks[h] * 1.4426950408889634f : -INFINITY, L = sinks ? 1.f : 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int z = 0; z < parts; z += 4) {
@@ -895,13 +899,13 @@ extern "C" int sx_attn_prefill_tc(const void* q, const void* k_pages, const void
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
   return sx_launch(kern, dim3(nh, n_tiles), dim3(FT_THREADS), smem, stream, mq, mk, mv, (bf16*)out, tile_seq, tile_q0,
-                   cu_seqlens, seq_past, seq_lens, block_table, maxp, nh, nkv, scale * 1.4426950408889634f, window, sinks, status, (float*)nullptr, 0, T);
+                   cu_seqlens, seq_past, seq_lens, block_table, maxp, nh, nkv, scale * 1.4426950408889634f, window, sinks, status, (float*)nullptr, 0, (const int*)nullptr);
 }
 
-// The same with a tile's keys cut into `parts` (or fewer) stretches of `chunk` blocks of 128 keys: no tile has more than parts * chunk.  `part` holds
-// parts * T * nh * 132 floats.  seq_of_token [T] names each token's sequence.
+// The same with a tile's keys cut into `parts` (or fewer) stretches of `chunk` blocks of 128 keys: no tile has more than parts * chunk.  tile_row [n_tiles]:
+// where in `part`, rows of nh * 132 floats, a tile's sums begin (rows of the tile * its stretches), -1 for tiles of one stretch.
 extern "C" int sx_attn_prefill_tc_parts(const void* q, const void* k_pages, const void* v_pages, void* out, float* part, long long T,
-                                        long long n_pages, const int* tile_seq, const int* tile_q0, int n_tiles, const int* seq_of_token,
+                                        long long n_pages, const int* tile_seq, const int* tile_q0, const int* tile_row, int n_tiles,
                                         const int* cu_seqlens, const int* seq_past, const int* seq_lens, const int* block_table,
                                         int maxp, int nh, int nkv, int hd, float scale, int window, const float* sinks, int chunk, int parts,
                                         cudaStream_t stream) {
@@ -921,10 +925,10 @@ extern "C" int sx_attn_prefill_tc_parts(const void* q, const void* k_pages, cons
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
   rc = sx_launch(kern, dim3(nh, n_tiles, parts), dim3(FT_THREADS), smem, stream, mq, mk, mv, (bf16*)out, tile_seq, tile_q0, cu_seqlens, seq_past, seq_lens,
-                 block_table, maxp, nh, nkv, scale * 1.4426950408889634f, window, (const float*)nullptr, status, part, chunk, T);
+                 block_table, maxp, nh, nkv, scale * 1.4426950408889634f, window, sinks, status, part, chunk, tile_row);
   if (rc) return rc;
-  return sx_launch(attn_tc_parts_merge_kernel, dim3((unsigned)((T * nh + 7) / 8)), dim3(256), 0, stream, (const float*)part, (bf16*)out, seq_of_token, cu_seqlens,
-                   seq_past, (int)T, T, nh, chunk, window, sinks);
+  return sx_launch(attn_tc_parts_merge_kernel, dim3((unsigned)(FT_BM * nh / 8), n_tiles), dim3(256), 0, stream, (const float*)part, (bf16*)out, tile_seq, tile_q0,
+                   tile_row, cu_seqlens, seq_past, nh, chunk, window, sinks);
 }
 
 // 0, or which bounded wait ran out (1 producer, 2-5 MMA issuer, 6-9 softmax)

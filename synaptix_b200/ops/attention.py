@@ -319,15 +319,17 @@ TC_KEY_BLOCK = 128
 _TC_BLOCK_US, _TC_START_US = 1.27, 4.5       # what a block of attn_tc takes for 128 keys, and beside them
 
 
+def _key_blocks(tiles, window: Optional[int]):
+    """Of each tile, (first position, last position): how many blocks of 128 keys its rows see."""
+    return [last // TC_KEY_BLOCK + 1 - (max(0, first - window + 1) // TC_KEY_BLOCK if window else 0) for first, last in tiles]
+
+
 def tc_parts(tiles, nh: int, window: Optional[int], device) -> Tuple[int, int]:
     """``(blocks of 128 keys a part, parts of the longest tile)`` where the tiles' keys are better cut into parts, else ``(0, 1)``.  ``tiles``:
     (first position, last position) of each 128-row tile.  A way to cut takes its work dealt out evenly and half a block more, at least as long as its longest
     block, and some 6 us to join.  Measured, 5 portions of 85 to 127 tokens over 6,000 to
     9,000 keys, 32 heads: whole tiles (160 blocks on 148 SMs) 151 us, cut 126."""
-    counts = []
-    for first, last in tiles:
-        lo = max(0, first - window + 1) // TC_KEY_BLOCK if window else 0
-        counts.append(last // TC_KEY_BLOCK + 1 - lo)
+    counts = _key_blocks(tiles, window)
     sms = sm_count(device)
     most, total = max(counts), sum(counts) * nh
 
@@ -345,22 +347,35 @@ def tc_parts(tiles, nh: int, window: Optional[int], device) -> Tuple[int, int]:
     return (cut, -(-most // cut)) if cut else (0, 1)
 
 
+def tc_part_rows(tiles, chunk: int, window: Optional[int]):
+    """Where the sums of each tile begin among those of all tiles cut into stretches of ``chunk`` blocks of 128 keys, in rows (-1: a tile of one stretch,
+    which keeps none), and how many rows there are."""
+    places, total = [], 0
+    for (first, last), blocks in zip(tiles, _key_blocks(tiles, window)):
+        parts = -(-blocks // chunk)
+        places.append(total if parts > 1 else -1)
+        total += parts * (last - first + 1) if parts > 1 else 0
+    return places, total
+
+
 def attn_prefill_tc_parts(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tile_seq: torch.Tensor, tile_q0: torch.Tensor,
-                          seq_of_token: torch.Tensor, cu_seqlens: torch.Tensor, seq_past: torch.Tensor, seq_lens: torch.Tensor,
+                          tile_row: torch.Tensor, part_rows: int, cu_seqlens: torch.Tensor, seq_past: torch.Tensor, seq_lens: torch.Tensor,
                           block_table: torch.Tensor, nh: int, nkv: int, hd: int, scale: float, window: Optional[int], chunk: int, parts: int,
                           sinks: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``attn_prefill_tc`` with every tile's keys cut into stretches of ``chunk`` blocks of 128, ``parts`` for the longest tile (``tc_parts``), which
-    blocks of their own take and a second kernel joins."""
-    require_cuda(q, k_pages, v_pages, tile_seq, tile_q0, seq_of_token, cu_seqlens, seq_past, seq_lens, block_table, sinks)
+    blocks of their own take and a second kernel joins; ``tile_row`` and ``part_rows`` are what ``tc_part_rows`` gives."""
+    require_cuda(q, k_pages, v_pages, tile_seq, tile_q0, tile_row, cu_seqlens, seq_past, seq_lens, block_table, sinks)
     _check_sinks(sinks, nh)
     T = q.shape[0]
     if not tc_prefill_supported(q.dtype, nh, nkv, hd) or k_pages.dtype != q.dtype:
         raise KernelError("attn_prefill_tc: bfloat16 and head size 128")
+    if tile_row.dtype != torch.int32 or tile_row.numel() != tile_seq.numel() or not 0 <= part_rows < 1 << 31:
+        raise KernelError("attn_prefill_tc_parts: a first row per tile (int32)")
     out = torch.empty((T, nh * hd), dtype=q.dtype, device=q.device)
-    part = torch.empty(parts * T * nh * (hd + 4), dtype=torch.float32, device=q.device)
+    part = torch.empty(part_rows * nh * (hd + 4), dtype=torch.float32, device=q.device)
     check(launcher("attn_tc", "sx_attn_prefill_tc_parts")(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), part.data_ptr(), T, k_pages.shape[0], tile_seq.data_ptr(),
-        tile_q0.data_ptr(), tile_seq.numel(), seq_of_token.data_ptr(), cu_seqlens.data_ptr(), seq_past.data_ptr(), seq_lens.data_ptr(),
+        tile_q0.data_ptr(), tile_row.data_ptr(), tile_seq.numel(), cu_seqlens.data_ptr(), seq_past.data_ptr(), seq_lens.data_ptr(),
         block_table.data_ptr(), block_table.shape[1], nh, nkv, hd, scale, 0 if window is None else int(window),
         None if sinks is None else sinks.data_ptr(), chunk, parts, raw_stream()), "attn_prefill_tc_parts", launches=2)
     return out

@@ -412,18 +412,21 @@ def kv8_attention(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tens
         return kv8_tile(q, pages, ctx, block_table, nh, scale, window, softcap=softcap, sinks=sinks, chunk=chunk, out=out, out_col=out_col,
                         out_scale=out_scale)
     from . import TC_TILE_ROWS, _query_tiles, attention, tc_prefill_supported
-    from .attention import attn_prefill_tc_parts, tc_parts
+    from .attention import attn_prefill_tc_parts, tc_part_rows, tc_parts
     _check_device("kv8_attention", q, *pages, ctx.seq_lens, block_table, sinks, out)
     k, v, table = _read(pages, ctx, block_table, q.dtype, window, chunk, True)
     if out is None and softcap is None and chunk is None and out_scale == 1.0 and tc_prefill_supported(q.dtype, nh, nkv, hd):
         cu, past = ctx.host["cu_seqlens"], ctx.host["seq_past"]
         cut = ctx.scratch.get(("kv8_parts", nh, window))
-        if cut is None or cut[2] != cu or cut[3] != past:
+        if cut is None or cut[4] != cu or cut[5] != past:
             tiles = [(p + q0, min(p + q0 + TC_TILE_ROWS, p + b - a) - 1) for a, b, p in zip(cu, cu[1:], past) for q0 in range(0, b - a, TC_TILE_ROWS)]
-            cut = ctx.scratch[("kv8_parts", nh, window)] = tc_parts(tiles, nh, window, q.device) + (list(cu), list(past))
+            chunk, parts = tc_parts(tiles, nh, window, q.device)
+            places, rows = tc_part_rows(tiles, chunk, window) if parts > 1 else ([], 0)
+            places = torch.from_numpy(np.asarray(places, dtype=np.int32)).to(q.device, non_blocking=True)
+            cut = ctx.scratch[("kv8_parts", nh, window)] = (chunk, parts, places, rows, list(cu), list(past))
         if cut[1] > 1:
             tile_seq, tile_q0 = _query_tiles(ctx, TC_TILE_ROWS, q.device)
-            return attn_prefill_tc_parts(q, k, v, tile_seq, tile_q0, ctx.seq_of_token, ctx.cu_seqlens, ctx.seq_past, ctx.seq_lens, table, nh, nkv, hd,
+            return attn_prefill_tc_parts(q, k, v, tile_seq, tile_q0, cut[2], cut[3], ctx.cu_seqlens, ctx.seq_past, ctx.seq_lens, table, nh, nkv, hd,
                                          scale, window, cut[0], cut[1], sinks=sinks)
     return attention(q, k, v, ctx, table, nh, nkv, hd, scale, window, softcap=softcap, sinks=sinks, chunk=chunk, out=out, out_col=out_col,
                      out_scale=out_scale)

@@ -70,6 +70,32 @@ def test_rows_that_are_not_finite_in_short_stretches(monkeypatch, window):
     assert torch.equal(res[0][~bad], res[1][~bad]) and not res[0].isnan().any()
 
 
+@pytest.mark.parametrize("sinks", [False, True])
+def test_a_long_tile_among_many_short_ones_takes_no_room_for_them(sinks):
+    """64 tokens behind 12,000 keys are cut; the 20 prompts beside them are not, and need no room for stretches."""
+    from synaptix_b200 import ops
+    lens, new, nh, nkv, hd = [12064] + [300] * 20, [64] + [300] * 20, 16, 2, 128
+    held, q, s = filled(lens, nkv, hd), (2 * randn(sum(new), nh, hd, seed=3)).bfloat16(), randn(nh, seed=9) if sinks else None
+    ctx, pages, table, x = on_gpu(step(lens, new)), held.pages(), held.table.cuda(), q.view(q.shape[0], -1).cuda()
+    sink = None if s is None else s.cuda()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = ops.kv8_attention(x, pages, ctx, table, nh, nkv, hd, 0.1, sinks=sink)
+    torch.cuda.synchronize()
+    cut = ctx.scratch[("kv8_parts", nh, None)]
+    assert cut[1] > 1
+    read = 2 * sum(-(-n // 64) for n in lens) * nkv * 64 * hd * 2
+    sums = cut[1] * 64 * nh * (hd + 4) * 4
+    assert torch.cuda.max_memory_allocated() - before <= read + got.numel() * 2 + sums + (1 << 20)
+    for i in (0, 1, 20):
+        at = sum(new[:i])
+        part, n, m = slice(at, at + new[i]), lens[i], new[i]
+        want, weight = P.attend(q[part], held.keys[i], held.values[i], torch.arange(n - m, n), 0.1, sinks=s)
+        tol = bound(q[part], held, i, want, weight, None, 0.1, torch.bfloat16, hd, True, portions=True)
+        assert ((got[part].cpu().double() - want).abs() <= tol).all(), i
+
+
 # ---- the format's ends
 
 def values_of_exponents(lens, nkv, hd, exponents, seed=0):

@@ -1,4 +1,4 @@
-"""A cache in eight bits, as far as it goes without a GPU: a context that comes back with other lengths, refusals."""
+"""A cache in eight bits, as far as it goes without a GPU: a context that comes back with other lengths, refusals, room for cut tiles."""
 import pytest
 import torch
 
@@ -48,3 +48,14 @@ def test_a_request_that_cannot_be_held_in_eight_bits_is_refused_beside_an_equal_
         Cache(requests, kv_dtype="fp8", **kw)
     assert len(Cache(requests, **kw).kv_groups) == 1                  # (in the compute dtype they share a group)
     assert len(Cache([takes, BundleRequest((state, takes))], kv_dtype="fp8", **kw).kv_groups) == 1
+
+
+def test_places_of_cut_tiles():
+    from synaptix_b200.ops.attention import tc_part_rows
+    tiles = [(0, 99), (100000, 100063), (0, 127), (128, 128), (5000, 5009), (700, 827)]
+    assert tc_part_rows(tiles, 261, None) == ([-1, 0, -1, -1, -1, -1], 3 * 64)                # 782 blocks in three
+    assert tc_part_rows(tiles, 2, None) == ([-1, 0, -1, -1, 391 * 64, 391 * 64 + 20 * 10],
+                                            391 * 64 + 20 * 10 + 4 * 128)
+    # a window of 200: keys 99,801 to 100,063 are blocks 779 to 781; 4,801 to 5,009 37 to 39; 501 to 827 3 to 6
+    assert tc_part_rows(tiles, 2, 200) == ([-1, 0, -1, -1, 2 * 64, 2 * 64 + 2 * 10], 2 * 64 + 2 * 10 + 2 * 128)
+    assert tc_part_rows([], 1, None) == ([], 0)
