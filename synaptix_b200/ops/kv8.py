@@ -420,10 +420,12 @@ def kv8_attention(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tens
         cut = ctx.scratch.get(("kv8_parts", nh, window))
         if cut is None or cut[4] != cu or cut[5] != past:
             tiles = [(p + q0, min(p + q0 + TC_TILE_ROWS, p + b - a) - 1) for a, b, p in zip(cu, cu[1:], past) for q0 in range(0, b - a, TC_TILE_ROWS)]
-            chunk, parts = tc_parts(tiles, nh, window, q.device)
-            places, rows = tc_part_rows(tiles, chunk, window) if parts > 1 else ([], 0)
-            places = torch.from_numpy(np.asarray(places, dtype=np.int32)).to(q.device, non_blocking=True)
-            cut = ctx.scratch[("kv8_parts", nh, window)] = (chunk, parts, places, rows, list(cu), list(past))
+            blocks, parts = tc_parts(tiles, nh, window, q.device)
+            places = rows = None
+            if parts > 1:
+                places, rows = tc_part_rows(tiles, blocks, window)
+                places = torch.from_numpy(np.asarray(places, dtype=np.int32)).to(q.device, non_blocking=True)
+            cut = ctx.scratch[("kv8_parts", nh, window)] = (blocks, parts, places, rows, list(cu), list(past))
         if cut[1] > 1:
             tile_seq, tile_q0 = _query_tiles(ctx, TC_TILE_ROWS, q.device)
             return attn_prefill_tc_parts(q, k, v, tile_seq, tile_q0, cut[2], cut[3], ctx.cu_seqlens, ctx.seq_past, ctx.seq_lens, table, nh, nkv, hd,

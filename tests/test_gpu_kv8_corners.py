@@ -19,6 +19,15 @@ def attend(q, held, ctx, nh, nkv, hd, scale, window=None, **kw):
     return ops.kv8_attention(q.view(q.shape[0], -1).cuda(), held.pages(), on_gpu(ctx), held.table.cuda(), nh, nkv, hd, scale, window, **kw).cpu().view(-1, nh, hd)
 
 
+@pytest.fixture
+def read_back(monkeypatch):
+    """All portions go through pages read back, whatever is faster."""
+    from synaptix_b200.ops import kv8
+    monkeypatch.setattr(kv8, "FEW_NEW_TOKENS", 0)
+    for name in ("TILE_BF16_ROWS", "TILE_BF16_PAGES"):
+        monkeypatch.setattr(kv8, name, {64: 0, 128: 0})
+
+
 # ---- cut tiles (csrc/attn_tc.cu)
 
 @pytest.mark.parametrize("what", ["key", "value"])
@@ -94,6 +103,20 @@ def test_a_long_tile_among_many_short_ones_takes_no_room_for_them(sinks):
         want, weight = P.attend(q[part], held.keys[i], held.values[i], torch.arange(n - m, n), 0.1, sinks=s)
         tol = bound(q[part], held, i, want, weight, None, 0.1, torch.bfloat16, hd, True, portions=True)
         assert ((got[part].cpu().double() - want).abs() <= tol).all(), i
+
+
+@pytest.mark.parametrize("new", [[700], [300, 400]])
+@pytest.mark.parametrize("nh,nkv,hd", [(32, 8, 128), (64, 8, 64)])
+def test_the_first_layer_of_a_step_takes_the_kernel_that_the_others_take(read_back, new, nh, nkv, hd):
+    """What the first call makes for its context changes nothing but the time: the same bits from all calls, and those of the kernel itself."""
+    from synaptix_b200 import ops
+    held, q, ctx = filled(new, nkv, hd), (2 * randn(sum(new), nh, hd, seed=3)).bfloat16(), step(new, new)
+    first, second = (attend(q, held, ctx, nh, nkv, hd, 0.1) for _ in range(2))
+    k, v, table = ops.kv8_read(held.pages(), ctx, held.table.cuda(), torch.bfloat16)
+    tiles = ops._query_tiles(ctx, 128 if hd == 128 else 64, k.device)
+    whole = (ops.attn_prefill_tc if hd == 128 else ops.attn_prefill)(q.view(sum(new), -1).cuda(), k, v, *tiles, ctx.cu_seqlens, ctx.seq_past, ctx.seq_lens, table,
+                                                                     nh, nkv, hd, 0.1, None)
+    assert torch.equal(first, second) and torch.equal(first, whole.cpu().view(first.shape))
 
 
 # ---- the format's ends
@@ -187,15 +210,6 @@ def littered(lens, new, nkv, hd, window=None, chunk=None, seed=0):
             held.v[page, :, ::3, r] = 0x7f if j % 2 else 0xff
             held.v_exp[page, :, r] = 100 + (j * 7) % 155
     return held
-
-
-@pytest.fixture
-def read_back(monkeypatch):
-    """All portions go through pages read back, whatever is faster."""
-    from synaptix_b200.ops import kv8
-    monkeypatch.setattr(kv8, "FEW_NEW_TOKENS", 0)
-    for name in ("TILE_BF16_ROWS", "TILE_BF16_PAGES"):
-        monkeypatch.setattr(kv8, name, {64: 0, 128: 0})
 
 
 OPTIONS = [{}, dict(window=50), dict(window=64), dict(window=200, chunk=96)]
