@@ -404,13 +404,13 @@ extern "C" int sx_kv8_prepare(const void* qkv, void* q_out, void* k_pages, void*
 // row, by their scores, and to no others (a weight of zero times NaN would).
 // Eight sequences of 4,969 to 12,000 tokens, 8 heads of 128, to bfloat16: 70 to 73 us for 411 MB moved, 5.6 to 5.8 TB/s: HBM, nine tenths of a plain copy's rate.
 // ---------------------------------------------------------------------------------------
-template <typename T> __device__ __forceinline__ void kv8_store8(T* dst, const uint32_t (&pairs)[4], float f, bool held) {
+template <typename T> __device__ __forceinline__ void kv8_store8(T* dst, const uint32_t (&pairs)[4], float f) {
   float x[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 v = kv8_float2(pairs[i]);
-    x[2 * i] = held ? v.x * f : 0.f;
-    x[2 * i + 1] = held ? v.y * f : 0.f;
+    x[2 * i] = f != 0.f ? v.x * f : 0.f;
+    x[2 * i + 1] = f != 0.f ? v.y * f : 0.f;
   }
   Kv8Vec<T>::store8(dst, x);
 }
@@ -454,15 +454,15 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(
   }
   if (threadIdx.x < 2 * SX_PAGE) {
     const int key = threadIdx.x & (SX_PAGE - 1), ve = v_exp[from * SX_PAGE + key];
-    const bool gone = page_from && ve == KV8_NAN;
-    if (threadIdx.x < SX_PAGE) s_k[key] = kv8_scale(gone ? KV8_NAN : k_exp[from * SX_PAGE + key]);
-    else s_v[key] = gone ? 0.f : kv8_scale(ve);
+    const bool there = key < held && key >= from_key, gone = page_from && ve == KV8_NAN;      // (a factor of zero: zeros, whatever the codes are)
+    if (threadIdx.x < SX_PAGE) s_k[key] = there ? kv8_scale(gone ? KV8_NAN : k_exp[from * SX_PAGE + key]) : 0.f;
+    else s_v[key] = there && !gone ? kv8_scale(ve) : 0.f;
   }
   __syncthreads();
   auto put_k = [&](int o, const uint2 w) {
     const int key = o / groups, d = o % groups * 8;
     const uint32_t pairs[4] = {w.x, w.x >> 16, w.y, w.y >> 16};
-    kv8_store8<T>(k_out + to + key * hd + d, pairs, s_k[key], key < held && key >= from_key);
+    kv8_store8<T>(k_out + to + key * hd + d, pairs, s_k[key]);
   };
   auto put_v = [&](int o, const uint32_t (&w)[8]) {
     const int key = v_key(o), group = v_group(o);
@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(
       uint32_t pairs[4];
 #pragma unroll
       for (int d = 0; d < 4; ++d) pairs[d] = __byte_perm(w[2 * d], w[2 * d + 1], n | (4 + n) << 4);
-      kv8_store8<T>(v_out + to + (key + n) * hd + group * 8, pairs, s_v[key + n], key + n < held && key + n >= from_key && s_v[key + n] != 0.f);
+      kv8_store8<T>(v_out + to + (key + n) * hd + group * 8, pairs, s_v[key + n]);
     }
   };
   if constexpr (HD != 0) {
