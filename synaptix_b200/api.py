@@ -25,7 +25,9 @@ class LLM:
     ``max_tokens = max_batch * max_seq``.
 
     ``kv_dtype="fp8"`` holds keys and values in eight bits (e4m3 codes and a power of two per head and token): half the cache of
-    bfloat16, and half the bytes that a step reads of it.  Models whose keys belong to other mixers than ``Attention`` refuse it.
+    bfloat16, and half the bytes that a step reads of it; steps of one sequence and short prompts run slower than with bfloat16.  Prompt portions that are read
+    back (``ops.kv8_attention``) hold their sequences' keys and values of one layer in the compute dtype beside it while they attend.  Models whose keys belong to
+    other mixers than ``Attention`` refuse it.
     """
 
     def __init__(self, model_dir: str, compute_dtype="bf16", device: str = "cuda:0",

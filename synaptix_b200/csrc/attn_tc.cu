@@ -9,7 +9,9 @@
 //              halves meet through shared memory), writes P = 2^(s*c - m*c) as packed bfloat16 back
 //              into tensor memory over the scores it has read (tcgen05.st), rescales its half row of O
 //              when the reference point m moved, and at the end writes O / l.  m moves lazily (only
-//              when the maximum grew by more than 2^8), which spares most rescalings.  At the start
+//              when the maximum grew by more than 2^8), which spares most rescalings.  (P is rounded to
+//              bfloat16 because both operands of a product have one type and V is bfloat16: half a step is
+//              2^-8 of a weight, where results are rounded by as much; l sums the weights as they are.)  At the start
 //              the same threads copy the Q tile from shared memory into tensor memory
 // Both products take their A operand (Q, P) from tensor memory, so an MMA reads only its B operand
 // (K, V) from shared memory: with A in shared memory as well, a 128 x 128 x 16 MMA needs all of the

@@ -365,11 +365,17 @@ def kv8_attention(q: torch.Tensor, pages: KV8Pages, ctx, block_table: torch.Tens
     """Causal attention of the step's packed queries ``q [T, nh * hd]`` over a cache in eight bits that already holds the step's
     keys and values: ``[T, nh * hd]`` in ``q``'s dtype.  The options are those of ``ops.attention``.
 
-    ``q`` has a row for every token of the step; places of the cache that the step's tokens do not see may hold anything.
+    ``q`` has a row for every token of the step; places of the cache that the step's tokens do not see may hold anything.  Kernels on the codes load
+    queries 16 bytes at a time and refuse a ``q`` that does not begin at a multiple of 16.
+
+    A bfloat16 query goes into the products over the codes as two e4m3 numbers: elements down to 2^-9 of the row's largest are exact, smaller ones off by at most
+    2^-18 of it; rows whose largest magnitude is below 2^-99 lose more.  Weights are rounded to half precision there, to bfloat16 by the 16-bit cache's
+    kernels (denominators sum them as they are), and kept to 22 bits in float32.  Results are divided at the end: values times the number of keys seen stay below 2^127.
 
     Single tokens, portions of a few tokens and float32 portions attend over the codes.  Longer portions read the pages back once
     (``kv8_read``) and attend over the result with the kernels of the 16- and 32-bit cache: a page serves many rows there, and
-    turning its codes again in every block that reads it would cost more than writing it out once."""
+    turning its codes again in every block that reads it would cost more than writing it out once.  What is read back takes ``2 nkv hd`` elements of ``q``'s
+    dtype a token of the step's sequences (131,072 tokens of 8 heads of 128 in bfloat16: 537 MB) until the call's kernels are done."""
     _check_pages(pages, "kv8_attention", nkv, hd)
     seq_lens = ctx.seq_lens
     if seq_lens.dtype is not torch.int32 or block_table.dtype is not torch.int32:
